@@ -20,8 +20,10 @@ import warnings
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libflashfwd_b200.so")
 
-FA_OK, FA_INVALID_ARG, FA_UNSUPPORTED, FA_CUDA_ERROR, FA_DEVICE_TIMEOUT = range(5)
-STATUS_NAMES = {0: "FA_OK", 1: "FA_INVALID_ARG", 2: "FA_UNSUPPORTED", 3: "FA_CUDA_ERROR", 4: "FA_DEVICE_TIMEOUT"}
+FA_OK, FA_INVALID_ARG, FA_UNSUPPORTED, FA_CUDA_ERROR, FA_DEVICE_TIMEOUT, FA_BAD_INDEX = range(6)
+STATUS_NAMES = {0: "FA_OK", 1: "FA_INVALID_ARG", 2: "FA_UNSUPPORTED", 3: "FA_CUDA_ERROR", 4: "FA_DEVICE_TIMEOUT",
+                5: "FA_BAD_INDEX"}
+FA_FP16, FA_BF16 = range(2)
 
 # every symbol include/flash_forward_b200.h declares
 EXPORTS = (
@@ -43,7 +45,23 @@ EXPORTS = (
     "flash_forward_kv_range",
     "flash_forward_head_group",
     "flash_forward_shutdown",
+    "flash_cache_append",
+    "flash_decode",
+    "flash_decode_workspace_bytes",
 )
+
+
+class PagedCacheStruct(ctypes.Structure):  # fa_paged_cache
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("page_stride", ctypes.c_longlong),
+                ("head_stride", ctypes.c_longlong), ("token_stride", ctypes.c_longlong), ("num_pages", ctypes.c_int),
+                ("page_size", ctypes.c_int), ("kv_heads", ctypes.c_int), ("head_dim", ctypes.c_int),
+                ("dtype", ctypes.c_int), ("page_table", ctypes.c_void_p), ("table_stride", ctypes.c_longlong),
+                ("max_pages", ctypes.c_int), ("lengths", ctypes.c_void_p), ("counts", ctypes.c_void_p)]
+
+
+class RowsStruct(ctypes.Structure):  # fa_rows
+    _fields_ = [("data", ctypes.c_void_p), ("batch_stride", ctypes.c_longlong), ("head_stride", ctypes.c_longlong),
+                ("token_stride", ctypes.c_longlong)]
 
 _lock = threading.RLock()  # around the first load of either
 _lib = None
@@ -111,6 +129,13 @@ def _open():
     L.flash_forward_head_group.restype = i
     L.flash_forward_shutdown.argtypes = []
     L.flash_forward_shutdown.restype = i
+    cache, rows = ctypes.POINTER(PagedCacheStruct), ctypes.POINTER(RowsStruct)
+    L.flash_cache_append.argtypes = [cache, rows, rows, rows, vp, i, i, i, vp, i, i, i, vp]
+    L.flash_cache_append.restype = i
+    L.flash_decode.argtypes = [cache, rows, vp, vp, i, i, i, f, i, vp, vp, ctypes.c_size_t, vp]
+    L.flash_decode.restype = i
+    L.flash_decode_workspace_bytes.argtypes = [i, i, i, i]
+    L.flash_decode_workspace_bytes.restype = ctypes.c_size_t
     return L
 
 
@@ -325,4 +350,125 @@ def _enqueue_forward(device, torch, q, k, v, out, causal, window_left, window_ri
                                 int(bool(causal)), window_left, window_right, stream, kernel, variant, None)
     if rc != FA_OK:
         _raise(rc)
+    return (out, lse) if return_lse else out
+
+
+def _check_cache(torch, k_pages, v_pages, page_table, lengths, counts, batch):
+    """What the kernels get the address of; the pages' own contents are the caller's."""
+    def ints(t, shape):
+        return t.is_cuda and t.get_device() == device and t.dtype == torch.int32 and tuple(t.shape) == shape
+    if not (k_pages.is_cuda and k_pages.dim() == 4 and k_pages.dtype in (torch.float16, torch.bfloat16) and
+            k_pages.stride(3) == 1):
+        raise AssertionError("k_pages: an fp16 or bf16 CUDA tensor [num_pages, kv_heads, page_size, head_dim] with "
+                             "head_dim contiguous is needed")
+    device = k_pages.get_device()
+    if not (v_pages.is_cuda and v_pages.get_device() == device and v_pages.dtype == k_pages.dtype and
+            v_pages.shape == k_pages.shape and v_pages.stride() == k_pages.stride()):
+        raise AssertionError("v_pages has to be like k_pages, strides included, on its device")
+    if not (page_table.dim() == 2 and ints(page_table, (batch, page_table.shape[1])) and page_table.stride(1) == 1):
+        raise AssertionError("page_table: int32 [batch, max_pages] on the cache's device, rows contiguous, is needed")
+    if not (ints(lengths, (batch,)) and lengths.is_contiguous()):
+        raise AssertionError("lengths: contiguous int32 [batch] on the cache's device is needed")
+    if counts is not None and not (ints(counts, (batch,)) and counts.is_contiguous()):
+        raise AssertionError("counts: contiguous int32 [batch] on the cache's device is needed")
+    return device
+
+
+def _cache_struct(torch, k_pages, v_pages, page_table, lengths, counts):
+    num_pages, kv_heads, page_size, head_dim = k_pages.shape
+    return PagedCacheStruct(k_pages.data_ptr(), v_pages.data_ptr(), *k_pages.stride()[:3], num_pages, page_size, kv_heads,
+                            head_dim, FA_FP16 if k_pages.dtype == torch.float16 else FA_BF16, page_table.data_ptr(),
+                            page_table.stride(0), page_table.shape[1], lengths.data_ptr(),
+                            None if counts is None else counts.data_ptr())
+
+
+def _rows_struct(name, x, k_pages, heads, batch, tokens):
+    if not (x.is_cuda and x.get_device() == k_pages.get_device() and x.dtype == k_pages.dtype and x.dim() == 4 and
+            tuple(x.shape) == (batch, heads, tokens, k_pages.shape[3]) and x.stride(3) == 1):
+        raise AssertionError(f"{name}: [batch, heads, tokens, head_dim] like the cache, with head_dim contiguous, is needed")
+    return RowsStruct(x.data_ptr(), *x.stride()[:3])
+
+
+def _on_device(torch, device, call, *args):
+    """call(*args, stream) with `device` current and the stream that is current there."""
+    if device == torch.cuda.current_device():
+        rc = call(*args, _current_raw_stream(torch, device))
+    else:
+        with torch.cuda.device(device):
+            rc = call(*args, _current_raw_stream(torch, device))
+    if rc != FA_OK:
+        _raise(rc)
+
+
+def cache_append(k, v, k_pages, v_pages, page_table, lengths, counts=None, q=None, rotary=None, interleaved=False,
+                 q_out=None):
+    """Writes new keys and values into a paged cache (flash_cache_append of the C header, which says what it does).
+
+    k, v: [batch, kv_heads, tokens, head_dim], any strides with head_dim contiguous. k_pages, v_pages: [num_pages, kv_heads,
+    page_size, head_dim], likewise (pages that hold [token][head] are passed as their transposed view). page_table: int32
+    [batch, max_pages]. lengths: int32 [batch], the sequences' tokens with the new ones; counts: int32 [batch], the new
+    tokens of each, where rows behind them are padding. rotary: float32 [positions, rotary_dim], cosines and sines: keys,
+    and the queries q [batch, q_heads, tokens, head_dim], are rotated. Returns the rotated queries (q_out, contiguous, if
+    given), or None without q.
+    """
+    import torch
+
+    batch, kv_heads, tokens = k.shape[:3] if k.dim() == 4 else (0, 0, 0)
+    device = _check_cache(torch, k_pages, v_pages, page_table, lengths, counts, batch)
+    if kv_heads != k_pages.shape[1]:
+        raise AssertionError("k and v need the heads of the cache")
+    ks, vs = (_rows_struct(n, x, k_pages, kv_heads, batch, tokens) for n, x in (("k", k), ("v", v)))
+    if rotary is not None and not (rotary.is_cuda and rotary.get_device() == device and rotary.dtype == torch.float32 and
+                                   rotary.dim() == 2 and rotary.is_contiguous()):
+        raise AssertionError("rotary: contiguous float32 [positions, rotary_dim] on the cache's device is needed")
+    qs, q_heads = None, 0
+    if q is not None:
+        q_heads = q.shape[1] if q.dim() == 4 else 0
+        qs = _rows_struct("q", q, k_pages, q_heads, batch, tokens)
+        shape = (batch, q_heads, tokens, k_pages.shape[3])
+        if q_out is None:
+            q_out = torch.empty(shape, device=q.device, dtype=q.dtype)
+        elif not (q_out.is_cuda and q_out.get_device() == device and q_out.dtype == q.dtype and
+                  tuple(q_out.shape) == shape and q_out.is_contiguous()):
+            raise AssertionError("q_out: a contiguous tensor like q is needed")
+    elif q_out is not None:
+        raise AssertionError("q_out needs q")
+    cache = _cache_struct(torch, k_pages, v_pages, page_table, lengths, counts)
+    _on_device(torch, device, lib().flash_cache_append, cache, ks, vs, qs, None if q is None else q_out.data_ptr(), batch,
+               tokens, q_heads, None if rotary is None else rotary.data_ptr(), 0 if rotary is None else rotary.shape[1],
+               0 if rotary is None else rotary.shape[0], int(bool(interleaved)))
+    return q_out
+
+
+def attention_decode(q, k_pages, v_pages, page_table, lengths, counts=None, softmax_scale=0.0, window_left=-1,
+                     alibi_slopes=None, return_lse=False, out=None):
+    """Attention of the newest tokens of every sequence over a paged cache (flash_decode of the C header).
+
+    q: [batch, q_heads, tokens, head_dim], any strides with head_dim contiguous, q_heads a multiple of the cache's heads;
+    the cache as for cache_append, after it. Returns the output, contiguous and shaped like q (`out` if given), and with
+    return_lse also float32 [batch, q_heads, tokens].
+    """
+    import torch
+
+    batch, q_heads, tokens = q.shape[:3] if q.dim() == 4 else (0, 0, 0)
+    device = _check_cache(torch, k_pages, v_pages, page_table, lengths, counts, batch)
+    qs = _rows_struct("q", q, k_pages, q_heads, batch, tokens)
+    if alibi_slopes is not None and not (alibi_slopes.is_cuda and alibi_slopes.get_device() == device and
+                                         alibi_slopes.dtype == torch.float32 and alibi_slopes.is_contiguous() and
+                                         alibi_slopes.numel() == q_heads):
+        raise AssertionError("alibi_slopes: a contiguous float32 tensor on q's device, one slope per head, is needed")
+    shape = (batch, q_heads, tokens, k_pages.shape[3])
+    if out is None:
+        out = torch.empty(shape, device=q.device, dtype=q.dtype)
+    elif not (out.is_cuda and out.get_device() == device and out.dtype == q.dtype and tuple(out.shape) == shape and
+              out.is_contiguous()):
+        raise AssertionError("out: a contiguous tensor like q is needed")
+    lse = torch.empty(shape[:3], device=q.device, dtype=torch.float32) if return_lse else None
+    L = lib()
+    nbytes = L.flash_decode_workspace_bytes(tokens, q_heads, k_pages.shape[1], k_pages.shape[3])
+    workspace = torch.empty(max(nbytes, 16), device=q.device, dtype=torch.uint8)
+    cache = _cache_struct(torch, k_pages, v_pages, page_table, lengths, counts)
+    _on_device(torch, device, L.flash_decode, cache, qs, out.data_ptr(), None if lse is None else lse.data_ptr(), batch,
+               tokens, q_heads, softmax_scale, window_left, None if alibi_slopes is None else alibi_slopes.data_ptr(),
+               workspace.data_ptr(), nbytes)
     return (out, lse) if return_lse else out

@@ -21,13 +21,16 @@
 #include "fwd_pair_ahead.cuh"
 #include "fwd_persistent.cuh"
 #include "fwd_serial.cuh"
+#include "host.h"
 #include "work_items.h"
 
 namespace {
-
 thread_local char g_err[512] = "";
+}  // namespace
 
-int fail(int code, const char* fmt, const char* a = "", const char* b = "") {
+namespace fa_host {
+
+int fail(int code, const char* fmt, const char* a, const char* b) {
   snprintf(g_err, sizeof(g_err), fmt, a, b);
   return code;
 }
@@ -36,12 +39,6 @@ int fail_cuda(const char* what, cudaError_t e) {
   return FA_CUDA_ERROR;
 }
 
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-// The driver entry point is looked up at run time so that the library links against the CUDA
-// runtime only and can be loaded (for symbol checks) on a machine without a driver.
 EncodeTiledFn encode_tiled_fn() {
   static EncodeTiledFn fn = nullptr;
   static std::once_flag once;
@@ -55,33 +52,19 @@ EncodeTiledFn encode_tiled_fn() {
   return fn;
 }
 
-constexpr int kMaxDevices = 64;
-// Launches in flight at the same time must not share a pair of scheduler words (the kernel leaves its pair at zero).
-// The first kOwnedSlots streams that are used on a device each own a pair: launches on one stream run one after the
-// other, so nothing more is needed. Streams are told apart by their id, which is never used again after a stream is
-// destroyed (nothing tells this library that one was, so its pair stays taken until flash_forward_shutdown()). Launches
-// on any further stream take the 64 remaining pairs in turn, and one that reuses a pair last used on ANOTHER stream
-// first makes its stream wait for that earlier launch (an event per pair). (With an event behind every launch a call
-// cost 1 us more on the host, and the kernel behind it could not start early. 256 owners: eight times one of
-// PyTorch's stream pools; finding the last of them takes 0.1 us.)
-constexpr int kOwnedSlots = 256;
-constexpr int kSchedSlots = kOwnedSlots + 64;
-constexpr size_t kDeviceWords = 4 + 2 * kSchedSlots;
-struct DeviceState {
-  std::mutex mu;
-  bool probed = false;
-  bool is_sm100 = false;
-  int num_sms = 0;
-  int* status = nullptr;  // device words: [0] status, then kSchedSlots pairs of scheduler words
-  int num_owned = 0;                           // pairs 0 .. num_owned-1 belong to the streams owner[]
-  unsigned long long owner[kOwnedSlots] = {};  // stream ids
-  unsigned next_sched = 0;
-  cudaEvent_t slot_done[kSchedSlots] = {};     // recorded behind the last launch that used the pair
-  unsigned long long slot_stream[kSchedSlots] = {};  // the id of that launch's stream
-  bool slot_used[kSchedSlots] = {};
-  unsigned long long acquired_by = 0;  // the stream id of the launch between sched_acquire and sched_release
-  bool attr_set[29] = {};
-};
+int check_scale(float softmax_scale) {
+  if (!(softmax_scale == softmax_scale)) return fail(FA_INVALID_ARG, "softmax_scale is NaN");
+  // (hidden scores are pushed to about -3e38 before the scale is applied: a scale this small would bring them back)
+  if (softmax_scale > 3.0e38f || (softmax_scale > 0.f && softmax_scale < 1.0e-30f))
+    return fail(FA_INVALID_ARG, "softmax_scale must be a finite value of at least 1e-30 (or <= 0 for 1/sqrt(head_dim))");
+  return FA_OK;
+}
+
+}  // namespace fa_host
+
+using namespace fa_host;
+
+namespace {
 
 // Hands out the scheduler words for one launch on `st`. Call with s->mu held; `*slot_out` is passed to
 // sched_release() right after the launch, under the same lock.
@@ -126,6 +109,10 @@ int sched_release(DeviceState* s, cudaStream_t st, int slot) {
 }
 DeviceState g_dev[kMaxDevices];
 
+}  // namespace
+
+namespace fa_host {
+
 int device_state(DeviceState** out) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -153,11 +140,26 @@ int device_state(DeviceState** out) {
   return FA_OK;
 }
 
-// 4-D map over one [bh][seqlen][head_dim] fp16 tensor: {64 contiguous elements, row, 64-wide
-// panel, head}. One box = 128 rows x all panels of one head, landing in shared memory as
-// [panel][row][64] with the 128-byte swizzle a UMMA descriptor expects. Out-of-range rows of
-// a ragged last tile read as zero.
-int make_map(CUtensorMap* map, const void* base, int bh, int seqlen, int head_dim, int box_rows, int box_panels = 0) {
+int device_state_for(cudaStream_t st, DeviceState** out, bool* captured) {
+  cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+  cudaError_t e = cudaStreamIsCapturing(st, &cap);
+  if (e != cudaSuccess) return fail_cuda("cudaStreamIsCapturing", e);
+  *captured = cap != cudaStreamCaptureStatusNone;
+  if (*captured) {
+    int dev = 0;
+    if ((e = cudaGetDevice(&dev)) != cudaSuccess) return fail_cuda("cudaGetDevice", e);
+    bool probed = false;
+    if (dev >= 0 && dev < kMaxDevices) {
+      std::lock_guard<std::mutex> lk(g_dev[dev].mu);
+      probed = g_dev[dev].probed;
+    }
+    if (!probed)
+      return fail(FA_UNSUPPORTED, "the first call on a device allocates a few words: make it before a capture begins");
+  }
+  return device_state(out);
+}
+
+int make_map(CUtensorMap* map, const void* base, int bh, int seqlen, int head_dim, int box_rows, int box_panels) {
   if (box_panels <= 0) box_panels = head_dim / 64;
   EncodeTiledFn enc = encode_tiled_fn();
   if (!enc) return fail(FA_CUDA_ERROR, "cuTensorMapEncodeTiled entry point not available");
@@ -174,6 +176,10 @@ int make_map(CUtensorMap* map, const void* base, int bh, int seqlen, int head_di
   }
   return FA_OK;
 }
+
+}  // namespace fa_host
+
+namespace {
 
 template <typename K>
 int ensure_smem_attr(DeviceState* s, int slot, K kernel, int bytes) {
@@ -401,11 +407,6 @@ int launch_persistent_noalloc(NoAllocState* s, const CUtensorMap& mq, const CUte
 
 }  // namespace
 
-// A window that reaches past either end of the sequence for every row is no window. Mapping it to
-// "unbounded" (-1) here keeps the tile arithmetic (row - window_left, row + window_right) inside int
-// for every legal argument, INT_MAX included.
-static inline int norm_window(int w, int seqlen) { return (w < 0 || w >= seqlen) ? -1 : w; }
-
 extern "C" {
 
 const char* flash_forward_last_error(void) { return g_err; }
@@ -477,10 +478,7 @@ static int forward_impl(const void* q, const void* k, const void* v, void* o, in
   if ((long long)batch * heads > 0x7fffffffLL) return fail(FA_INVALID_ARG, "batch*heads overflows int");
   if (kernel < 0 || kernel > 2) return fail(FA_INVALID_ARG, "kernel must be 0 (default), 1 (serial) or 2 (CTA pair)");
   if (kernel == 2 && head_dim != 128) return fail(FA_UNSUPPORTED, "the CTA-pair kernel needs head_dim 128");
-  if (!(softmax_scale == softmax_scale)) return fail(FA_INVALID_ARG, "softmax_scale is NaN");
-  // (hidden scores are pushed to about -3e38 before the scale is applied: a scale this small would bring them back)
-  if (softmax_scale > 3.0e38f || (softmax_scale > 0.f && softmax_scale < 1.0e-30f))
-    return fail(FA_INVALID_ARG, "softmax_scale must be a finite value of at least 1e-30 (or <= 0 for 1/sqrt(head_dim))");
+  if (int bad = check_scale(softmax_scale); bad != FA_OK) return bad;
   if (!(dropout_prob >= 0.f && dropout_prob <= 1.f)) return fail(FA_INVALID_ARG, "dropout_prob must lie in [0, 1]");
   // keep threshold in 1/256 steps (nearest); a probability below 1/512 keeps everything and takes the plain kernel
   const unsigned keep_thr = (unsigned)rintf(256.f * (1.f - dropout_prob));
@@ -621,17 +619,18 @@ int flash_forward_check(void* stream) {
   cudaError_t e = cudaStreamSynchronize(st);
   if (e != cudaSuccess) return fail_cuda("cudaStreamSynchronize", e);
   if (!s->status) return FA_OK;
-  int host = 0;
-  if ((e = cudaMemcpy(&host, s->status, sizeof(int), cudaMemcpyDeviceToHost)) != cudaSuccess)
+  int host[2] = {0, 0};
+  if ((e = cudaMemcpy(host, s->status, sizeof(host), cudaMemcpyDeviceToHost)) != cudaSuccess)
     return fail_cuda("cudaMemcpy(status)", e);
-  if (host != 0) {
-    // Only the status word is cleared: the scheduler words belong to launches that may still be running on other
-    // streams, and a kernel that gave up still leaves its own pair at zero (every CTA reaches the final count).
-    cudaMemset(s->status, 0, sizeof(int));
-    snprintf(g_err, sizeof(g_err), "a wait inside the attention kernel ran out of time (status word %d)", host);
+  if (host[0] == 0 && host[1] == 0) return FA_OK;
+  // Only the status words are cleared: the scheduler words belong to launches that may still be running on other
+  // streams, and a kernel that gave up still leaves its own pair at zero (every CTA reaches the final count).
+  cudaMemset(s->status, 0, sizeof(host));
+  if (host[0] != 0) {
+    snprintf(g_err, sizeof(g_err), "a wait inside the attention kernel ran out of time (status word %d)", host[0]);
     return FA_DEVICE_TIMEOUT;
   }
-  return FA_OK;
+  return fail(FA_BAD_INDEX, "a page of a page table, a length, a count or a position in device memory was out of range");
 }
 
 int run_flash_attention_c(int B, int N, int S, int d, void* Q, void* K, void* V, void* O, void* L, void* M,
@@ -777,10 +776,7 @@ int flash_forward_noalloc(const void* q, const void* k, const void* v, void* o, 
              slot, kNoAllocSlots);
     return FA_INVALID_ARG;
   }
-  if (!(softmax_scale == softmax_scale)) return fail(FA_INVALID_ARG, "softmax_scale is NaN");
-  // (hidden scores are pushed to about -3e38 before the scale is applied: a scale this small would bring them back)
-  if (softmax_scale > 3.0e38f || (softmax_scale > 0.f && softmax_scale < 1.0e-30f))
-    return fail(FA_INVALID_ARG, "softmax_scale must be a finite value of at least 1e-30 (or <= 0 for 1/sqrt(head_dim))");
+  if (int bad = check_scale(softmax_scale); bad != FA_OK) return bad;
   const long long bh_ll = (long long)batch * heads;
   const int pairs = (seqlen + 2 * fa::kBlockM - 1) / (2 * fa::kBlockM);
   // the work counter in the scratch is a 32-bit int to which the kernel adds the grid size

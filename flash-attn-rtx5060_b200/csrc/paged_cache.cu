@@ -1,0 +1,227 @@
+// Host side of the paged key-value cache: argument checks, tensor maps and launches of flash_cache_append and flash_decode.
+#include <cmath>
+#include <cstring>
+
+#include "host.h"
+#include "paged_cache.cuh"
+
+using namespace fa_host;
+
+namespace {
+
+// Two CTAs on each of a B200's 148 SMs: three (head_dim 64: six) stages of 32 KB (16 KB) each keep up to 192 KB a SM in
+// flight. On a device with fewer SMs they run one after the other.
+constexpr int kDecodeCtas = 296;
+
+int check_cache(const fa_paged_cache* c, int batch, int tokens, int q_heads) {
+  if (!c) return fail(FA_INVALID_ARG, "cache is null");
+  if (!c->k || !c->v || !c->page_table || !c->lengths) return fail(FA_INVALID_ARG, "null pointer in the cache");
+  if (c->dtype != FA_FP16 && c->dtype != FA_BF16) return fail(FA_UNSUPPORTED, "dtype must be FA_FP16 or FA_BF16");
+  if (c->head_dim != 64 && c->head_dim != 128) return fail(FA_UNSUPPORTED, "head_dim must be 64 or 128");
+  if (batch <= 0 || tokens <= 0) return fail(FA_INVALID_ARG, "batch and tokens must be positive");
+  if (c->kv_heads <= 0 || c->num_pages <= 0 || c->max_pages <= 0)
+    return fail(FA_INVALID_ARG, "kv_heads, num_pages and max_pages must be positive");
+  if (c->page_size <= 0 || c->page_size % 8 != 0) return fail(FA_UNSUPPORTED, "page_size must be a multiple of 8");
+  if (static_cast<long long>(c->max_pages) * c->page_size > 0x7fffffffLL - 65536)
+    return fail(FA_INVALID_ARG, "max_pages * page_size does not fit 31 bits");
+  if (c->table_stride < c->max_pages && batch > 1)
+    return fail(FA_INVALID_ARG, "table_stride is smaller than max_pages");
+  if ((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) & 15)
+    return fail(FA_INVALID_ARG, "pages must be 16-byte aligned");
+  if ((reinterpret_cast<uintptr_t>(c->page_table) | reinterpret_cast<uintptr_t>(c->lengths) |
+       reinterpret_cast<uintptr_t>(c->counts)) & 3)
+    return fail(FA_INVALID_ARG, "page_table, lengths and counts must be 4-byte aligned");
+  const long long strides[3] = {c->page_stride, c->head_stride, c->token_stride};
+  const int extents[3] = {c->num_pages, c->kv_heads, c->page_size};
+  for (int i = 0; i < 3; ++i)
+    if (extents[i] > 1 && (strides[i] < c->head_dim || strides[i] % 8 != 0 || strides[i] >= 1ll << 38))
+      return fail(FA_INVALID_ARG, "strides of the pages must be multiples of 8 elements, of head_dim or more");
+  if (q_heads < 0 || q_heads % c->kv_heads != 0)
+    return fail(FA_INVALID_ARG, "the query heads must be a multiple of kv_heads");
+  return FA_OK;
+}
+
+int check_rows(const fa_rows* r, int batch, int heads, int tokens) {
+  if (!r || !r->data) return fail(FA_INVALID_ARG, "null rows");
+  if (reinterpret_cast<uintptr_t>(r->data) & 15) return fail(FA_INVALID_ARG, "rows must be 16-byte aligned");
+  const long long strides[3] = {r->batch_stride, r->head_stride, r->token_stride};
+  const int extents[3] = {batch, heads, tokens};
+  for (int i = 0; i < 3; ++i)
+    if (extents[i] > 1 && (strides[i] < 0 || strides[i] % 8 != 0))
+      return fail(FA_INVALID_ARG, "strides of the rows must be multiples of 8 elements and not negative");
+  return FA_OK;
+}
+
+// (a stride along an extent of 1 may be anything: it is not used)
+fa::StridedRows rows_of(const fa_rows* r) {
+  return fa::StridedRows{r->data, r->batch_stride, r->head_stride, r->token_stride};
+}
+
+fa::CacheView view_of(const fa_paged_cache* c, int batch, int tokens, DeviceState* s) {
+  return fa::CacheView{c->page_stride, c->head_stride, c->token_stride, c->num_pages, c->page_size, c->kv_heads,
+                       c->page_table, c->table_stride, c->max_pages, c->lengths, c->counts, batch, tokens,
+                       s->status + 1};
+}
+
+// 5-D map over the pages of K or V: {64 contiguous elements, token of the page, 64-wide panel, head, page}. One box is
+// `box_rows` tokens of a head, [panel][token][64] in shared memory with the 128-byte swizzle.
+int make_page_map(CUtensorMap* map, const fa_paged_cache* c, void* base, int box_rows) {
+  EncodeTiledFn enc = encode_tiled_fn();
+  if (!enc) return fail(FA_CUDA_ERROR, "cuTensorMapEncodeTiled entry point not available");
+  const cuuint64_t row = 2ull * c->head_dim;
+  cuuint64_t dims[5] = {64, (cuuint64_t)c->page_size, (cuuint64_t)(c->head_dim / 64), (cuuint64_t)c->kv_heads,
+                        (cuuint64_t)c->num_pages};
+  cuuint64_t strides[4] = {2ull * c->token_stride, 128, c->kv_heads > 1 ? 2ull * c->head_stride : row,
+                           c->num_pages > 1 ? 2ull * c->page_stride : row};
+  cuuint32_t box[5] = {64, (cuuint32_t)box_rows, (cuuint32_t)(c->head_dim / 64), 1, 1};
+  cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+  CUresult r = enc(map, c->dtype == FA_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, base,
+                   dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(FA_CUDA_ERROR, "cuTensorMapEncodeTiled refused the map of the pages");
+  return FA_OK;
+}
+
+// Rows (query heads of a key head times new tokens) of a CTA's tile: 16 where they fit, else 32 or 64, so that a tile of
+// keys is read for as many rows as there are.
+int tile_rows(long long rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
+
+template <typename T, int D, int kRowWarps>
+int launch_decode(const CUtensorMap& mk, const CUtensorMap& mv, const fa::DecodeParams& p, cudaStream_t st, bool early) {
+  using Cfg = fa::DecodeCfg<D, kRowWarps>;
+  constexpr auto kernel = fa::decode_kernel<T, D, kRowWarps>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes);
+  if (e != cudaSuccess) return fail_cuda("cudaFuncSetAttribute(MaxDynamicSharedMemorySize)", e);
+  e = launch_early(kernel, dim3(p.ctas), Cfg::kThreads, Cfg::kSmemBytes, st, early, mk, mv, p);
+  if (e != cudaSuccess) return fail_cuda("launch decode_kernel", e);
+  const long long rows = static_cast<long long>(p.cache.batch) * p.q_heads * p.cache.tokens;
+  e = launch_early(fa::decode_join_kernel<T, D>, dim3(static_cast<unsigned>((rows + 3) / 4)), 128, 0, st, early, p,
+                   static_cast<int>(Cfg::kRows));
+  if (e != cudaSuccess) return fail_cuda("launch decode_join_kernel", e);
+  return FA_OK;
+}
+
+template <typename T, int D>
+int launch_decode_rows(int rows, const CUtensorMap& mk, const CUtensorMap& mv, const fa::DecodeParams& p, cudaStream_t st,
+                       bool early) {
+  return rows == 16   ? launch_decode<T, D, 1>(mk, mv, p, st, early)
+         : rows == 32 ? launch_decode<T, D, 2>(mk, mv, p, st, early)
+                      : launch_decode<T, D, 4>(mk, mv, p, st, early);
+}
+
+}  // namespace
+
+extern "C" {
+
+int flash_cache_append(const fa_paged_cache* cache, const fa_rows* k, const fa_rows* v, const fa_rows* q, void* q_out,
+                       int batch, int tokens, int q_heads, const float* rotary, int rotary_dim, int rotary_positions,
+                       int interleaved, void* stream) {
+  int rc = check_cache(cache, batch, tokens, q_heads);
+  if (rc != FA_OK) return rc;
+  if ((rc = check_rows(k, batch, cache->kv_heads, tokens)) != FA_OK) return rc;
+  if ((rc = check_rows(v, batch, cache->kv_heads, tokens)) != FA_OK) return rc;
+  const bool has_q = q != nullptr;
+  if (has_q != (q_out != nullptr) || has_q != (q_heads > 0))
+    return fail(FA_INVALID_ARG, "q, q_out and q_heads come together or not at all");
+  if (has_q && (rc = check_rows(q, batch, q_heads, tokens)) != FA_OK) return rc;
+  if (reinterpret_cast<uintptr_t>(q_out) & 15) return fail(FA_INVALID_ARG, "q_out must be 16-byte aligned");
+  if (has_q && !rotary) return fail(FA_INVALID_ARG, "queries are taken only to be rotated");
+  if (rotary) {
+    if (rotary_dim <= 0 || rotary_dim > cache->head_dim || rotary_dim % 16 != 0)
+      return fail(FA_UNSUPPORTED, "rotary_dim must be a multiple of 16, up to head_dim");
+    if (rotary_positions <= 0) return fail(FA_INVALID_ARG, "rotary_positions must be positive");
+    if (reinterpret_cast<uintptr_t>(rotary) & 15) return fail(FA_INVALID_ARG, "rotary must be 16-byte aligned");
+  }
+  const long long row_units = (2ll * cache->kv_heads + q_heads) * (cache->head_dim / 16);  // of a token
+  if (static_cast<double>(batch) * tokens * row_units >= 256.0 * 0x7fffffff) return fail(FA_INVALID_ARG, "too many rows");
+  const long long units = static_cast<long long>(batch) * tokens * row_units;
+
+  DeviceState* s = nullptr;
+  bool captured = false;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if ((rc = device_state_for(st, &s, &captured)) != FA_OK) return rc;
+  if (!s->is_sm100) return fail(FA_UNSUPPORTED, "this library runs on compute capability 10.x (B200) only");
+  fa::AppendParams p;
+  memset(&p, 0, sizeof(p));
+  p.cache = view_of(cache, batch, tokens, s);
+  p.k_pages = cache->k;
+  p.v_pages = cache->v;
+  p.k = rows_of(k);
+  p.v = rows_of(v);
+  if (has_q) p.q = rows_of(q);
+  p.q_out = q_out;
+  p.q_heads = q_heads;
+  p.rotary = rotary;
+  p.rotary_dim = rotary ? rotary_dim : 0;
+  p.positions = rotary_positions;
+  p.interleaved = interleaved ? 1 : 0;
+  p.units = units;
+  const bool half = cache->dtype == FA_FP16, d64 = cache->head_dim == 64;
+  const auto kernel = half ? (d64 ? fa::cache_append_kernel<__half, 64> : fa::cache_append_kernel<__half, 128>)
+                           : (d64 ? fa::cache_append_kernel<__nv_bfloat16, 64> : fa::cache_append_kernel<__nv_bfloat16, 128>);
+  cudaError_t e = launch_early(kernel, dim3(static_cast<unsigned>((units + 255) / 256)), 256, 0, st, !captured, p);
+  if (e != cudaSuccess) return fail_cuda("launch cache_append_kernel", e);
+  return FA_OK;
+}
+
+size_t flash_decode_workspace_bytes(int tokens, int q_heads, int kv_heads, int head_dim) {
+  if (tokens <= 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads != 0 || head_dim <= 0) return 0;
+  return static_cast<size_t>(kDecodeCtas) * 2 * tile_rows(static_cast<long long>(q_heads / kv_heads) * tokens) *
+         (head_dim + 2) * sizeof(float);
+}
+
+int flash_decode(const fa_paged_cache* cache, const fa_rows* q, void* o, float* lse, int batch, int tokens, int q_heads,
+                 float softmax_scale, int window_left, const float* alibi_slopes, void* workspace, size_t workspace_bytes,
+                 void* stream) {
+  int rc = check_cache(cache, batch, tokens, q_heads);
+  if (rc != FA_OK) return rc;
+  if (q_heads <= 0) return fail(FA_INVALID_ARG, "q_heads must be positive");
+  if ((rc = check_rows(q, batch, q_heads, tokens)) != FA_OK) return rc;
+  if (!o || (reinterpret_cast<uintptr_t>(o) & 15)) return fail(FA_INVALID_ARG, "o must be there and 16-byte aligned");
+  if ((reinterpret_cast<uintptr_t>(lse) | reinterpret_cast<uintptr_t>(alibi_slopes)) & 3)
+    return fail(FA_INVALID_ARG, "lse and alibi_slopes must be 4-byte aligned");
+  if ((rc = check_scale(softmax_scale)) != FA_OK) return rc;
+  const long long rows = static_cast<long long>(q_heads / cache->kv_heads) * tokens;
+  if (static_cast<double>(batch) * q_heads * tokens > 0x7fffffff - 64)  // (so are the rows of a key head)
+    return fail(FA_INVALID_ARG, "too many rows");
+  if (!workspace || workspace_bytes < flash_decode_workspace_bytes(tokens, q_heads, cache->kv_heads, cache->head_dim))
+    return fail(FA_INVALID_ARG, "workspace is null or smaller than flash_decode_workspace_bytes()");
+  if (reinterpret_cast<uintptr_t>(workspace) & 15) return fail(FA_INVALID_ARG, "workspace must be 16-byte aligned");
+
+  DeviceState* s = nullptr;
+  bool captured = false;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if ((rc = device_state_for(st, &s, &captured)) != FA_OK) return rc;
+  if (!s->is_sm100) return fail(FA_UNSUPPORTED, "this library runs on compute capability 10.x (B200) only");
+  if (softmax_scale <= 0.f) softmax_scale = 1.0f / sqrtf(static_cast<float>(cache->head_dim));
+
+  const int tile = tile_rows(rows);
+  fa::DecodeParams p;
+  memset(&p, 0, sizeof(p));
+  p.cache = view_of(cache, batch, tokens, s);
+  p.q = rows_of(q);
+  p.o = o;
+  p.lse = lse;
+  p.q_heads = q_heads;
+  p.group = q_heads / cache->kv_heads;
+  p.scale_log2 = softmax_scale * 1.4426950408889634f;
+  p.window_left = window_left;
+  p.alibi_slopes = alibi_slopes;
+  p.box_rows = cache->page_size & -cache->page_size;
+  if (p.box_rows > fa::kDecodeKeys) p.box_rows = fa::kDecodeKeys;
+  p.row_tiles = static_cast<int>((rows + tile - 1) / tile);
+  p.ctas = kDecodeCtas;
+  p.part_o = static_cast<float*>(workspace);
+  p.part_ml = p.part_o + static_cast<size_t>(kDecodeCtas) * 2 * tile * cache->head_dim;
+  p.status = s->status;
+  CUtensorMap mk, mv;
+  if ((rc = make_page_map(&mk, cache, cache->k, p.box_rows)) != FA_OK) return rc;
+  if ((rc = make_page_map(&mv, cache, cache->v, p.box_rows)) != FA_OK) return rc;
+  if (cache->dtype == FA_FP16)
+    return cache->head_dim == 64 ? launch_decode_rows<__half, 64>(tile, mk, mv, p, st, !captured)
+                                 : launch_decode_rows<__half, 128>(tile, mk, mv, p, st, !captured);
+  return cache->head_dim == 64 ? launch_decode_rows<__nv_bfloat16, 64>(tile, mk, mv, p, st, !captured)
+                               : launch_decode_rows<__nv_bfloat16, 128>(tile, mk, mv, p, st, !captured);
+}
+
+}  // extern "C"

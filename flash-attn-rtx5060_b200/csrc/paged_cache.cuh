@@ -1,0 +1,678 @@
+// Kernels of the paged key-value cache: new keys and values enter it (cache_append_kernel), and the newest tokens of every
+// sequence attend to what it holds (decode_kernel, and decode_join_kernel for the sequences that several CTAs shared).
+//
+// The keys and values of a sequence lie in pages of `page_size` tokens that its row of the page table names in order:
+// token j is row j % page_size of page table[j / page_size]. Nothing of a page behind the sequence's last token, and no
+// entry of the table behind its last page, is read.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <type_traits>
+
+#include "ptx.cuh"
+
+namespace fa {
+
+struct CacheView {
+  long long page_stride, head_stride, token_stride;  // elements
+  int num_pages, page_size, kv_heads;
+  const int* page_table;  // [batch][table_stride], max_pages entries a row
+  long long table_stride;
+  int max_pages;
+  const int* lengths;  // tokens of every sequence, the new ones included
+  const int* counts;   // new tokens of every sequence, or nullptr: `tokens` each
+  int batch, tokens;
+  int* bad_index;  // device word, set to 1 where an index in device memory is out of range
+};
+
+struct StridedRows {  // [batch][head][token] rows of head_dim contiguous elements
+  const void* data;
+  long long batch_stride, head_stride, token_stride;  // elements
+};
+
+// Length and number of new tokens of sequence b, within what the table and the call can hold: 0 <= count <= tokens,
+// count <= length <= max_pages * page_size. Anything else is reported and cut to that.
+__device__ __forceinline__ void sequence_of(const CacheView& c, int b, int& length, int& count) {
+  const int len = c.lengths[b];
+  const int cnt = c.counts ? c.counts[b] : c.tokens;
+  const long long room = static_cast<long long>(c.max_pages) * c.page_size;
+  length = len < 0 ? 0 : len > room ? static_cast<int>(room) : len;
+  count = cnt < 0 ? 0 : cnt > c.tokens ? c.tokens : cnt;
+  // (a sequence of length 0 is one that is not there: it needs no count of its own)
+  if (length != len || (len > 0 && (count != cnt || count > length))) atomicExch(c.bad_index, 1);
+  if (count > length) count = length;
+}
+
+template <typename T>
+__device__ __forceinline__ float2 to_float2(uint32_t v) {
+  if constexpr (std::is_same_v<T, __half>) return __half22float2(*reinterpret_cast<__half2*>(&v));
+  else return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&v));
+}
+template <typename T>
+__device__ __forceinline__ uint32_t from_floats(float lo, float hi) {
+  if constexpr (std::is_same_v<T, __half>) {
+    return pack_f16x2(lo, hi);
+  } else {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// append
+// ---------------------------------------------------------------------------------------------------------------------
+struct AppendParams {
+  CacheView cache;
+  void *k_pages, *v_pages;
+  StridedRows k, v, q;  // q.data may be nullptr
+  void* q_out;          // [batch][q_heads][tokens][head_dim]
+  int q_heads;
+  const float* rotary;  // [positions][rotary_dim]: rotary_dim / 2 cosines, then as many sines; nullptr: nothing is rotated
+  int rotary_dim, positions, interleaved;
+  long long units;  // batch * tokens * (2 * kv_heads + q_heads) * (head_dim / 16)
+};
+
+// One thread moves 16 elements of one row as two 16-byte pieces: for a rotation of halves one piece of either half, so
+// that both elements of every pair are in one thread; else 32 bytes in a row. Keys and queries are turned in fp32 by the
+// cosine and sine of their position and rounded once; values, and what lies behind rotary_dim, are copied as bits.
+// Bound by the bytes moved; a step of generation by the launch and three dependent reads (length, page, row).
+template <typename T, int D>
+__global__ void __launch_bounds__(256) cache_append_kernel(const AppendParams p) {
+  const long long unit = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
+  griddep_wait();
+  if (unit >= p.units) return;
+  constexpr int kUnits = D / 16;
+  const int c = static_cast<int>(unit % kUnits);
+  const long long row = unit / kUnits;
+  const int heads = 2 * p.cache.kv_heads + p.q_heads;
+  const int h = static_cast<int>(row % heads);
+  const long long bt = row / heads;
+  const int t = static_cast<int>(bt % p.cache.tokens), b = static_cast<int>(bt / p.cache.tokens);
+
+  const bool is_q = h >= 2 * p.cache.kv_heads, is_v = !is_q && h >= p.cache.kv_heads;
+  const int head = is_q ? h - 2 * p.cache.kv_heads : is_v ? h - p.cache.kv_heads : h;
+  const StridedRows& src = is_q ? p.q : is_v ? p.v : p.k;
+  const T* from = static_cast<const T*>(src.data) + b * src.batch_stride + head * src.head_stride + t * src.token_stride;
+
+  const int half = p.rotary_dim / 2;
+  const bool turn = !is_v && c < p.rotary_dim / 16;
+  const int at0 = turn && !p.interleaved ? c * 8 : c * 16;
+  const int at1 = turn && !p.interleaved ? at0 + half : at0 + 8;
+  uint4 x0 = *reinterpret_cast<const uint4*>(from + at0), x1 = *reinterpret_cast<const uint4*>(from + at1);
+
+  int length, count;
+  sequence_of(p.cache, b, length, count);
+  const bool real = t < count;
+  if (!real && !is_q) return;
+  const int position = length - count + t;
+  T* to;
+  if (is_q) {
+    to = static_cast<T*>(p.q_out) + ((static_cast<long long>(b) * p.q_heads + head) * p.cache.tokens + t) * D;
+  } else {
+    const int page = p.cache.page_table[b * p.cache.table_stride + position / p.cache.page_size];
+    if (page < 0 || page >= p.cache.num_pages) {
+      atomicExch(p.cache.bad_index, 1);
+      return;
+    }
+    to = static_cast<T*>(is_v ? p.v_pages : p.k_pages) + page * p.cache.page_stride + head * p.cache.head_stride +
+         (position % p.cache.page_size) * p.cache.token_stride;
+  }
+  if (!real) {  // a padded query row
+    x0 = x1 = make_uint4(0, 0, 0, 0);
+  } else if (turn) {
+    if (position >= p.positions) {  // no angles: nothing is written
+      atomicExch(p.cache.bad_index, 1);
+      return;
+    }
+    const float* angles = p.rotary + static_cast<long long>(position) * p.rotary_dim + c * 8;
+    uint32_t a[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
+    float cs[8], sn[8];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      *reinterpret_cast<float4*>(cs + 4 * i) = *reinterpret_cast<const float4*>(angles + 4 * i);
+      *reinterpret_cast<float4*>(sn + 4 * i) = *reinterpret_cast<const float4*>(angles + half + 4 * i);
+    }
+    if (p.interleaved) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float2 z = to_float2<T>(a[i]);
+        a[i] = from_floats<T>(z.x * cs[i] - z.y * sn[i], z.x * sn[i] + z.y * cs[i]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 lo = to_float2<T>(a[i]), hi = to_float2<T>(a[4 + i]);
+        a[i] = from_floats<T>(lo.x * cs[2 * i] - hi.x * sn[2 * i], lo.y * cs[2 * i + 1] - hi.y * sn[2 * i + 1]);
+        a[4 + i] = from_floats<T>(lo.x * sn[2 * i] + hi.x * cs[2 * i], lo.y * sn[2 * i + 1] + hi.y * cs[2 * i + 1]);
+      }
+    }
+    x0 = make_uint4(a[0], a[1], a[2], a[3]);
+    x1 = make_uint4(a[4], a[5], a[6], a[7]);
+  }
+  *reinterpret_cast<uint4*>(to + at0) = x0;
+  *reinterpret_cast<uint4*>(to + at1) = x1;
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// attention of the newest tokens
+// ---------------------------------------------------------------------------------------------------------------------
+constexpr int kDecodeKeys = 64;  // keys of a tile
+
+struct DecodeParams {
+  CacheView cache;
+  StridedRows q;
+  void* o;     // [batch][q_heads][tokens][head_dim]
+  float* lse;  // [batch][q_heads][tokens], or nullptr
+  int q_heads, group;  // group: query heads of a key head
+  float scale_log2;
+  int window_left;  // < 0: unbounded
+  const float* alibi_slopes;
+  int box_rows;   // rows of a page that one TMA box brings: the largest power of two that divides page_size, 64 at most
+  int row_tiles;  // of the group * tokens rows of a key head
+  int ctas;
+  float* part_o;   // [ctas][2][rows of a tile][head_dim]
+  float* part_ml;  // [ctas][2][rows of a tile][2]: running maximum (log2 units) and sum
+  int* status;
+};
+
+// The work is one line of tiles of 64 keys: sequence by sequence, in each key head by key head (and row tile by row
+// tile), the tiles that the new tokens see. Every CTA takes an equal stretch of the line. A (sequence, key head, row tile)
+// that lies within one stretch is finished there; one that is cut has its parts written as (maximum, sum, unnormalised
+// output) and joined by decode_join_kernel in the order of the line, so the results depend on the lengths alone.
+struct DecodeLine {
+  __device__ static void tiles_of(const DecodeParams& p, int b, int& first, int& tiles, int& length, int& count) {
+    sequence_of(p.cache, b, length, count);
+    const int lo = p.window_left >= 0 && length - count > p.window_left ? length - count - p.window_left : 0;
+    first = lo / kDecodeKeys;
+    tiles = count > 0 ? (length + kDecodeKeys - 1) / kDecodeKeys - first : 0;
+  }
+  // Sums the tiles of one key head over all sequences and over those in front of `upto`. All lanes of a warp call it.
+  __device__ static void sum(const DecodeParams& p, int upto, long long& all, long long& before, int lane) {
+    all = before = 0;
+    for (int b = lane; b < p.cache.batch; b += 32) {
+      int first, tiles, length, count;
+      tiles_of(p, b, first, tiles, length, count);
+      all += tiles;
+      if (b < upto) before += tiles;
+    }
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) {
+      all += __shfl_xor_sync(0xffffffffu, all, s);
+      before += __shfl_xor_sync(0xffffffffu, before, s);
+    }
+  }
+  __device__ static long long share_of(const DecodeParams& p, long long all) {
+    const long long total = all * p.cache.kv_heads * p.row_tiles;
+    return (total + p.ctas - 1) / p.ctas;
+  }
+};
+
+// A stretch of the line, walked item by item; every role of a CTA walks it for itself.
+struct DecodeWalk {
+  long long at, begin, end;  // of the line
+  long long b_start;   // where sequence b starts
+  int b, first, tiles, length, count;
+
+  __device__ void start(const DecodeParams& p, int cta, int lane) {
+    long long all, before;
+    DecodeLine::sum(p, 0, all, before, lane);
+    const long long share = DecodeLine::share_of(p, all), total = all * p.cache.kv_heads * p.row_tiles;
+    at = begin = cta * share;
+    end = at + share < total ? at + share : total;
+    b = 0;
+    b_start = 0;
+    // the sequence that holds `at`, 32 at a time
+    const long long per = static_cast<long long>(p.cache.kv_heads) * p.row_tiles;
+    for (int b0 = 0; at < end; b0 += 32) {
+      int f = 0, n = 0, len = 0, cnt = 0;
+      if (b0 + lane < p.cache.batch) DecodeLine::tiles_of(p, b0 + lane, f, n, len, cnt);
+      long long upto = n;
+#pragma unroll
+      for (int s = 1; s < 32; s <<= 1) {
+        const long long v = __shfl_up_sync(0xffffffffu, upto, s);
+        if (lane >= s) upto += v;
+      }
+      upto = b_start + upto * per;
+      const unsigned found = __ballot_sync(0xffffffffu, upto > at);
+      if (found) {
+        const int src = __ffs(found) - 1;
+        b = b0 + src;
+        first = __shfl_sync(0xffffffffu, f, src);
+        tiles = __shfl_sync(0xffffffffu, n, src);
+        length = __shfl_sync(0xffffffffu, len, src);
+        count = __shfl_sync(0xffffffffu, cnt, src);
+        b_start = __shfl_sync(0xffffffffu, upto, src) - tiles * per;
+        return;
+      }
+      b_start = __shfl_sync(0xffffffffu, upto, 31);
+    }
+  }
+  // The item at `at`: key head, row tile, and its tiles [t0, t1) of [0, tiles). Moves on behind them.
+  __device__ bool next(const DecodeParams& p, int& kv_head, int& row_tile, int& t0, int& t1) {
+    if (at >= end) return false;
+    const long long per = static_cast<long long>(p.cache.kv_heads) * p.row_tiles;
+    while (at >= b_start + tiles * per) {
+      b_start += tiles * per;
+      ++b;
+      DecodeLine::tiles_of(p, b, first, tiles, length, count);
+    }
+    const int item = static_cast<int>((at - b_start) / tiles);
+    kv_head = item / p.row_tiles;
+    row_tile = item % p.row_tiles;
+    t0 = static_cast<int>((at - b_start) % tiles);
+    t1 = static_cast<int>(end - at < tiles - t0 ? t0 + (end - at) : tiles);
+    at += t1 - t0;
+    return true;
+  }
+};
+
+template <int D, int kRowWarps>
+struct DecodeCfg {
+  static constexpr int kThreads = 160;  // four warps that compute, one that loads
+  static constexpr int kRows = 16 * kRowWarps;
+  static constexpr int kKeyWarps = 4 / kRowWarps;
+  static constexpr int kWarpKeys = kDecodeKeys / kKeyWarps;  // of a tile, a warp's
+  static constexpr int kHalfBytes = kDecodeKeys * D * 2;     // K or V of a tile
+  static constexpr int kStages = D == 128 ? 3 : 6;
+  static constexpr int kOffJoin = kStages * 2 * kHalfBytes;
+  // O of two warps a row group (four key warps), or of one (two); with the maxima and sums of all
+  static constexpr int kJoinBytes = kKeyWarps == 1 ? 0 : (kKeyWarps / 2) * kRows * D * 4;
+  static constexpr int kOffMl = kOffJoin + kJoinBytes;
+  static constexpr int kOffBars = kOffMl + 4 * 16 * 8;
+  static constexpr int kSmemBytes = kOffBars + kStages * 16 + 16;
+};
+
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+__device__ __forceinline__ void ldsm4_trans(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same_v<T, __half>)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                 "{%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                 "{%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void tma_load_5d(void* smem_dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2,
+                                            int c3, int c4) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
+      :
+      : "r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2),
+        "r"(c3), "r"(c4)
+      : "memory");
+}
+// barrier of the four warps that compute
+__device__ __forceinline__ void compute_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+
+// A CTA's four compute warps take 16 * kRowWarps rows (a row: one query head of the key head's group and one new token)
+// and share a tile's keys where the rows are fewer than 64. The products run as m16n8k16 matrix instructions: a step of
+// generation reads every key for a handful of rows, so HBM is what bounds it (at 16 rows a tile of 64 keys is 32 KB and
+// 128 instructions of the SM's warps), and rows that are padding cost nothing that matters. Scores, maxima, sums and O
+// are fp32; P is rounded to the cache's type for the second product, as the operand has to be, against a maximum that
+// is exact for the warp's own keys.
+template <typename T, int D, int kRowWarps>
+__global__ void __launch_bounds__(160, 2)
+decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+              const __grid_constant__ DecodeParams p) {
+  using Cfg = DecodeCfg<D, kRowWarps>;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + Cfg::kOffBars);
+  uint64_t* empty = full + Cfg::kStages;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(empty + Cfg::kStages);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < Cfg::kStages; ++i) {
+      mbar_init(full + i, 1);
+      mbar_init(empty + i, 4);
+    }
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  __syncthreads();
+  griddep_wait();
+  DecodeWalk walk;
+  walk.start(p, blockIdx.x, lane);
+  griddep_launch();
+  int kv_head, row_tile, t0, t1, stage = 0;
+  uint32_t phase = 0;
+
+  if (warp == 4) {
+    // ---- loads: lane i brings box i of the tile's keys and of its values ----
+    const int boxes = kDecodeKeys / p.box_rows;
+    const uint32_t box_bytes = p.box_rows * D * 2;
+    bool ok = true;
+    while (ok && walk.next(p, kv_head, row_tile, t0, t1)) {
+      const int lo = p.window_left >= 0 && walk.length - walk.count > p.window_left
+                         ? walk.length - walk.count - p.window_left : 0;
+      const int* table = p.cache.page_table + walk.b * p.cache.table_stride;
+      auto page_of = [&](int tile) {  // -1: the box holds nothing that is seen
+        const int key = (walk.first + tile) * kDecodeKeys + lane * p.box_rows;
+        if (lane >= boxes || tile >= t1 || key >= walk.length || key + p.box_rows <= lo) return -1;
+        const int page = table[key / p.cache.page_size];
+        if (page >= 0 && page < p.cache.num_pages) return page;
+        atomicExch(p.cache.bad_index, 1);
+        return -1;
+      };
+      int page = page_of(t0);
+      for (int t = t0; t < t1; ++t) {
+        const int next_page = page_of(t + 1);
+        ok = mbar_wait_warp(empty + stage, phase ^ 1, abort_flag);
+        if (!ok) break;
+        const unsigned here = __ballot_sync(0xffffffffu, page >= 0);
+        if (lane == 0) mbar_arrive_expect_tx(full + stage, 2 * box_bytes * __popc(here));
+        __syncwarp();
+        if (page >= 0) {
+          uint8_t* dst = smem + stage * 2 * Cfg::kHalfBytes + lane * box_bytes;
+          const int row = ((walk.first + t) * kDecodeKeys + lane * p.box_rows) % p.cache.page_size;
+          tma_load_5d(dst, &map_k, full + stage, 0, row, 0, kv_head, page);
+          tma_load_5d(dst + Cfg::kHalfBytes, &map_v, full + stage, 0, row, 0, kv_head, page);
+        }
+        page = next_page;
+        if (++stage == Cfg::kStages) stage = 0, phase ^= 1;
+      }
+    }
+    if (!ok && lane == 0) {
+      atomicExch(p.status, 1);
+      for (int i = 0; i < 64; ++i) __nanosleep(2000);  // loads in flight land before the CTA retires
+    }
+    return;
+  }
+
+  // ---- compute ----
+  const int row_warp = warp % kRowWarps, key_warp = warp / kRowWarps;
+  const int quad = lane >> 2, in_quad = lane & 3;  // fragments: rows quad and quad + 8, columns 2 * in_quad and the next
+  const int rows = p.group * p.cache.tokens;
+  // where this lane's rows of the operands of ldmatrix start: K as [key][d], V (transposed on the way) as [key][d]
+  const int k_row = key_warp * Cfg::kWarpKeys + (lane >> 4) * 8 + (lane & 7), k_chunk = (lane >> 3) & 1;
+  const int v_row = key_warp * Cfg::kWarpKeys + (lane & 15), v_chunk = lane >> 4;
+  const int box_shift = __ffs(p.box_rows) - 1;
+  auto row_base = [&](int row) {  // of a row of the tile, first 128 bytes; its other panel is box_rows * 128 further
+    return (row >> box_shift) * (p.box_rows * D * 2) + (row & (p.box_rows - 1)) * 128;
+  };
+  const uint32_t panel = p.box_rows * 128;
+  bool ok = true;  // once a wait has run out, the warp goes on without its tiles: the others may wait for it
+
+  while (walk.next(p, kv_head, row_tile, t0, t1)) {
+    // this thread's two rows
+    uint32_t qf[D / 16][4];
+    float slope[2];
+    int last_key[2], out_row[2];  // the last key that the row sees; its place in the outputs, -1: there is none
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int r = row_tile * Cfg::kRows + row_warp * 16 + quad + 8 * i;
+      const int t = r / p.group, head = kv_head * p.group + r % p.group;
+      const bool there = r < rows, real = there && t < walk.count;
+      out_row[i] = there ? (walk.b * p.q_heads + head) * p.cache.tokens + t : -1;
+      last_key[i] = real ? walk.length - walk.count + t : -1;
+      slope[i] = real && p.alibi_slopes ? p.alibi_slopes[head] * 1.4426950408889634f : 0.f;
+      const T* q = static_cast<const T*>(p.q.data) + walk.b * p.q.batch_stride + head * p.q.head_stride +
+                   t * p.q.token_stride + 2 * in_quad;
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) {
+        qf[k][i] = real ? *reinterpret_cast<const uint32_t*>(q + 16 * k) : 0u;
+        qf[k][2 + i] = real ? *reinterpret_cast<const uint32_t*>(q + 16 * k + 8) : 0u;
+      }
+    }
+    const int first_query = walk.length - walk.count;
+    float o[D / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+#pragma unroll
+    for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+
+    for (int t = t0; t < t1; ++t) {
+      ok = ok && mbar_wait_warp(full + stage, phase, abort_flag);
+      if (ok) {
+        const int key0 = (walk.first + t) * kDecodeKeys;
+        const uint32_t k_smem = smem_u32(smem + stage * 2 * Cfg::kHalfBytes), v_smem = k_smem + Cfg::kHalfBytes;
+        float s[Cfg::kWarpKeys / 8][4];
+#pragma unroll
+        for (int n = 0; n < Cfg::kWarpKeys / 16; ++n) {
+          const uint32_t base = k_smem + row_base(k_row + 16 * n);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[2 * n][i] = s[2 * n + 1][i] = 0.f;
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k) {
+            uint32_t b[4];
+            ldsm4(base + (k / 4) * panel + ((((k % 4) * 2 + k_chunk) ^ (k_row & 7)) << 4), b);
+            mma16816<T>(s[2 * n], qf[k], b[0], b[1]);
+            mma16816<T>(s[2 * n + 1], qf[k], b[2], b[3]);
+          }
+        }
+        // does every row see every key of the tile?
+        const bool cut = key0 + kDecodeKeys > first_query + 1 ||
+                         (p.window_left >= 0 && key0 < walk.length - 1 - p.window_left);
+        const int warp_key = key0 + key_warp * Cfg::kWarpKeys + 2 * in_quad;
+        float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int n = 0; n < Cfg::kWarpKeys / 8; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int key = warp_key + 8 * n + (i & 1), r = i >> 1;
+            float x = s[n][i] * p.scale_log2;
+            if (p.alibi_slopes) x = fmaf(-slope[r], fabsf(static_cast<float>(last_key[r] - key)), x);
+            if (cut && (key > last_key[r] || (p.window_left >= 0 && key < last_key[r] - p.window_left))) x = -INFINITY;
+            s[n][i] = x;
+            top[r] = fmaxf(top[r], x);
+          }
+        float scale[2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
+          top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
+          top[r] = fmaxf(top[r], m[r]);
+        }
+        if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1])) {
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            scale[r] = top[r] == -INFINITY ? 1.f : ex2_approx(m[r] - top[r]);
+            m[r] = top[r];
+            l[r] *= scale[r];
+          }
+#pragma unroll
+          for (int n = 0; n < D / 8; ++n) {
+            o[n][0] *= scale[0];
+            o[n][1] *= scale[0];
+            o[n][2] *= scale[1];
+            o[n][3] *= scale[1];
+          }
+        }
+        const float off[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
+#pragma unroll
+        for (int n = 0; n < Cfg::kWarpKeys / 16; ++n) {
+          uint32_t pf[4];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float* x = s[2 * n + h];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = ex2_approx(x[i] - off[i >> 1]);
+            l[0] += x[0] + x[1];
+            l[1] += x[2] + x[3];
+            pf[2 * h] = from_floats<T>(x[0], x[1]);
+            pf[2 * h + 1] = from_floats<T>(x[2], x[3]);
+          }
+          const uint32_t base = v_smem + row_base(v_row + 16 * n);
+          if (cut) {
+            // what lies behind the last token, or in pages in front of the window, is not the sequence's: any bits at all,
+            // and 0 * NaN is NaN
+            uint32_t keep[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int key = warp_key + 16 * n + 8 * h;
+              const int lo = p.window_left >= 0 ? first_query - p.window_left : 0;
+              keep[h] = (key < walk.length && key >= lo ? 0xffffu : 0u) |
+                        (key + 1 < walk.length && key + 1 >= lo ? 0xffff0000u : 0u);
+            }
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d) {
+              uint32_t b[4];
+              ldsm4_trans(base + (d / 4) * panel + ((((d % 4) * 2 + v_chunk) ^ (v_row & 7)) << 4), b);
+              mma16816<T>(o[2 * d], pf, b[0] & keep[0], b[1] & keep[1]);
+              mma16816<T>(o[2 * d + 1], pf, b[2] & keep[0], b[3] & keep[1]);
+            }
+          } else {
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d) {
+              uint32_t b[4];
+              ldsm4_trans(base + (d / 4) * panel + ((((d % 4) * 2 + v_chunk) ^ (v_row & 7)) << 4), b);
+              mma16816<T>(o[2 * d], pf, b[0], b[1]);
+              mma16816<T>(o[2 * d + 1], pf, b[2], b[3]);
+            }
+          }
+        }
+      }
+      __syncwarp();
+      mbar_arrive_lane0(empty + stage, lane);
+      if (++stage == Cfg::kStages) stage = 0, phase ^= 1;
+    }
+
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+    }
+    if constexpr (Cfg::kKeyWarps > 1) {
+      // join the key warps: a common maximum, then the outputs pairwise through shared memory
+      float2* ml = reinterpret_cast<float2*>(smem + Cfg::kOffMl);
+      if (in_quad == 0) {
+        ml[warp * 16 + quad] = make_float2(m[0], l[0]);
+        ml[warp * 16 + quad + 8] = make_float2(m[1], l[1]);
+      }
+      compute_sync();
+      float scale[2];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        float top = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < Cfg::kKeyWarps; ++w) top = fmaxf(top, ml[(w * kRowWarps + row_warp) * 16 + quad + 8 * r].x);
+        const float off = top == -INFINITY ? 0.f : top;
+#pragma unroll
+        for (int w = 0; w < Cfg::kKeyWarps; ++w) {
+          const float2 other = ml[(w * kRowWarps + row_warp) * 16 + quad + 8 * r];
+          sum += other.y * ex2_approx(other.x - off);
+        }
+        scale[r] = ex2_approx(m[r] - off);
+        m[r] = top;
+        l[r] = sum;
+      }
+#pragma unroll
+      for (int step = Cfg::kKeyWarps / 2; step > 0; step /= 2) {
+        float2* buf = reinterpret_cast<float2*>(smem + Cfg::kOffJoin) +
+                      ((key_warp % step) * kRowWarps + row_warp) * (16 * D / 2) + lane;
+        if (key_warp >= step && key_warp < 2 * step) {
+#pragma unroll
+          for (int n = 0; n < D / 8; ++n) {
+            const float c0 = step == Cfg::kKeyWarps / 2 ? scale[0] : 1.f, c1 = step == Cfg::kKeyWarps / 2 ? scale[1] : 1.f;
+            buf[(2 * n) * 32] = make_float2(o[n][0] * c0, o[n][1] * c0);
+            buf[(2 * n + 1) * 32] = make_float2(o[n][2] * c1, o[n][3] * c1);
+          }
+        }
+        compute_sync();
+        if (key_warp < step) {
+#pragma unroll
+          for (int n = 0; n < D / 8; ++n) {
+            const float c0 = step == Cfg::kKeyWarps / 2 ? scale[0] : 1.f, c1 = step == Cfg::kKeyWarps / 2 ? scale[1] : 1.f;
+            const float2 a = buf[(2 * n) * 32], c = buf[(2 * n + 1) * 32];
+            o[n][0] = fmaf(o[n][0], c0, a.x);
+            o[n][1] = fmaf(o[n][1], c0, a.y);
+            o[n][2] = fmaf(o[n][2], c1, c.x);
+            o[n][3] = fmaf(o[n][3], c1, c.y);
+          }
+        }
+        compute_sync();
+      }
+    }
+    if (key_warp == 0) {
+      const bool whole = t0 == 0 && t1 == walk.tiles;
+      const long long part =
+          (2ll * blockIdx.x + (walk.at - (t1 - t0) == walk.begin ? 0 : 1)) * Cfg::kRows + row_warp * 16 + quad;
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        if (out_row[r] < 0) continue;
+        const bool real = last_key[r] >= 0;
+        if (whole) {
+          const float inv = real && l[r] != 0.f ? 1.f / l[r] : 0.f;
+          T* to = static_cast<T*>(p.o) + static_cast<long long>(out_row[r]) * D + 2 * in_quad;
+#pragma unroll
+          for (int n = 0; n < D / 8; ++n)
+            *reinterpret_cast<uint32_t*>(to + 8 * n) =
+                real ? from_floats<T>(o[n][2 * r] * inv, o[n][2 * r + 1] * inv) : 0u;
+          if (p.lse && in_quad == 0) p.lse[out_row[r]] = real ? (m[r] + log2f(l[r])) * 0.6931471805599453f : -INFINITY;
+        } else {
+          float* to = p.part_o + (part + 8 * r) * D + 2 * in_quad;
+#pragma unroll
+          for (int n = 0; n < D / 8; ++n) *reinterpret_cast<float2*>(to + 8 * n) = make_float2(o[n][2 * r], o[n][2 * r + 1]);
+          if (in_quad == 0)
+            *reinterpret_cast<float2*>(p.part_ml + (part + 8 * r) * 2) = make_float2(m[r], l[r]);
+        }
+      }
+    }
+  }
+  if (!ok && lane == 0) atomicExch(p.status, 1);
+}
+
+// A warp a row: nothing to do where one CTA had the whole item; else the parts are joined in the order of the line. Rows
+// of sequences without keys, and rows of padding, are set to O = 0 and a log-sum-exp of -infinity.
+template <typename T, int D>
+__global__ void __launch_bounds__(128) decode_join_kernel(const __grid_constant__ DecodeParams p, int tile_rows) {
+  const int lane = threadIdx.x & 31;
+  const long long row = blockIdx.x * 4ll + (threadIdx.x >> 5);
+  griddep_wait();
+  if (row >= static_cast<long long>(p.cache.batch) * p.q_heads * p.cache.tokens) return;
+  const int t = static_cast<int>(row % p.cache.tokens);
+  const int bh = static_cast<int>(row / p.cache.tokens), head = bh % p.q_heads, b = bh / p.q_heads;
+  int first, tiles, length, count;
+  DecodeLine::tiles_of(p, b, first, tiles, length, count);
+  constexpr int kOwn = D / 32;  // elements of a lane
+  float o[kOwn], m = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int i = 0; i < kOwn; ++i) o[i] = 0.f;
+  if (tiles > 0 && t < count) {
+    long long all, before;
+    DecodeLine::sum(p, b, all, before, lane);
+    const int r = t * p.group + head % p.group, item = head / p.group * p.row_tiles + r / tile_rows;
+    const long long share = DecodeLine::share_of(p, all);
+    const long long s = before * p.cache.kv_heads * p.row_tiles + static_cast<long long>(item) * tiles;
+    const long long c0 = s / share, c1 = (s + tiles - 1) / share;
+    if (c0 == c1) return;
+    auto part = [&](long long c) { return (2 * c + (c == c0 && s != c * share ? 1 : 0)) * tile_rows + r % tile_rows; };
+    for (long long c = c0 + lane; c <= c1; c += 32) m = fmaxf(m, p.part_ml[2 * part(c)]);
+#pragma unroll
+    for (int i = 16; i > 0; i >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, i));
+    const float off = m == -INFINITY ? 0.f : m;
+#pragma unroll 4
+    for (long long c = c0; c <= c1; ++c) {
+      const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + 2 * part(c));
+      const float scale = ex2_approx(ml.x - off);
+      const float* from = p.part_o + part(c) * D + lane * kOwn;
+      l = fmaf(ml.y, scale, l);
+#pragma unroll
+      for (int i = 0; i < kOwn; i += 2) {
+        const float2 x = *reinterpret_cast<const float2*>(from + i);
+        o[i] = fmaf(x.x, scale, o[i]);
+        o[i + 1] = fmaf(x.y, scale, o[i + 1]);
+      }
+    }
+  }
+  const float inv = l != 0.f ? 1.f / l : 0.f;
+  T* to = static_cast<T*>(p.o) + row * D + lane * kOwn;
+#pragma unroll
+  for (int i = 0; i < kOwn; i += 2) *reinterpret_cast<uint32_t*>(to + i) = from_floats<T>(o[i] * inv, o[i + 1] * inv);
+  if (p.lse && lane == 0) p.lse[row] = (m + log2f(l)) * 0.6931471805599453f;
+}
+
+}  // namespace fa

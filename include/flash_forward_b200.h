@@ -22,7 +22,8 @@ enum {
   FA_INVALID_ARG = 1,    /* null or misaligned pointer, non-positive size */
   FA_UNSUPPORTED = 2,    /* head_dim not 64/128, a combination a kernel lacks, device is not sm_100 */
   FA_CUDA_ERROR = 3,     /* a CUDA runtime/driver call failed; see flash_forward_last_error() */
-  FA_DEVICE_TIMEOUT = 4  /* a bounded wait inside the kernel gave up (status word set) */
+  FA_DEVICE_TIMEOUT = 4, /* a bounded wait inside the kernel gave up (status word set) */
+  FA_BAD_INDEX = 5       /* a page, length, count or position in device memory was out of range (flash_forward_check) */
 };
 
 /* Attention forward O = softmax(scale * Q K^T + mask) V, asynchronous on `stream`.
@@ -151,8 +152,8 @@ int flash_forward_host(const void* q_host, const void* k_host, const void* v_hos
                        int window_right, void* workspace, size_t workspace_bytes, int chunk_heads);
 size_t flash_forward_host_workspace_bytes(int seqlen, int head_dim, int chunk_heads);
 
-/* Waits for `stream`, then reads and clears the current device's status word. Returns FA_OK,
- * FA_DEVICE_TIMEOUT, or FA_CUDA_ERROR. Replaces the reference's CUDA_CHECK(cudaDeviceSynchronize())
+/* Waits for `stream`, then reads and clears the current device's status words. Returns FA_OK,
+ * FA_DEVICE_TIMEOUT, FA_BAD_INDEX (flash_cache_append, flash_decode), or FA_CUDA_ERROR. Replaces the reference's CUDA_CHECK(cudaDeviceSynchronize())
  * + exit (src/flash_forward.h:654-655). There is ONE status word per device, not per stream: a
  * time-out raised by a launch on another stream of the device is reported (and consumed) by whichever
  * check comes first. Like flash_forward() it allocates the device's scratch on first use; hosts that
@@ -231,6 +232,83 @@ int flash_forward_noalloc(const void* q, const void* k, const void* v, void* o, 
  * returns FA_OK or FA_DEVICE_TIMEOUT. The word is written by every call on that slot. No counterpart
  * in the reference. */
 int flash_forward_noalloc_check(void* stream, int slot);
+
+/* ---- paged key-value cache ---------------------------------------------------------------
+ * The keys and values of many sequences in one pool of pages, for generation token by token. No counterpart in the
+ * reference. Pages hold page_size tokens (a multiple of 8) of every key head; sequence b has its tokens, in order, in the
+ * pages that row b of page_table names: token j is row j % page_size of page page_table[b][j / page_size]. Nothing behind a
+ * sequence's last token is read or written: neither entries of the table nor the rest of its last page, which may hold
+ * anything. Sequences may share pages that are only read.
+ *
+ * lengths[b] counts the tokens of sequence b with the new ones of the call; counts[b], where given, of the call's `tokens`
+ * rows those that are new tokens: the first counts[b], the rest is padding (counts == NULL: all of them). So new row t of
+ * sequence b is its token lengths[b] - counts[b] + t, both for flash_cache_append, which puts it there, and for
+ * flash_decode, whose query t sees the tokens up to that one. A length of 0 is a sequence without keys.
+ *
+ * page_table, lengths and counts are read on the device when the kernels run, so that a captured call can be replayed with
+ * new contents. The kernels check what they read there: a page outside [0, num_pages), a length outside [0, max_pages *
+ * page_size], a count outside [0, tokens] or above the length, a position without angles is skipped or cut to the range and
+ * reported by flash_forward_check() as FA_BAD_INDEX; what the call wrote for that sequence is then undefined. */
+enum { FA_FP16 = 0, FA_BF16 = 1 };
+
+typedef struct fa_paged_cache {
+  void* k;                /* device memory, 16-byte aligned; the element (page, head, token, i) of K lies at */
+  void* v;                /* k + page * page_stride + head * head_stride + token * token_stride + i, and so for V */
+  long long page_stride;  /* in elements, multiples of 8: pages may be [head][token] or [token][head] */
+  long long head_stride;
+  long long token_stride;
+  int num_pages;
+  int page_size;
+  int kv_heads;
+  int head_dim;           /* 64 or 128 */
+  int dtype;              /* FA_FP16 or FA_BF16: of the cache and of all tensors of a call on it */
+  const int* page_table;  /* device, [batch][table_stride], of which max_pages entries belong to a sequence */
+  long long table_stride;
+  int max_pages;
+  const int* lengths;     /* device, [batch] */
+  const int* counts;      /* device, [batch], or NULL */
+} fa_paged_cache;
+
+/* Rows [batch][head][token] of head_dim contiguous elements: row (b, h, t) at data + b * batch_stride + h * head_stride +
+ * t * token_stride, in elements, multiples of 8; data 16-byte aligned. */
+typedef struct fa_rows {
+  const void* data;
+  long long batch_stride;
+  long long head_stride;
+  long long token_stride;
+} fa_rows;
+
+/* Writes the new keys and values (k, v: batch x kv_heads x tokens rows) to their places in the cache. Asynchronous on
+ * `stream`, one launch.
+ *   rotary     device, float [rotary_positions][rotary_dim], 16-byte aligned: for every position rotary_dim / 2 cosines,
+ *              then as many sines. Keys are rotated by their position's angles on the way: with i < rotary_dim / 2, the
+ *              elements (i, i + rotary_dim / 2), or (2i, 2i + 1) if `interleaved`, become (x cos_i - y sin_i, x sin_i + y
+ *              cos_i) in fp32, rounded once; elements from rotary_dim on stay as they are. rotary_dim: a multiple of 16.
+ *              NULL: nothing is rotated.
+ *   q, q_out   the new tokens' queries (batch x q_heads x tokens rows) rotated in the same way into q_out, contiguous
+ *              [batch][q_heads][tokens][head_dim]; rows of padding become 0. NULL, NULL and q_heads 0: none. q_out may be
+ *              q's own memory if q is laid out like it.
+ * The caller sees to it that no two new tokens of a call have the same place. */
+int flash_cache_append(const fa_paged_cache* cache, const fa_rows* k, const fa_rows* v, const fa_rows* q, void* q_out,
+                       int batch, int tokens, int q_heads, const float* rotary, int rotary_dim, int rotary_positions,
+                       int interleaved, void* stream);
+
+/* Attention of the newest `tokens` tokens of every sequence (one for a step of generation, several to check guessed ones)
+ * over the cache: O = softmax(scale * q K^T + mask) V. Query head h reads key head h / (q_heads / kv_heads); q_heads is a
+ * multiple of kv_heads. Query t of sequence b, at position i = lengths[b] - counts[b] + t, sees the keys j <= i, and with
+ * window_left >= 0 those with j >= i - window_left; pages that lie in front of every query's window are not read.
+ * alibi_slopes (NULL, or q_heads floats on the device) as for flash_forward_alibi(); softmax_scale as for flash_forward().
+ *   o    contiguous [batch][q_heads][tokens][head_dim], 16-byte aligned
+ *   lse  NULL, or float [batch][q_heads][tokens]: the log-sum-exp as in flash_forward_lse()
+ * Rows of padding, and of sequences without keys, are O = 0 and lse = -infinity.
+ * workspace: flash_decode_workspace_bytes() bytes of device memory, 16-byte aligned, with any contents; calls that may
+ * overlap on the GPU need one each. Asynchronous on `stream`, two launches; may be captured into a CUDA graph once a call
+ * has been made on the device. Two calls with the same arguments give the same bits; how a sequence's keys are shared out
+ * depends on the lengths of the whole batch. */
+int flash_decode(const fa_paged_cache* cache, const fa_rows* q, void* o, float* lse, int batch, int tokens, int q_heads,
+                 float softmax_scale, int window_left, const float* alibi_slopes, void* workspace, size_t workspace_bytes,
+                 void* stream);
+size_t flash_decode_workspace_bytes(int tokens, int q_heads, int kv_heads, int head_dim);
 
 /* Frees the per-device status words, events and streams this library created, and forgets what it
  * learned about each device (scratch addresses, kernel attributes), so that it can be used again

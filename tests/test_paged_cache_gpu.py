@@ -1,0 +1,303 @@
+"""flash_cache_append and flash_decode on the GPU against the plain 64-bit implementation.
+
+Tolerances. Append: an element is a * cos - b * sin in fp32 (two roundings of products, one of the sum: 3 * 2^-24 of |a| +
+|b| at most) rounded once to the cache's type: half a step of the value and that. Decode: P is rounded to the cache's type
+(half a step each, relative: eps/2 of sum P|V|), the output once more (eps/2 of |O|); the scores are fp32 sums of d products
+whose error moves P by a factor that 2^-13 of sum P|V| covers (scores of up to 2^6 with a relative error of 2^-20 give 2^-14
+each, on a term and on the sum that it is divided by)."""
+import math
+
+import pytest
+import torch
+
+import paged_cache_oracle as oracle
+
+pytestmark = pytest.mark.gpu
+LSE_TOL = 5e-4  # as for flash_forward_lse: fp32 scores, ex2 and lg2
+
+
+def check_decode(pkg, batch, q, dtype_eps=None, counts=False, **kw):
+    slopes = kw.get("alibi_slopes")
+    want, want_lse, size = oracle.decode(batch, q, **kw)
+    gkw = dict(kw, alibi_slopes=None if slopes is None else slopes.cuda())
+    out, lse = pkg.attention_decode(q.cuda(), *batch.cuda(), counts=batch.cuda_counts() if counts else None,
+                                    return_lse=True, **gkw)
+    pkg.check(torch.cuda.current_stream().cuda_stream)
+    out, lse = out.cpu(), lse.cpu()
+    assert out.is_contiguous() and torch.isfinite(out).all()
+    eps = torch.finfo(batch.dtype).eps / 2
+    bound = eps * (want.abs() + size) + 2.0 ** -13 * size + torch.finfo(batch.dtype).tiny
+    err = (out.double() - want).abs()
+    assert (err <= bound).all(), float((err / bound).max())
+    empty = torch.isinf(want_lse)
+    assert (lse[empty] == -math.inf).all() and (out[empty] == 0).all()
+    assert ((lse[~empty].double() - want_lse[~empty]).abs() <= LSE_TOL).all()
+    return out, lse
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("head_dim", [64, 128])
+@pytest.mark.parametrize("q_heads,kv_heads,tokens,page,lengths", [
+    (4, 4, 1, 16, [1]),                              # one key
+    (8, 2, 1, 16, [1, 2, 15, 16, 17, 63, 64, 65]),   # around the ends of pages and tiles
+    (8, 8, 1, 8, [129, 0, 77, 0]),                   # sequences without keys between others
+    (6, 1, 1, 24, [0, 0, 300]),                      # pages that end inside a tile, first sequences empty
+    (40, 2, 1, 128, [500, 41]),                      # 20 queries a key head: two groups of 16 rows
+    (70, 1, 1, 64, [130]),                           # 70: more than a tile of 64 rows
+    (7, 1, 3, 32, [3, 4, 200]),                      # several tokens, sequences that hold nothing else
+    (16, 4, 8, 256, [600, 8]),
+    (1, 1, 1, 16, [4100]),                           # cut among many CTAs
+])
+def test_decode(pkg, dtype, head_dim, q_heads, kv_heads, tokens, page, lengths):
+    b = oracle.Batch(len(lengths) + head_dim, lengths, [min(tokens, n) for n in lengths], tokens, kv_heads, head_dim, page,
+                     dtype)
+    check_decode(pkg, b, b.rows(q_heads))
+
+
+@pytest.mark.parametrize("window", [0, 1, 63, 64, 200, 100000, 2 ** 31 - 1])
+@pytest.mark.parametrize("alibi", [False, True])
+def test_decode_window_and_alibi(pkg, window, alibi):
+    b = oracle.Batch(5, [1, 64, 65, 333, 700], [1, 3, 3, 3, 3], 3, 2, 64, 16, "fp16")
+    slopes = torch.tensor([0.5, 0.01, -0.02, 0.0]) if alibi else None
+    check_decode(pkg, b, b.rows(4), counts=True, window_left=window, alibi_slopes=slopes)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_decode_many_sequences(pkg, dtype):
+    """More sequences than lanes of a warp, lengths of every kind, some of them empty."""
+    lengths = [(37 * i * i) % 400 for i in range(150)]
+    b = oracle.Batch(3, lengths, [min(1, n) for n in lengths], 1, 2, 64, 16, dtype, token_major=True)
+    check_decode(pkg, b, b.rows(4))
+
+
+def test_decode_counts(pkg):
+    """A padded batch: rows behind a sequence's count are 0 and -infinity, in tiles that no mask cuts too."""
+    b = oracle.Batch(4, [500, 300, 4, 0, 129], [4, 1, 2, 0, 0], 4, 2, 128, 16, "fp16")
+    check_decode(pkg, b, b.rows(6), counts=True)
+
+
+@pytest.mark.parametrize("fill", [math.nan, math.inf])
+@pytest.mark.parametrize("window", [-1, 70])
+def test_decode_ignores_what_is_not_the_sequences(pkg, fill, window):
+    """The rest of last pages, pages that no sequence names and pages in front of the window hold anything."""
+    b = oracle.Batch(6, [1, 40, 200, 317], [1, 1, 1, 1], 1, 2, 128, 32, "fp16", fill=fill)
+    if window >= 0:
+        for i, n in enumerate(b.lengths):
+            gone = max(0, n - 1 - window)
+            for j in range(gone):  # tokens in front of the window: overwritten; whole pages: given back
+                b.k_pages[b.table[i, j // 32], :, j % 32] = fill
+                b.v_pages[b.table[i, j // 32], :, j % 32] = fill
+            b.table[i, :gone // 32] = -1
+    check_decode(pkg, b, b.rows(4), window_left=window)
+
+
+def test_decode_large_scores_and_scale(pkg):
+    b = oracle.Batch(8, [1000, 90], [1, 1], 1, 1, 64, 16, "fp16")
+    check_decode(pkg, b, b.rows(2), softmax_scale=0.5)  # scores of +-15
+    q = b.rows(2)
+    out, _ = pkg.attention_decode(q.cuda() * 100, *b.cuda(), return_lse=True)  # scores of hundreds: one key takes all
+    want, _, _ = oracle.decode(b, q * 100)
+    assert torch.isfinite(out).all() and ((out.cpu().double() - want).abs() <= 2e-2).all()
+
+
+def test_decode_nan_and_infinity_where_they_are_seen(pkg):
+    b = oracle.Batch(9, [100, 100], [1, 1], 1, 1, 64, 16, "fp16")
+    b.k_pages[b.table[1, 2], 0, 3, 5] = math.nan
+    out, lse = pkg.attention_decode(b.rows(4).cuda(), *b.cuda(), return_lse=True)
+    assert torch.isfinite(out[0]).all() and torch.isnan(out[1]).all() and torch.isnan(lse[1]).all()
+
+
+def test_decode_is_the_same_every_time_and_on_views(pkg):
+    b = oracle.Batch(10, [3000, 17, 900], [2, 2, 2], 2, 2, 128, 16, "bf16")
+    args, q = b.cuda(), b.rows(8).cuda()
+    first = pkg.attention_decode(q, *args, return_lse=True)
+    # the same rows out of a fused projection, a table with longer rows, the pool in the middle of a larger one
+    fused = torch.randn((3, 2, 12, 128), device="cuda").bfloat16()
+    fused[:, :, 2:10] = q.transpose(1, 2)
+    table = torch.full((3, args[2].shape[1] + 5), -1, dtype=torch.int32, device="cuda")
+    table[:, :args[2].shape[1]] = args[2]
+    pools = []
+    for x in args[:2]:
+        wide = torch.full((x.shape[0] + 2, x.shape[1] + 3, x.shape[2], x.shape[3]), math.nan, device="cuda", dtype=x.dtype)
+        wide[1:-1, 2:4] = x
+        pools.append(wide[1:-1, 2:4])
+    second = pkg.attention_decode(fused.transpose(1, 2)[:, 2:10], *pools, table[:, :args[2].shape[1]], args[3],
+                                  return_lse=True)
+    for x, y in zip(first, second):
+        assert torch.equal(x, y)
+
+
+def test_decode_far_offsets(pkg):
+    """A pool of more than 2^32 elements: the sequence's pages lie at its end."""
+    pages, heads, page, d = 40000, 8, 128, 128  # 5.2e9 elements a tensor
+    k = torch.zeros((pages, heads, page, d), dtype=torch.float16, device="cuda")
+    v = torch.zeros_like(k)
+    b = oracle.Batch(11, [200], [1], 1, heads, d, page, "fp16", spare=0)
+    k[-2:], v[-2:] = b.k_pages.cuda(), b.v_pages.cuda()
+    table = b.table.clone()
+    table[:, :2] += pages - 2
+    q = b.rows(8)
+    out, lse = pkg.attention_decode(q.cuda(), k, v, table.cuda(), b.cuda()[3], return_lse=True)
+    near, near_lse = check_decode(pkg, b, q)
+    assert torch.equal(out.cpu(), near) and torch.equal(lse.cpu(), near_lse)
+    # and the append writes there
+    new = b.rows(8)
+    pkg.cache_append(new.cuda(), new.cuda(), k, v, table.cuda(), b.cuda()[3])
+    pkg.check(torch.cuda.current_stream().cuda_stream)
+    assert torch.equal(k[table[0, 1], :, 199 - 128].cpu(), new[0, :, 0])
+    assert int((k != 0).any(-1).sum()) <= 200 * heads
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("head_dim,rotary_dim,token_major", [(64, 64, False), (64, 16, True), (128, 128, True),
+                                                             (128, 96, False), (128, 32, False)])
+def test_append(pkg, dtype, interleaved, head_dim, rotary_dim, token_major):
+    lengths, counts = [1, 17, 5, 40, 0, 33], [1, 5, 5, 2, 0, 0]
+    b = oracle.Batch(20 + rotary_dim, lengths, counts, 5, 2, head_dim, 16, dtype, token_major=token_major)
+    k, v, q = b.rows(2), b.rows(2), b.rows(6)
+    k[1, 0, 2, 3] = math.inf  # copied or turned like any other
+    rotary = oracle.angles(64, rotary_dim)
+    want = oracle.append(b, k, v, q, rotary, interleaved)
+    k_pages, v_pages, table, lens = b.cuda()
+    before = k_pages.clone()
+    turned = pkg.cache_append(k.cuda(), v.cuda(), k_pages, v_pages, table, lens, counts=b.cuda_counts(), q=q.cuda(),
+                              rotary=rotary.cuda(), interleaved=interleaved)
+    pkg.check(torch.cuda.current_stream().cuda_stream)
+    assert torch.equal(v_pages.cpu().double(), want[1])
+    eps = torch.finfo(b.dtype).eps / 2
+    for got, w, src in ((k_pages.cpu(), want[0], 6.0), (turned.cpu(), want[2], 6.0)):
+        same = torch.isinf(w) | torch.isnan(w)
+        assert torch.equal(torch.isnan(got[same]), torch.isnan(w[same]))
+        err = (got.double() - w).abs()[~same]
+        # |a| + |b| of normal values is below 12
+        assert (err <= eps * w[~same].abs() + 3 * 2.0 ** -24 * 2 * src + torch.finfo(b.dtype).tiny).all()
+    touched = torch.zeros(k_pages.shape[0], 16, dtype=torch.bool)
+    for i, (n, c) in enumerate(zip(lengths, counts)):
+        for j in range(n - c, n):
+            touched[b.table[i, j // 16], j % 16] = True
+    untouched = ~touched[:, None, :, None].expand(k_pages.shape)
+    assert torch.equal(k_pages.cpu()[untouched], before.cpu()[untouched])
+
+
+def test_append_without_rotation_and_in_place(pkg):
+    b = oracle.Batch(31, [9, 30], [3, 3], 3, 4, 64, 8, "fp16")
+    k, v = b.rows(4), b.rows(4)
+    want = oracle.append(b, k, v)
+    args = b.cuda()
+    assert pkg.cache_append(k.cuda(), v.cuda(), *args) is None
+    assert torch.equal(args[0].cpu().double(), want[0]) and torch.equal(args[1].cpu().double(), want[1])
+    rotary, q = oracle.angles(32, 64).cuda(), b.rows(4).cuda().contiguous()
+    apart = pkg.cache_append(k.cuda(), v.cuda(), *args, q=q, rotary=rotary)
+    same = pkg.cache_append(k.cuda(), v.cuda(), *args, q=q, rotary=rotary, q_out=q)
+    assert same is q and torch.equal(q, apart)
+
+
+def test_bad_indices_are_reported(pkg):
+    """Pages, lengths, counts and positions outside their ranges become a status; the other sequences are unharmed."""
+    stream = torch.cuda.current_stream().cuda_stream
+
+    def reported():
+        with pytest.raises(pkg.FlashForwardError) as e:
+            pkg.check(stream)
+        assert e.value.code == pkg.FA_BAD_INDEX
+        pkg.check(stream)  # and forgotten
+
+    b = oracle.Batch(40, [40, 200], [2, 2], 2, 2, 64, 16, "fp16")
+    q, k = b.rows(4).cuda(), b.rows(2).cuda()
+    good = pkg.attention_decode(q, *b.cuda())
+    for page in (-1, b.k_pages.shape[0], 2 ** 30, -2 ** 31):
+        args = b.cuda()
+        args[2][0, 2] = page
+        out = pkg.attention_decode(q, *args)
+        reported()
+        assert torch.equal(out[1], good[1])
+        before = args[0].clone()
+        pkg.cache_append(k[:1], k[:1], args[0], args[1], args[2][:1], args[3][:1])
+        reported()
+        assert torch.equal(args[0], before)
+    for length in (-3, 10 ** 6, 2 ** 31 - 1):
+        args = b.cuda()
+        args[3][1] = length
+        args[2][1] = args[2][0, 0]  # every page of the row can be read
+        pkg.attention_decode(q, *args)
+        reported()
+        pkg.cache_append(k, k, *args)
+        reported()
+    for counts in ([3, 2], [-1, 2], [2, 2 ** 31 - 1]):
+        pkg.attention_decode(q, *b.cuda(), counts=torch.tensor(counts, dtype=torch.int32).cuda())
+        reported()
+    args = b.cuda()
+    before = args[0].clone()
+    pkg.cache_append(k, k, *args, q=q, rotary=oracle.angles(150, 64).cuda())  # sequence 1 is at 198
+    reported()
+    assert torch.equal(args[0][args[2][1, 12].item()], before[args[2][1, 12].item()])
+
+
+def test_generation_steps_captured_and_replayed(pkg):
+    """Append and decode of a step as one graph, replayed with lengths that grow, against the same steps by call."""
+    tokens, heads, kv_heads, d, page = 1, 8, 2, 64, 16
+    b = oracle.Batch(50, [30, 5, 64], [1, 1, 1], tokens, kv_heads, d, page, "fp16", spare=8)
+    spare = sorted(set(range(b.k_pages.shape[0])) - {int(x) for x in b.table.flatten() if x >= 0})
+    for i, need in enumerate([2, 1, 4]):  # room to grow
+        b.table[i, need] = spare[i]
+    rotary = oracle.angles(128, d).cuda()
+    steps = [(b.rows(kv_heads).cuda(), b.rows(kv_heads).cuda(), b.rows(heads).cuda()) for _ in range(4)]
+
+    def step(k, v, q, k_pages, v_pages, table, lengths):
+        turned = pkg.cache_append(k, v, k_pages, v_pages, table, lengths, q=q, rotary=rotary)
+        return pkg.attention_decode(turned, k_pages, v_pages, table, lengths, return_lse=True)
+
+    eager_args, want = b.cuda(), []
+    for s in steps:
+        want.append([x.clone() for x in step(*s, *eager_args)])
+        eager_args[3] += 1
+    args = b.cuda()
+    held = [torch.empty_like(x) for x in steps[0]]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(*held, *args)
+    for s, w in zip(steps, want):
+        for x, y in zip(held, s):
+            x.copy_(y)
+        graph.replay()
+        assert all(torch.equal(x, y) for x, y in zip(got, w))
+        args[3] += 1
+    pkg.check(torch.cuda.current_stream().cuda_stream)
+    assert torch.equal(args[0], eager_args[0]) and torch.equal(args[1], eager_args[1])
+
+
+def test_prompt_then_steps_is_the_forward(pkg):
+    """A prompt through attention_forward, its keys into the cache, then one token at a time: the rows that attention_forward
+    gives for the whole sequence."""
+    B, H, N, d, prompt = 2, 4, 150, 128, 131
+    g = torch.Generator(device="cuda").manual_seed(1)
+    q, k, v = (torch.randn((B, H, N, d), generator=g, device="cuda", dtype=torch.float16) for _ in range(3))
+    whole, lse = pkg.attention_forward(q, k, v, causal=True, return_lse=True)
+    k_pages, v_pages = (torch.full((20, H, 16, d), math.nan, device="cuda", dtype=torch.float16) for _ in range(2))
+    table = torch.randperm(20, device="cuda").int().view(2, 10)
+    lengths = torch.full((B,), prompt, dtype=torch.int32, device="cuda")
+    pkg.cache_append(k[:, :, :prompt], v[:, :, :prompt], k_pages, v_pages, table, lengths)
+    for i in range(prompt, N, 1):
+        lengths += 1
+        pkg.cache_append(k[:, :, i:i + 1], v[:, :, i:i + 1], k_pages, v_pages, table, lengths)
+        out, out_lse = pkg.attention_decode(q[:, :, i:i + 1], k_pages, v_pages, table, lengths, return_lse=True)
+        # both are within 2 eps/2 of sum P|V|, which is below 1.5 here, and of |O|
+        assert ((out[:, :, 0] - whole[:, :, i]).abs().float() <= 4 * 2.0 ** -11 * 1.5).all()
+        assert ((out_lse[:, :, 0] - lse[:, :, i]).abs() <= 2 * LSE_TOL).all()
+    pkg.check(torch.cuda.current_stream().cuda_stream)
+
+
+def test_on_two_streams(pkg):
+    b = oracle.Batch(60, [2500, 700], [1, 1], 1, 4, 128, 16, "fp16")
+    args, q = b.cuda(), b.rows(16).cuda()
+    want = pkg.attention_decode(q, *args)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = []
+    for _ in range(10):
+        for s in streams:
+            with torch.cuda.stream(s):
+                outs.append(pkg.attention_decode(q, *args))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, want) for x in outs)

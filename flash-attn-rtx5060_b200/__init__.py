@@ -45,6 +45,8 @@ EXPORTS = (
     "flash_forward_kv_range",
     "flash_forward_head_group",
     "flash_forward_shutdown",
+    "flash_backward",
+    "flash_backward_workspace_bytes",
     "flash_cache_append",
     "flash_decode",
     "flash_decode_workspace_bytes",
@@ -129,6 +131,10 @@ def _open():
     L.flash_forward_head_group.restype = i
     L.flash_forward_shutdown.argtypes = []
     L.flash_forward_shutdown.restype = i
+    L.flash_backward.argtypes = [vp] * 10 + [i, i, i, i, f, i, i, i, vp, vp, ctypes.c_size_t, vp]
+    L.flash_backward.restype = i
+    L.flash_backward_workspace_bytes.argtypes = [i, i, i]
+    L.flash_backward_workspace_bytes.restype = ctypes.c_size_t
     cache, rows = ctypes.POINTER(PagedCacheStruct), ctypes.POINTER(RowsStruct)
     L.flash_cache_append.argtypes = [cache, rows, rows, rows, vp, i, i, i, vp, i, i, i, vp]
     L.flash_cache_append.restype = i
@@ -351,6 +357,40 @@ def _enqueue_forward(device, torch, q, k, v, out, causal, window_left, window_ri
     if rc != FA_OK:
         _raise(rc)
     return (out, lse) if return_lse else out
+
+
+def attention_backward(q, k, v, out, lse, dout, causal=False, window_left=-1, window_right=-1, softmax_scale=0.0,
+                       alibi_slopes=None, dlse=None, dq=None, dk=None, dv=None):
+    """Gradients of attention_forward(q, k, v, ..., return_lse=True), whose results are `out` and `lse`, for the gradient
+    `dout` of out (and `dlse` of lse, if given): (dq, dk, dv), flash_backward of the C header.
+
+    All tensors as attention_forward takes and gives them; dout is made contiguous if it is not. dq, dk, dv, if given,
+    are contiguous tensors like q that are written.
+    """
+    import torch
+
+    dout = dout.contiguous()
+    _check_operands(torch, q, k, v, out, alibi_slopes)
+    device = q.get_device()
+
+    def fits(t, shape, dtype):
+        return t.is_cuda and t.get_device() == device and t.dtype == dtype and t.shape == shape and t.is_contiguous()
+    for name, t in (("out", out), ("dout", dout), ("dq", dq), ("dk", dk), ("dv", dv)):
+        if not (fits(t, q.shape, q.dtype) if t is not None else name[1:] in "qkv"):
+            raise AssertionError(f"{name} has to be like q, contiguous, on its device")
+    for name, t in (("lse", lse), ("dlse", dlse)):
+        if not (fits(t, q.shape[:3], torch.float32) if t is not None else name == "dlse"):
+            raise AssertionError(f"{name}: contiguous float32 [B, H, N] on q's device is needed")
+    dq, dk, dv = (torch.empty_like(q) if t is None else t for t in (dq, dk, dv))
+    B, H, N, d = q.shape
+    L = lib()
+    nbytes = L.flash_backward_workspace_bytes(B, H, N)
+    workspace = torch.empty(max(nbytes, 16), device=q.device, dtype=torch.uint8)
+    _on_device(torch, device, L.flash_backward, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), dout.data_ptr(),
+               lse.data_ptr(), None if dlse is None else dlse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), B, H,
+               N, d, softmax_scale, int(bool(causal)), window_left, window_right,
+               None if alibi_slopes is None else alibi_slopes.data_ptr(), workspace.data_ptr(), nbytes)
+    return dq, dk, dv
 
 
 def _check_cache(torch, k_pages, v_pages, page_table, lengths, counts, batch):

@@ -109,6 +109,27 @@ int flash_forward_dropout(const void* q, const void* k, const void* v, void* o, 
                           int head_dim, float softmax_scale, int is_causal, int window_left, int window_right,
                           const float* alibi_slopes, float dropout_prob, unsigned long long seed, void* stream);
 
+/* The forward's backward pass: dQ, dK and dV from Q, K, V, the forward's output O and log-sum-exp (flash_forward_lse) and
+ * the gradient dO. The probabilities are taken again from the scores: with s_ij the scaled, biased score,
+ *   P_ij = exp(s_ij - lse_i) where key j is visible to query i, else 0;  dS_ij = P_ij (dO_i.V_j - dO_i.O_i + dlse_i)
+ *   dQ_i = scale sum_j dS_ij K_j,  dK_j = scale sum_i dS_ij Q_i,  dV_j = sum_i P_ij dO_i
+ * No counterpart in the reference, whose kernel is a forward. All tensors fp16, contiguous [batch][heads][seqlen][head_dim],
+ * 16-byte aligned; the outputs must not overlap the inputs. Scale, causal flag, windows and alibi_slopes (NULL: no bias) are
+ * those of the forward call; dropout has no backward pass here.
+ *   lse, d_lse   float [batch][heads][seqlen]; d_lse is the gradient of the log-sum-exp, NULL for none (it is needed where
+ *                the outputs over disjoint key ranges were merged by it)
+ * P and dS are rounded to fp16 for the tensor cores, scaled by powers of two so that neither long rows nor small or large
+ * gradients cost precision; all sums are fp32. dK, dV and dQ are summed in one order: two calls with the same arguments give
+ * the same bits.
+ * workspace: flash_backward_workspace_bytes() bytes of device memory, 256-byte aligned, with any contents; calls that may
+ * overlap on the GPU need one each. Asynchronous on `stream`, two launches; may be captured into a CUDA graph once a call of
+ * this library has been made on the device. batch*heads up to 65535. flash_forward_check() reports a wait that ran out. */
+int flash_backward(const void* q, const void* k, const void* v, const void* o, const void* d_o, const float* lse,
+                   const float* d_lse, void* dq, void* dk, void* dv, int batch, int heads, int seqlen, int head_dim,
+                   float softmax_scale, int is_causal, int window_left, int window_right, const float* alibi_slopes,
+                   void* workspace, size_t workspace_bytes, void* stream);
+size_t flash_backward_workspace_bytes(int batch, int heads, int seqlen);
+
 /* Keep probability flash_forward_dropout() uses for `dropout_prob` (a multiple of 1/256; 1.0 when nothing is
  * dropped), or -1 when dropout_prob is outside [0, 1]. Needs no GPU. */
 double flash_forward_dropout_keep_probability(float dropout_prob);

@@ -68,6 +68,7 @@ class RowsStruct(ctypes.Structure):  # fa_rows
 _lock = threading.RLock()  # around the first load of either
 _lib = None
 _native = None  # forward() of _torch_binding once looked for; answers NotImplemented where there is none
+_native_operators = None  # its backward(), append() and decode(), likewise
 
 
 class FlashForwardError(RuntimeError):
@@ -149,7 +150,7 @@ def _load_native():
     """The native form of attention_forward (host/torch_binding.cpp), if it was built against the torch it is used with.
     Without it everything runs through ctypes, with the same results. With it the loaded library's flash_forward_noalloc is
     called without ctypes as well, where the arguments are plain numbers."""
-    global _native
+    global _native, _native_operators
     L = lib()
     with _lock:
         if _native is not None:
@@ -166,8 +167,12 @@ def _load_native():
         except ImportError:
             usable = False
         if not usable:
+            _native_operators = 3 * (lambda *args: NotImplemented,)
             _native = lambda *args: NotImplemented  # noqa: E731
             return _native
+        operators = (L.flash_backward, L.flash_backward_workspace_bytes, L.flash_cache_append, L.flash_decode,
+                     L.flash_decode_workspace_bytes)
+        _native_operators = _torch_binding.bind_operators(*(ctypes.cast(fn, ctypes.c_void_p).value for fn in operators))
         entry_points = (L.flash_forward, L.flash_forward_alibi, L.flash_forward_lse, L.flash_forward_dropout,
                         L.flash_forward_noalloc)
         _native, noalloc = _torch_binding.bind(*(ctypes.cast(fn, ctypes.c_void_p).value for fn in entry_points),
@@ -192,6 +197,16 @@ def _called_natively(L, fn, native):
     same.__name__, same.argtypes, same.restype = fn.__name__, fn.argtypes, fn.restype
     NativelyCalled.__call__ = native
     return same
+
+
+def _answered_natively(which, *args):
+    """The answer of backward() (0), append() (1) or decode() (2) of the binding, or NotImplemented."""
+    if _native_operators is None:
+        _load_native()
+    r = _native_operators[which](*args) if _native_operators is not None else NotImplemented
+    if type(r) is int:
+        _raise(r)
+    return r
 
 
 def _raise(code):
@@ -367,6 +382,10 @@ def attention_backward(q, k, v, out, lse, dout, causal=False, window_left=-1, wi
     All tensors as attention_forward takes and gives them; dout is made contiguous if it is not. dq, dk, dv, if given,
     are contiguous tensors like q that are written.
     """
+    r = _answered_natively(0, q, k, v, out, lse, dout, causal, window_left, window_right, softmax_scale, alibi_slopes, dlse,
+                           dq, dk, dv)
+    if r is not NotImplemented:
+        return r
     import torch
 
     dout = dout.contiguous()
@@ -451,6 +470,9 @@ def cache_append(k, v, k_pages, v_pages, page_table, lengths, counts=None, q=Non
     and the queries q [batch, q_heads, tokens, head_dim], are rotated. Returns the rotated queries (q_out, contiguous, if
     given), or None without q.
     """
+    r = _answered_natively(1, k, v, k_pages, v_pages, page_table, lengths, counts, q, rotary, interleaved, q_out)
+    if r is not NotImplemented:
+        return r
     import torch
 
     batch, kv_heads, tokens = k.shape[:3] if k.dim() == 4 else (0, 0, 0)
@@ -488,6 +510,10 @@ def attention_decode(q, k_pages, v_pages, page_table, lengths, counts=None, soft
     the cache as for cache_append, after it. Returns the output, contiguous and shaped like q (`out` if given), and with
     return_lse also float32 [batch, q_heads, tokens].
     """
+    r = _answered_natively(2, q, k_pages, v_pages, page_table, lengths, counts, softmax_scale, window_left, alibi_slopes,
+                           return_lse, out)
+    if r is not NotImplemented:
+        return r
     import torch
 
     batch, q_heads, tokens = q.shape[:3] if q.dim() == 4 else (0, 0, 0)

@@ -92,7 +92,8 @@ __global__ void __launch_bounds__(256) bwd_rows_kernel(const BwdParams p) {
 
 template <int D>
 struct BwdCfg {
-  static constexpr int kThreads = 384;
+  static constexpr int kSoftmaxWarps = 16;
+  static constexpr int kThreads = (kSoftmaxWarps + 4) * 32;
   static constexpr int kTileBytes = 128 * D * 2;
   static constexpr int kPanelBytes = 128 * 128;
   // Ring slots of the first and of the second column tensor. A first tile is held longest (for dQ from the scores of the
@@ -102,10 +103,16 @@ struct BwdCfg {
   static constexpr int kOffSecond = kOffFirst + kFirst * kTileBytes;
   static constexpr int kOffStats = kOffSecond + kSecond * kTileBytes;  // per slot float[2][128]
   static constexpr int kOffBars = kOffStats + kStats * 1024;
-  static constexpr int kNumBars = 1 + 2 * (kFirst + kSecond + kStats) + 6;
+  static constexpr int kNumBars = 2 * (kFirst + kSecond + kStats) + 9;
   static constexpr int kSmemBytes = kOffBars + kNumBars * 8 + 16;
   static constexpr uint32_t kTmemCols = 512;
-  static constexpr int kRegSoftmax = 208, kRegOthers = 88;  // 256 * 208 + 128 * 88 = 384 * 168
+  // Tensor memory: score regions of 128 columns, in which the fp16 operands of the second products take the place of the
+  // scores that they are made of (32 columns' operand in the first 16 of the 32), and the accumulators. S has two regions for
+  // dQ and at head_dim 64, where there is room: the scores of a tile are then computed while the tile before is worked on.
+  static constexpr uint32_t kColS = 0, kColDp = 128, kColOdd = 256, kColDv = D == 128 ? 256 : 384,
+                            kColDk = D == 128 ? 384 : 448, kColDq = 384;
+  // launched with 96 registers a thread: 512 * 104 + 128 * 64 <= 640 * 96
+  static constexpr int kRegSoftmax = 104, kRegOthers = 64;
 };
 
 // One work item: 128 rows of a head (queries for dQ, keys for dK and dV) against the columns (keys, queries) that they
@@ -155,147 +162,366 @@ __device__ __forceinline__ float bwd_unit(const BwdParams& p, int bh, int lane) 
   return __uint_as_float(static_cast<uint32_t>(min(max(127 - (exponent - 126), 27), 227)) << 23);
 }
 
-struct BwdBars {
-  uint64_t *own_full, *first_full, *second_full, *stats_full, *first_empty, *second_empty, *stats_empty, *s_full, *dp_full,
-      *p_ready, *ds_ready, *acc_full;
-  volatile int* abort_flag;
+// A role's place in a ring of slots, or on a barrier that is used again and again (one slot).
+template <int kSlots>
+struct Turn {
+  int slot = 0;
+  uint32_t parity = 0;
+  __device__ __forceinline__ void advance() {
+    if (++slot == kSlots) slot = 0, parity ^= 1;
+  }
 };
 
-// The eight softmax warps: a thread has one row and 64 columns of every tile (warps 0-3 the first 64, 4-7 the others).
-// kDq: row statistics are the thread's own, P is not needed further; else they come by column through shared memory.
+struct BwdBars {
+  uint64_t *first_full, *first_empty, *second_full, *second_empty, *stats_full, *own_full, *own_empty, *s_full, *dp_full,
+      *acc_full;  // s_full: two
+  uint64_t *stats_empty, *p_ready, *ds_ready, *acc_empty;
+  volatile int* abort_flag;
+  volatile float* unit;  // of the items of even and odd turn
+};
+
+// dK and dV at head_dim 128 have one region for S.
+template <int D>
+__device__ __forceinline__ constexpr bool bwd_two_s(bool is_dq) {
+  return D == 64 || is_dq;
+}
+
+// Of every kBwdPolyOf pairs of exponentials one is taken on the FMA pipe instead of the special-function unit.
+constexpr int kBwdPolyOf = 4;
+
+// State that a softmax warp carries from item to item.
+template <int D>
+struct SoftmaxTurns {
+  Turn<BwdCfg<D>::kStats> stats;
+  uint32_t s = 0, dp = 0, acc = 0;  // parities; s: bit 0, bit 1 of either s_full
+};
+
+// The sixteen softmax warps: a thread has one row and 32 columns of every tile (warps 0-3 the first 32, and so on).
+// kDq: the statistics (14 - log2(e) * lse and -delta / 2^e) are the row's, P is not needed further; else they are the
+// columns', and P goes to the tensor cores too. Returns false once a wait has run out.
 template <int D, bool kAlibi, bool kDq>
 __device__ __forceinline__ bool bwd_softmax(const BwdParams& p, const BwdItem& it, const BwdBars& b, const uint8_t* smem,
-                                            uint32_t tmem_base, int warp, int lane) {
+                                            uint32_t tmem_base, int warp, int lane, int turn, SoftmaxTurns<D>& at) {
   using Cfg = BwdCfg<D>;
-  constexpr uint32_t kColDp = kDq ? 256 : 128;
-  const int half = warp >> 2;
+  const int quarter = warp >> 2;
   const uint32_t lane_base = (warp & 3) * 32u;
   const int row = it.r0 + static_cast<int>(lane_base) + lane;
-  const float unit = bwd_unit(p, it.bh, lane);
-  const uint64_t scale2 = f2_pack(p.scale_log2, p.scale_log2), unit2 = f2_pack(unit, unit);
-  float nl = -INFINITY, nd = 0.f;  // 14 - log2(e) * lse and -delta / 2^e of the row
-  if (kDq && row < p.seqlen) {
-    const size_t at = static_cast<size_t>(it.bh) * p.seqlen + row;
-    nl = fmaf(p.lse[at], -1.4426950408889634f, 14.f);
-    nd = -p.delta[at] * unit;
-  }
+  const uint64_t scale2 = f2_pack(p.scale_log2, p.scale_log2);
   const float slope = kAlibi ? p.alibi_slopes[it.bh % p.heads] * 1.4426950408889634f : 0.f;
   const int r_last = min(it.r0 + 127, p.seqlen - 1);
-  bool ok = true;
+  const uint32_t tDp = tmem_addr(tmem_base, lane_base, Cfg::kColDp + quarter * 32);
+  bool ok = true;  // (looked at once a tile: a vote behind each wait costs more than the wait)
+  float unit = 1.f, nl = 0.f, nd = 0.f;
+  if (kDq) {
+    ok &= mbar_wait(b.stats_full + at.stats.slot, at.stats.parity, b.abort_flag);
+    const float* stats = reinterpret_cast<const float*>(smem + Cfg::kOffStats + at.stats.slot * 1024);
+    nl = stats[lane_base + lane];
+    nd = stats[128 + lane_base + lane];
+    unit = b.unit[turn & 1];
+    __syncwarp();
+    mbar_arrive_lane0(b.stats_empty + at.stats.slot, lane);
+    at.stats.advance();
+  }
   for (int i = 0; i < it.tiles; ++i) {
-    const int stage = i % Cfg::kStats;
-    const uint32_t tS = tmem_addr(tmem_base, lane_base, (kDq ? (i & 1) * 128 : 0) + half * 64);
-    const uint32_t tDp = tmem_addr(tmem_base, lane_base, kColDp + half * 64);
-    const int c_tile = (it.begin + i) * 128, c0 = c_tile + half * 64;
-    const bool cut = kv_tile_needs_mask(c_tile, it.r0, r_last, it.left, it.right, p.seqlen);
-    const int c_lo = it.left >= 0 ? row - it.left - c0 : -1;
-    const int c_hi = min(it.right >= 0 ? row + it.right : p.seqlen - 1, p.seqlen - 1) - c0;
-    const float4* col_nl = reinterpret_cast<const float4*>(smem + Cfg::kOffStats + stage * 1024 + half * 256);
+    const int odd = bwd_two_s<D>(kDq) ? i & 1 : 0;
+    const uint32_t tS = tmem_addr(tmem_base, lane_base, (odd ? Cfg::kColOdd : Cfg::kColS) + quarter * 32);
+    const int c_tile = (it.begin + i) * 128, c0 = c_tile + quarter * 32;
+    const float4* col_nl = reinterpret_cast<const float4*>(smem + Cfg::kOffStats + at.stats.slot * 1024 + quarter * 128);
     const float4* col_nd = col_nl + 32;
 
-    if (!kDq) ok = ok && mbar_wait_warp(b.stats_full + stage, (i / Cfg::kStats) & 1, b.abort_flag);
-    ok = ok && (kDq ? mbar_wait_warp(b.s_full + (i & 1), (i >> 1) & 1, b.abort_flag)
-                    : mbar_wait_warp(b.s_full, i & 1, b.abort_flag));
-    if (!ok) return false;
+    if (!kDq) {
+      ok &= mbar_wait(b.stats_full + at.stats.slot, at.stats.parity, b.abort_flag);
+      if (i == 0) unit = b.unit[turn & 1];
+    }
+    ok &= mbar_wait(b.s_full + odd, at.s >> odd & 1u, b.abort_flag);
+    at.s ^= 1u << odd;
     tc_fence_after();
-    float e[64];
-#pragma unroll
-    for (int ch = 0; ch < 2; ++ch) {
+    float e[32];
+    {
       uint32_t r[32];
-      tmem_ld32(tS + ch * 32, r);
+      tmem_ld32(tS, r);
       tmem_wait_ld();
       tmem_ld_fence(r);
 #pragma unroll
       for (int c = 0; c < 32; c += 4) {
-        float x[4];
-        const float4 n = kDq ? make_float4(nl, nl, nl, nl) : col_nl[(ch * 32 + c) / 4];
-        f2_unpack(f2_fma(f2_pack(__uint_as_float(r[c]), __uint_as_float(r[c + 1])), scale2, f2_pack(n.x, n.y)), x[0], x[1]);
-        f2_unpack(f2_fma(f2_pack(__uint_as_float(r[c + 2]), __uint_as_float(r[c + 3])), scale2, f2_pack(n.z, n.w)), x[2],
-                  x[3]);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int col = ch * 32 + c + k;
-          if (kAlibi) x[k] = fmaf(-slope, fabsf(static_cast<float>(row - c0 - col)), x[k]);
-          if (cut && (col < c_lo || col > c_hi)) x[k] = -INFINITY;
-          e[col] = ex2_approx(x[k]);
-        }
+        const float4 n = kDq ? make_float4(nl, nl, nl, nl) : col_nl[c / 4];
+        f2_unpack(f2_fma(f2_pack(__uint_as_float(r[c]), __uint_as_float(r[c + 1])), scale2, f2_pack(n.x, n.y)), e[c], e[c + 1]);
+        f2_unpack(f2_fma(f2_pack(__uint_as_float(r[c + 2]), __uint_as_float(r[c + 3])), scale2, f2_pack(n.z, n.w)), e[c + 2],
+                  e[c + 3]);
       }
-      if (!kDq) {
-        uint32_t pk[16];
+    }
+    if (kAlibi) {
 #pragma unroll
-        for (int c = 0; c < 16; ++c) pk[c] = pack_f16x2(e[ch * 32 + 2 * c], e[ch * 32 + 2 * c + 1]);
-        tmem_st16(tS + ch * 16, pk);
+      for (int c = 0; c < 32; ++c) e[c] = fmaf(-slope, fabsf(static_cast<float>(row - c0 - c)), e[c]);
+    }
+    if (kv_tile_needs_mask(c_tile, it.r0, r_last, it.left, it.right, p.seqlen)) {
+      const int c_lo = it.left >= 0 ? row - it.left - c0 : -1;
+      const int c_hi = min(it.right >= 0 ? row + it.right : p.seqlen - 1, p.seqlen - 1) - c0;
+#pragma unroll
+      for (int c = 0; c < 32; ++c)
+        if (c < c_lo || c > c_hi) e[c] = -INFINITY;
+    }
+#pragma unroll
+    for (int c = 0; c < 32; c += 2) {
+      if (kBwdPolyOf > 0 && c / 2 % (kBwdPolyOf > 0 ? kBwdPolyOf : 1) == 1) {
+        exp2_poly(e[c], e[c + 1], e[c], e[c + 1]);
+      } else {
+        e[c] = ex2_approx(e[c]);
+        e[c + 1] = ex2_approx(e[c + 1]);
       }
     }
     if (!kDq) {
+      uint32_t pk[16];
+#pragma unroll
+      for (int c = 0; c < 16; ++c) pk[c] = pack_f16x2(e[2 * c], e[2 * c + 1]);
+      tmem_st16(tS, pk);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
       mbar_arrive_lane0(b.p_ready, lane);
     }
-    ok = mbar_wait_warp(b.dp_full, i & 1, b.abort_flag);
-    if (!ok) return false;
+    ok &= mbar_wait(b.dp_full, at.dp, b.abort_flag);
+    at.dp ^= 1;
     tc_fence_after();
-#pragma unroll
-    for (int ch = 0; ch < 2; ++ch) {
+    {
       uint32_t r[32], pk[16];
-      tmem_ld32(tDp + ch * 32, r);
+      tmem_ld32(tDp, r);
       tmem_wait_ld();
       tmem_ld_fence(r);
+      const uint64_t unit2 = f2_pack(unit, unit);
 #pragma unroll
       for (int c = 0; c < 32; c += 4) {
-        const float4 n = kDq ? make_float4(nd, nd, nd, nd) : col_nd[(ch * 32 + c) / 4];
+        const float4 n = kDq ? make_float4(nd, nd, nd, nd) : col_nd[c / 4];
 #pragma unroll
         for (int k = 0; k < 4; k += 2) {
           float d0, d1;
           const uint64_t t = f2_fma(f2_pack(__uint_as_float(r[c + k]), __uint_as_float(r[c + k + 1])), unit2,
                                     k ? f2_pack(n.z, n.w) : f2_pack(n.x, n.y));
-          f2_unpack(f2_mul(t, f2_pack(e[ch * 32 + c + k], e[ch * 32 + c + k + 1])), d0, d1);
+          f2_unpack(f2_mul(t, f2_pack(e[c + k], e[c + k + 1])), d0, d1);
           pk[(c + k) / 2] = pack_f16x2(d0, d1);
         }
       }
-      tmem_st16((kDq ? tS : tDp) + ch * 16, pk);
+      tmem_st16(kDq ? tS : tDp, pk);
     }
     tmem_wait_st();
     tc_fence_before();
     __syncwarp();
     mbar_arrive_lane0(b.ds_ready, lane);
-    if (!kDq) mbar_arrive_lane0(b.stats_empty + stage, lane);
+    if (!kDq) {
+      mbar_arrive_lane0(b.stats_empty + at.stats.slot, lane);
+      at.stats.advance();
+    }
+    if (!__all_sync(0xffffffffu, ok)) return false;
   }
 
-  // ---- epilogue ----
-  if (!mbar_wait_warp(b.acc_full, 0, b.abort_flag)) return false;
+  // ---- epilogue: dQ a quarter of the columns a warp; dV the first eight warps, dK the others, half of the columns each ----
+  ok &= mbar_wait(b.acc_full, at.acc, b.abort_flag);
+  at.acc ^= 1;
   tc_fence_after();
-  const float ds_scale = p.scale * 0x1p-14f / unit;  // (a power of two but for p.scale)
-  const float factor = kDq || half ? ds_scale : 0x1p-14f;
-  const uint32_t acc = tmem_addr(tmem_base, lane_base, kDq ? 384 + half * (D / 2) : half ? 384 : 256);
-  __half* out = (kDq ? p.dq + half * (D / 2) : half ? p.dk : p.dv) + (static_cast<size_t>(it.bh) * p.seqlen + row) * D;
+  constexpr int kCols = kDq ? D / 4 : D / 2;
+  const int col = kDq ? quarter * kCols : (quarter & 1) * kCols;
+  const float factor = kDq || quarter >= 2 ? p.scale * 0x1p-14f / unit : 0x1p-14f;
+  const uint32_t acc =
+      tmem_addr(tmem_base, lane_base, (kDq ? Cfg::kColDq : quarter >= 2 ? Cfg::kColDk : Cfg::kColDv) + col);
+  __half* out = (kDq ? p.dq : quarter >= 2 ? p.dk : p.dv) + (static_cast<size_t>(it.bh) * p.seqlen + row) * D + col;
 #pragma unroll
-  for (int ch = 0; ch < (kDq ? D / 64 : D / 32); ++ch) {
-    uint32_t r[32];
-    tmem_ld32(acc + ch * 32, r);
+  for (int ch = 0; ch < kCols / 16; ++ch) {
+    uint32_t r[16];
+    tmem_ld16(acc + ch * 16, r);
     tmem_wait_ld();
-    tmem_ld_fence(r);
+    tmem_ld_fence16(r);
     if (row < p.seqlen) {
 #pragma unroll
-      for (int c = 0; c < 32; c += 8) {
+      for (int c = 0; c < 16; c += 8) {
         uint32_t w[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k)
           w[k] = pack_f16x2(__uint_as_float(r[c + 2 * k]) * factor, __uint_as_float(r[c + 2 * k + 1]) * factor);
-        *reinterpret_cast<uint4*>(out + ch * 32 + c) = make_uint4(w[0], w[1], w[2], w[3]);
+        *reinterpret_cast<uint4*>(out + ch * 16 + c) = make_uint4(w[0], w[1], w[2], w[3]);
       }
+    }
+  }
+  tc_fence_before();
+  __syncwarp();
+  mbar_arrive_lane0(b.acc_empty, lane);
+  return __all_sync(0xffffffffu, ok);
+}
+
+// The k-th work item of a CTA, or an index past the last: every other round of CTAs is dealt backwards, so that the CTAs'
+// sums are alike although the items of a group of heads get shorter under a causal mask.
+__device__ __forceinline__ int bwd_index(int k) {
+  return k * static_cast<int>(gridDim.x) + static_cast<int>(k & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+}
+
+// The warp that issues the products of all items.
+template <int D>
+__device__ __forceinline__ bool bwd_issue(const BwdParams& p, const BwdBars& b, uint8_t* smem, uint32_t tmem_base) {
+  using Cfg = BwdCfg<D>;
+  constexpr uint32_t idesc_s = umma_idesc_f16(128, 128, 0, 0), idesc_acc = umma_idesc_f16(128, D, 0, 1);
+  // descriptors of shared-memory operands: a constant high word (row stride, version, 128-byte swizzle), and low words that
+  // differ by the start address
+  constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+  constexpr uint32_t kKMajor = 1u << 16, kMnMajor = static_cast<uint32_t>(Cfg::kPanelBytes >> 4) << 16, kTile = Cfg::kTileBytes >> 4;
+  const uint32_t own = smem_u32(smem) >> 4, first = smem_u32(smem + Cfg::kOffFirst) >> 4,
+                 second = smem_u32(smem + Cfg::kOffSecond) >> 4;
+  // scores: 128 x 128, over head_dim
+  auto scores = [&](uint32_t col, uint32_t a, uint32_t tile) {
+#pragma unroll
+    for (int h = 0; h < D / 64; ++h)
+      umma_qk64(tmem_base + col, (a + h * (Cfg::kPanelBytes >> 4)) | kKMajor, (tile + h * (Cfg::kPanelBytes >> 4)) | kKMajor,
+                kDescHi, idesc_s, h);
+  };
+  // acc += X tile over 128 columns, fp16 X in the place of scores at column `x`
+  auto accumulate = [&](uint32_t col, uint32_t x, uint32_t tile, bool more) {
+    umma_x64(tmem_base + col, tmem_base + x, tile | kMnMajor, kDescHi, idesc_acc, more);
+    umma_x64(tmem_base + col, tmem_base + x + 64, (tile + 4 * (2048 >> 4)) | kMnMajor, kDescHi, idesc_acc, 1);
+  };
+  bool ok = true;
+  // (a wait that has run out is noticed at the end of the tile: a vote behind each costs more than the wait)
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    ok &= mbar_wait(bar, parity, b.abort_flag);
+    tc_fence_after();
+  };
+  Turn<Cfg::kFirst> f_scores, f_acc;  // first tiles: whose scores come next, whose product comes next
+  Turn<Cfg::kSecond> s_scores, s_acc;
+  uint32_t p_at = 0, ds_at = 0, own_at = 0, acc_at = 1;  // (the accumulators are free at the start)
+  for (int k = 0, index; (index = bwd_index(k)) < 2 * p.tiles * p.bh && ok; ++k) {
+    const BwdItem it = bwd_item(p, index);
+    const int n = it.tiles;
+    const bool two_s = bwd_two_s<D>(it.is_dq);
+    auto s_col = [&](int i) { return two_s && (i & 1) ? Cfg::kColOdd : Cfg::kColS; };
+    auto scores_first = [&](int i) {
+      wait(b.first_full + f_scores.slot, f_scores.parity);
+      scores(s_col(i), own, first + f_scores.slot * kTile);
+      umma_commit_warp(b.s_full + (two_s ? i & 1 : 0));
+      f_scores.advance();
+    };
+    auto scores_second = [&](int i) {
+      wait(b.second_full + s_scores.slot, s_scores.parity);
+      scores(Cfg::kColDp, own + kTile, second + s_scores.slot * kTile);
+      umma_commit_warp(b.dp_full);
+      umma_commit_warp(b.second_empty + s_scores.slot, it.is_dq);
+      umma_commit_warp(b.own_empty, i + 1 == n);
+      s_scores.advance();
+    };
+    auto product_first = [&](int i) {
+      accumulate(it.is_dq ? Cfg::kColDq : Cfg::kColDk, it.is_dq ? s_col(i) : Cfg::kColDp, first + f_acc.slot * kTile, i > 0);
+      umma_commit_warp(b.first_empty + f_acc.slot);
+      f_acc.advance();
+    };
+    // S and dP of the item before have been used: its products stand in front of what follows here
+    wait(b.own_full, own_at);
+    own_at ^= 1;
+    scores_first(0);
+    scores_second(0);
+    wait(b.acc_empty, acc_at);  // (before the odd S, which may lie where an accumulator of the item before is)
+    acc_at ^= 1;
+    if (two_s && n > 1) scores_first(1);
+    if (it.is_dq) {
+      for (int i = 0; i < n && ok; ++i) {
+        wait(b.ds_ready, ds_at);
+        ds_at ^= 1;
+        if (i + 1 < n) scores_second(i + 1);  // the softmax of the next tile waits for this one first
+        product_first(i);
+        if (i + 2 < n) scores_first(i + 2);
+        s_acc.advance();
+        ok = __all_sync(0xffffffffu, ok);
+      }
+    } else {
+      for (int i = 0; i < n && ok; ++i) {
+        wait(b.p_ready, p_at);
+        p_at ^= 1;
+        accumulate(Cfg::kColDv, s_col(i), second + s_acc.slot * kTile, i > 0);
+        umma_commit_warp(b.second_empty + s_acc.slot);
+        s_acc.advance();
+        if (i + 1 + two_s < n) scores_first(i + 1 + two_s);
+        wait(b.ds_ready, ds_at);
+        ds_at ^= 1;
+        product_first(i);
+        if (i + 1 < n) scores_second(i + 1);
+        ok = __all_sync(0xffffffffu, ok);
+      }
+    }
+    umma_commit_warp(b.acc_full);
+  }
+  return ok;
+}
+
+// The thread that loads the tiles of all items.
+template <int D>
+__device__ __forceinline__ bool bwd_load(const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensorMap& map_v,
+                                         const CUtensorMap& map_do, const BwdParams& p, const BwdBars& b, uint8_t* smem) {
+  using Cfg = BwdCfg<D>;
+  Turn<Cfg::kFirst> f;
+  Turn<Cfg::kSecond> s;
+  Turn<1> own;
+  own.parity = f.parity = s.parity = 1;  // (everything is free at the start)
+  for (int k = 0, index; (index = bwd_index(k)) < 2 * p.tiles * p.bh; ++k) {
+    const BwdItem it = bwd_item(p, index);
+    const CUtensorMap *own0 = it.is_dq ? &map_q : &map_k, *own1 = it.is_dq ? &map_do : &map_v;
+    const CUtensorMap *first = it.is_dq ? &map_k : &map_q, *second = it.is_dq ? &map_v : &map_do;
+    for (int i = 0; i < it.tiles; ++i) {
+      const int c0 = (it.begin + i) * 128;
+      if (!mbar_wait(b.first_empty + f.slot, f.parity, b.abort_flag)) return false;
+      mbar_arrive_expect_tx(b.first_full + f.slot, Cfg::kTileBytes);
+      tma_load_4d(smem + Cfg::kOffFirst + f.slot * Cfg::kTileBytes, first, b.first_full + f.slot, 0, c0, 0, it.bh);
+      f.advance();
+      if (i == 0) {
+        if (!mbar_wait(b.own_empty, own.parity, b.abort_flag)) return false;
+        own.advance();
+        mbar_arrive_expect_tx(b.own_full, 2 * Cfg::kTileBytes);
+        tma_load_4d(smem, own0, b.own_full, 0, it.r0, 0, it.bh);
+        tma_load_4d(smem + Cfg::kTileBytes, own1, b.own_full, 0, it.r0, 0, it.bh);
+      }
+      if (!mbar_wait(b.second_empty + s.slot, s.parity, b.abort_flag)) return false;
+      mbar_arrive_expect_tx(b.second_full + s.slot, Cfg::kTileBytes);
+#ifdef FA_TEST_WITHHOLD_LOAD
+      if (!(p.withhold && index == 0 && i == it.tiles - 1))
+#endif
+        tma_load_4d(smem + Cfg::kOffSecond + s.slot * Cfg::kTileBytes, second, b.second_full + s.slot, 0, c0, 0, it.bh);
+      s.advance();
     }
   }
   return true;
 }
 
-// 12 warps: 0-7 softmax, 8 issues the products, 9 loads tiles, 10 loads the column statistics, 11 only donates registers.
-// Tensor memory: for dK and dV S (P in its place) at column 0, dP (dS in its place) at 128, dV at 256, dK at 384; for dQ two
-// S (dS in its place) at 0 and 128, dP at 256, dQ at 384. fp16 P and dS of columns 0-63 of a tile lie in the first 32 columns
-// of their region, of columns 64-127 in columns 64-95, so that neither half of the warps writes where the other still reads.
+// The warp that brings the statistics: for dK and dV those of every column tile, for dQ those of the item's own rows.
+template <int D>
+__device__ __forceinline__ void bwd_stats(const BwdParams& p, const BwdBars& b, uint8_t* smem, int lane) {
+  using Cfg = BwdCfg<D>;
+  Turn<Cfg::kStats> at;
+  at.parity = 1;
+  for (int k = 0, index; (index = bwd_index(k)) < 2 * p.tiles * p.bh; ++k) {
+    const BwdItem it = bwd_item(p, index);
+    const float unit = bwd_unit(p, it.bh, lane);
+    for (int i = 0; i < (it.is_dq ? 1 : it.tiles); ++i) {
+      float nl[4], nd[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int c = (it.is_dq ? it.r0 : (it.begin + i) * 128) + j * 32 + lane;
+        const size_t from = static_cast<size_t>(it.bh) * p.seqlen + c;
+        nl[j] = c < p.seqlen ? fmaf(p.lse[from], -1.4426950408889634f, 14.f) : -INFINITY;
+        nd[j] = c < p.seqlen ? -p.delta[from] * unit : 0.f;
+      }
+      if (!mbar_wait_warp(b.stats_empty + at.slot, at.parity, b.abort_flag)) return;
+      float* to = reinterpret_cast<float*>(smem + Cfg::kOffStats + at.slot * 1024);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        to[j * 32 + lane] = nl[j];
+        to[128 + j * 32 + lane] = nd[j];
+      }
+      if (i == 0 && lane == 0) b.unit[k & 1] = unit;
+      __syncwarp();
+      mbar_arrive_lane0(b.stats_full + at.slot, lane);
+      at.advance();
+    }
+  }
+}
+
+// One CTA a SM walks the work items bwd_index(0), bwd_index(1), ... 20 warps: 0-15 softmax and epilogue, 16 issues
+// the products, 17 loads tiles, 18 brings the statistics, 19 only donates registers.
 template <int D, bool kAlibi>
-__global__ void __launch_bounds__(384, 1)
+__global__ void __launch_bounds__(640, 1)
 bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
            const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do,
            const __grid_constant__ BwdParams p) {
@@ -303,44 +529,37 @@ bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cfg::kOffBars);
   BwdBars b;
-  b.own_full = bars;
-  b.first_full = bars + 1;
+  b.first_full = bars;
   b.first_empty = b.first_full + Cfg::kFirst;
   b.second_full = b.first_empty + Cfg::kFirst;
   b.second_empty = b.second_full + Cfg::kSecond;
   b.stats_full = b.second_empty + Cfg::kSecond;
-  b.stats_empty = b.stats_full + Cfg::kStats;
-  b.s_full = b.stats_empty + Cfg::kStats;  // two
-  b.dp_full = b.s_full + 2;
-  b.p_ready = b.s_full + 3;
-  b.ds_ready = b.s_full + 4;
-  b.acc_full = b.s_full + 5;
+  b.own_full = b.stats_full + Cfg::kStats;
+  b.own_empty = b.own_full + 1;
+  b.acc_full = b.own_full + 2;
+  b.dp_full = b.own_full + 3;
+  b.s_full = b.own_full + 4;
+  b.stats_empty = b.own_full + 6;  // from here on it is the softmax warps that arrive
+  b.p_ready = b.stats_empty + Cfg::kStats;
+  b.ds_ready = b.p_ready + 1;
+  b.acc_empty = b.p_ready + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + Cfg::kNumBars);
   b.abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  b.unit = reinterpret_cast<volatile float*>(tmem_slot + 2);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  if (warp == 8) {
+  if (warp == 16) {
     tmem_alloc(tmem_slot, Cfg::kTmemCols);
     tmem_relinquish();
   }
   if (threadIdx.x == 0) {
-    mbar_init(b.own_full, 1);
-    for (int i = 0; i < 2 * Cfg::kFirst; ++i) mbar_init(b.first_full + i, 1);    // and first_empty
-    for (int i = 0; i < 2 * Cfg::kSecond; ++i) mbar_init(b.second_full + i, 1);  // and second_empty
-    for (int i = 0; i < Cfg::kStats; ++i) {
-      mbar_init(b.stats_full + i, 1);
-      mbar_init(b.stats_empty + i, 8);
+    for (int i = 0; i < Cfg::kNumBars; ++i) {
+      uint64_t* bar = bars + i;
+      mbar_init(bar, bar >= b.stats_empty ? Cfg::kSoftmaxWarps : 1);
     }
-    mbar_init(b.s_full, 1);
-    mbar_init(b.s_full + 1, 1);
-    mbar_init(b.dp_full, 1);
-    mbar_init(b.p_ready, 8);
-    mbar_init(b.ds_ready, 8);
-    mbar_init(b.acc_full, 1);
     *b.abort_flag = 0;
     fence_mbar_init();
   }
-  const BwdItem it = bwd_item(p, blockIdx.x);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -348,154 +567,33 @@ bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
   griddep_wait();
   griddep_launch();
 
-  if (warp < 8) {
+  if (warp < Cfg::kSoftmaxWarps) {
     reg_inc<Cfg::kRegSoftmax>();
-    if (it.is_dq) bwd_softmax<D, kAlibi, true>(p, it, b, smem, tmem_base, warp, lane);
-    else bwd_softmax<D, kAlibi, false>(p, it, b, smem, tmem_base, warp, lane);
+    SoftmaxTurns<D> at;
+    bool ok = true;
+    for (int k = 0, index; (index = bwd_index(k)) < 2 * p.tiles * p.bh && ok; ++k) {
+      const BwdItem it = bwd_item(p, index);
+      ok = it.is_dq ? bwd_softmax<D, kAlibi, true>(p, it, b, smem, tmem_base, warp, lane, k, at)
+                    : bwd_softmax<D, kAlibi, false>(p, it, b, smem, tmem_base, warp, lane, k, at);
+    }
   } else {
     reg_dec<Cfg::kRegOthers>();
-    bool ok = true;
-    if (warp == 8) {
-      // ---- products ----
-      constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);  // row stride, version, 128-byte swizzle
-      constexpr uint32_t kKMajor = 1u << 16, kMnMajor = (Cfg::kPanelBytes >> 4) << 16;  // leading-dimension offsets
-      constexpr uint32_t idesc_s = umma_idesc_f16(128, 128, 0, 0), idesc_acc = umma_idesc_f16(128, D, 0, 1);
-      constexpr uint32_t kTile = Cfg::kTileBytes >> 4, kPanel16 = Cfg::kPanelBytes >> 4;
-      auto low = [&](int offset) { return (smem_u32(smem + offset) >> 4) & 0x3fffu; };
-      const uint32_t own = low(0), first = low(Cfg::kOffFirst), second = low(Cfg::kOffSecond);
-      auto first_tile = [&](int i) { return first + i % Cfg::kFirst * kTile; };
-      auto second_tile = [&](int i) { return second + i % Cfg::kSecond * kTile; };
-      auto scores = [&](uint32_t col, uint32_t a, uint32_t tile) {
-#pragma unroll
-        for (int h = 0; h < D / 64; ++h)
-          umma_qk64(tmem_base + col, (a + h * kPanel16) | kKMajor, (tile + h * kPanel16) | kKMajor, kDescHi, idesc_s, h);
-      };
-      // acc += X tile, fp16 X at column `x` as described above
-      auto accumulate = [&](uint32_t col, uint32_t x, uint32_t tile, bool more) {
-        umma_pv64(tmem_base + col, tmem_base + x, tile | kMnMajor, kDescHi, idesc_acc, more);
-        umma_pv64(tmem_base + col, tmem_base + x + 64, (tile + 4 * (2048 >> 4)) | kMnMajor, kDescHi, idesc_acc, 1);
-      };
-      auto wait = [&](uint64_t* bar, uint32_t parity) {
-        ok = ok && mbar_wait_warp(bar, parity, b.abort_flag);
-        tc_fence_after();
-        return ok;
-      };
-      auto wait_first = [&](int i) { return wait(b.first_full + i % Cfg::kFirst, (i / Cfg::kFirst) & 1); };
-      auto wait_second = [&](int i) { return wait(b.second_full + i % Cfg::kSecond, (i / Cfg::kSecond) & 1); };
-      const int n = it.tiles;
-      wait(b.own_full, 0);
-      if (wait_first(0)) {
-        scores(0, own, first_tile(0));
-        umma_commit_warp(b.s_full);
-      }
-      if (it.is_dq) {
-        if (n > 1 && wait_first(1)) {
-          scores(128, own, first_tile(1));
-          umma_commit_warp(b.s_full + 1);
-        }
-        if (wait_second(0)) {
-          scores(256, own + kTile, second_tile(0));
-          umma_commit_warp(b.dp_full);
-          umma_commit_warp(b.second_empty);
-        }
-        for (int i = 0; i < n; ++i) {
-          if (!wait(b.ds_ready, i & 1)) break;
-          if (i + 1 < n) {  // the softmax of the next tile waits for this one first
-            if (!wait_second(i + 1)) break;
-            scores(256, own + kTile, second_tile(i + 1));
-            umma_commit_warp(b.dp_full);
-            umma_commit_warp(b.second_empty + (i + 1) % Cfg::kSecond);
-          }
-          accumulate(384, (i & 1) * 128, first_tile(i), i > 0);
-          umma_commit_warp(b.first_empty + i % Cfg::kFirst);
-          if (i + 2 < n) {
-            if (!wait_first(i + 2)) break;
-            scores((i & 1) * 128, own, first_tile(i + 2));
-            umma_commit_warp(b.s_full + (i & 1));
-          }
-        }
-      } else {
-        if (wait_second(0)) {
-          scores(128, own + kTile, second_tile(0));
-          umma_commit_warp(b.dp_full);
-        }
-        for (int i = 0; i < n; ++i) {
-          if (!wait(b.p_ready, i & 1)) break;
-          accumulate(256, 0, second_tile(i), i > 0);
-          umma_commit_warp(b.second_empty + i % Cfg::kSecond);
-          if (i + 1 < n) {
-            if (!wait_first(i + 1)) break;
-            scores(0, own, first_tile(i + 1));
-            umma_commit_warp(b.s_full);
-          }
-          if (!wait(b.ds_ready, i & 1)) break;
-          accumulate(384, 128, first_tile(i), i > 0);
-          umma_commit_warp(b.first_empty + i % Cfg::kFirst);
-          if (i + 1 < n) {
-            if (!wait_second(i + 1)) break;
-            scores(128, own + kTile, second_tile(i + 1));
-            umma_commit_warp(b.dp_full);
-          }
-        }
-      }
-      if (ok) umma_commit_warp(b.acc_full);
-    } else if (warp == 9) {
-      // ---- tiles ----
-      if (elect_one()) {
-        const CUtensorMap *own0 = it.is_dq ? &map_q : &map_k, *own1 = it.is_dq ? &map_do : &map_v;
-        const CUtensorMap *first = it.is_dq ? &map_k : &map_q, *second = it.is_dq ? &map_v : &map_do;
-        mbar_arrive_expect_tx(b.own_full, 2 * Cfg::kTileBytes);
-        tma_load_4d(smem, own0, b.own_full, 0, it.r0, 0, it.bh);
-        tma_load_4d(smem + Cfg::kTileBytes, own1, b.own_full, 0, it.r0, 0, it.bh);
-        for (int i = 0; i < it.tiles; ++i) {
-          const int c0 = (it.begin + i) * 128, f = i % Cfg::kFirst, s = i % Cfg::kSecond;
-          ok = mbar_wait(b.first_empty + f, ((i / Cfg::kFirst) & 1) ^ 1, b.abort_flag);
-          if (!ok) break;
-          mbar_arrive_expect_tx(b.first_full + f, Cfg::kTileBytes);
-          tma_load_4d(smem + Cfg::kOffFirst + f * Cfg::kTileBytes, first, b.first_full + f, 0, c0, 0, it.bh);
-          ok = mbar_wait(b.second_empty + s, ((i / Cfg::kSecond) & 1) ^ 1, b.abort_flag);
-          if (!ok) break;
-          mbar_arrive_expect_tx(b.second_full + s, Cfg::kTileBytes);
-#ifdef FA_TEST_WITHHOLD_LOAD
-          if (p.withhold && blockIdx.x == 0 && i == it.tiles - 1) continue;
-#endif
-          tma_load_4d(smem + Cfg::kOffSecond + s * Cfg::kTileBytes, second, b.second_full + s, 0, c0, 0, it.bh);
-        }
-        // a give-up leaves loads in flight; let them land before the CTA retires
-        if (!ok)
-          for (int i = 0; i < 64; ++i) __nanosleep(2000);
-      }
+    if (warp == 16) {
+      bwd_issue<D>(p, b, smem, tmem_base);
+    } else if (warp == 17) {
+      // (a give-up leaves loads in flight: they land before the CTA retires)
+      if (elect_one() && !bwd_load<D>(map_q, map_k, map_v, map_do, p, b, smem))
+        for (int i = 0; i < 64; ++i) __nanosleep(2000);
       __syncwarp();
-    } else if (warp == 10 && !it.is_dq) {
-      // ---- column statistics ----
-      const float unit = bwd_unit(p, it.bh, lane);
-      for (int i = 0; i < it.tiles; ++i) {
-        const int stage = i % Cfg::kStats;
-        float nl[4], nd[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int c = (it.begin + i) * 128 + k * 32 + lane;
-          const size_t at = static_cast<size_t>(it.bh) * p.seqlen + c;
-          nl[k] = c < p.seqlen ? fmaf(p.lse[at], -1.4426950408889634f, 14.f) : -INFINITY;
-          nd[k] = c < p.seqlen ? -p.delta[at] * unit : 0.f;
-        }
-        if (!mbar_wait_warp(b.stats_empty + stage, ((i / Cfg::kStats) & 1) ^ 1, b.abort_flag)) break;
-        float* to = reinterpret_cast<float*>(smem + Cfg::kOffStats + stage * 1024);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          to[k * 32 + lane] = nl[k];
-          to[128 + k * 32 + lane] = nd[k];
-        }
-        __syncwarp();
-        mbar_arrive_lane0(b.stats_full + stage, lane);
-      }
+    } else if (warp == 18) {
+      bwd_stats<D>(p, b, smem, lane);
     }
   }
 
   tc_fence_before();
   __syncthreads();
   if (threadIdx.x == 0 && *b.abort_flag != 0) atomicExch(p.status, 1);
-  if (warp == 8) tmem_dealloc(tmem_base, Cfg::kTmemCols);
+  if (warp == 16) tmem_dealloc(tmem_base, Cfg::kTmemCols);
 }
 
 }  // namespace fa

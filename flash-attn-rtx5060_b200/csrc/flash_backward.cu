@@ -12,14 +12,15 @@ namespace {
 size_t align256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
 
 template <int D, bool kAlibi>
-int launch(const CUtensorMap (&maps)[4], const fa::BwdParams& p, cudaStream_t st, bool early) {
+int launch(const CUtensorMap (&maps)[4], const fa::BwdParams& p, int num_sms, cudaStream_t st, bool early) {
   using Cfg = fa::BwdCfg<D>;
   cudaError_t e = launch_early(fa::bwd_rows_kernel<D>, dim3(p.tiles, p.bh), 256, 0, st, early, p);
   if (e != cudaSuccess) return fail_cuda("launch bwd_rows_kernel", e);
   constexpr auto kernel = fa::bwd_kernel<D, kAlibi>;
   e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes);
   if (e != cudaSuccess) return fail_cuda("cudaFuncSetAttribute(MaxDynamicSharedMemorySize)", e);
-  e = launch_early(kernel, dim3(2 * p.tiles * p.bh), Cfg::kThreads, Cfg::kSmemBytes, st, early, maps[0], maps[1], maps[2],
+  const int items = 2 * p.tiles * p.bh;
+  e = launch_early(kernel, dim3(items < num_sms ? items : num_sms), Cfg::kThreads, Cfg::kSmemBytes, st, early, maps[0], maps[1], maps[2],
                    maps[3], p);
   if (e != cudaSuccess) return fail_cuda("launch bwd_kernel", e);
   return FA_OK;
@@ -89,8 +90,8 @@ int backward(const void* q, const void* k, const void* v, const void* o, const v
   for (int i = 0; i < 4; ++i)
     if ((rc = make_map(&maps[i], tensors[i], p.bh, seqlen, head_dim, 128)) != FA_OK) return rc;
   if (head_dim == 64)
-    return alibi_slopes ? launch<64, true>(maps, p, st, !captured) : launch<64, false>(maps, p, st, !captured);
-  return alibi_slopes ? launch<128, true>(maps, p, st, !captured) : launch<128, false>(maps, p, st, !captured);
+    return alibi_slopes ? launch<64, true>(maps, p, s->num_sms, st, !captured) : launch<64, false>(maps, p, s->num_sms, st, !captured);
+  return alibi_slopes ? launch<128, true>(maps, p, s->num_sms, st, !captured) : launch<128, false>(maps, p, s->num_sms, st, !captured);
 }
 
 }  // namespace

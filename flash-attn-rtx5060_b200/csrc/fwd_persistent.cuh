@@ -98,28 +98,6 @@ struct PersistentCfg {
   static constexpr int kRegSoftmaxShort = 184, kRegEpilogueShort = 72;
 };
 
-// 2^x of two values on the FMA pipe: x = n + f with n the nearest integer (the usual addition of 1.5 * 2^23 rounds x to
-// one), 2^f a polynomial, 2^n by way of the exponent field. The polynomial is the minimax approximation of 2^f in
-// relative error on [-1/2, 1/2] among those of degree 5 with constant term 1 (Remez exchange): 1.6e-7 in fp32
-// arithmetic, where ex2.approx states 2.4e-7. 2^0 is exactly 1; below 2^-126.5, down to -infinity, the result is 0; NaN
-// stays NaN (a product, not an addition to the exponent field, and a maximum that keeps it).
-__device__ __forceinline__ void exp2_poly(float x0, float x1, float& e0, float& e1) {
-  const uint64_t x = f2_pack(max_nan(x0, -127.f), max_nan(x1, -127.f));
-  const uint64_t magic = f2_pack(12582912.f, 12582912.f);
-  const uint64_t t = f2_add(x, magic);
-  const uint64_t f = f2_add(x, f2_fma(t, f2_pack(-1.f, -1.f), magic));
-  uint64_t p = f2_fma(f2_pack(0x1.5bba14p-10f, 0x1.5bba14p-10f), f, f2_pack(0x1.3cea88p-7f, 0x1.3cea88p-7f));
-  p = f2_fma(p, f, f2_pack(0x1.c6b752p-5f, 0x1.c6b752p-5f));
-  p = f2_fma(p, f, f2_pack(0x1.ebf9bcp-3f, 0x1.ebf9bcp-3f));
-  p = f2_fma(p, f, f2_pack(0x1.62e42ap-1f, 0x1.62e42ap-1f));
-  p = f2_fma(p, f, f2_pack(1.f, 1.f));
-  float t0, t1;
-  f2_unpack(t, t0, t1);
-  const float s0 = __uint_as_float((__float_as_uint(t0) << 23) + 0x3f800000u);
-  const float s1 = __uint_as_float((__float_as_uint(t1) << 23) + 0x3f800000u);
-  f2_unpack(f2_mul(p, f2_pack(s0, s1)), e0, e1);
-}
-
 // exp2 of 2 * kPairs scores -> packed fp16x2 words; adds the exponentials into two (even, odd) pairs of partial row sums.
 // Of every kPolyOf pairs one takes exp2_poly instead of the special-function unit (0: none).
 template <int kPairs, int kPolyOf>

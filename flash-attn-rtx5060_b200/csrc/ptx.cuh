@@ -95,6 +95,28 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   return r;
 }
 
+// 2^x of two values on the FMA pipe: x = n + f with n the nearest integer (the usual addition of 1.5 * 2^23 rounds x to
+// one), 2^f a polynomial, 2^n by way of the exponent field. The polynomial is the minimax approximation of 2^f in
+// relative error on [-1/2, 1/2] among those of degree 5 with constant term 1 (Remez exchange): 1.6e-7 in fp32
+// arithmetic, where ex2.approx states 2.4e-7. 2^0 is exactly 1; below 2^-126.5, down to -infinity, the result is 0; NaN
+// stays NaN (a product, not an addition to the exponent field, and a maximum that keeps it).
+__device__ __forceinline__ void exp2_poly(float x0, float x1, float& e0, float& e1) {
+  const uint64_t x = f2_pack(max_nan(x0, -127.f), max_nan(x1, -127.f));
+  const uint64_t magic = f2_pack(12582912.f, 12582912.f);
+  const uint64_t t = f2_add(x, magic);
+  const uint64_t f = f2_add(x, f2_fma(t, f2_pack(-1.f, -1.f), magic));
+  uint64_t p = f2_fma(f2_pack(0x1.5bba14p-10f, 0x1.5bba14p-10f), f, f2_pack(0x1.3cea88p-7f, 0x1.3cea88p-7f));
+  p = f2_fma(p, f, f2_pack(0x1.c6b752p-5f, 0x1.c6b752p-5f));
+  p = f2_fma(p, f, f2_pack(0x1.ebf9bcp-3f, 0x1.ebf9bcp-3f));
+  p = f2_fma(p, f, f2_pack(0x1.62e42ap-1f, 0x1.62e42ap-1f));
+  p = f2_fma(p, f, f2_pack(1.f, 1.f));
+  float t0, t1;
+  f2_unpack(t, t0, t1);
+  const float s0 = __uint_as_float((__float_as_uint(t0) << 23) + 0x3f800000u);
+  const float s1 = __uint_as_float((__float_as_uint(t1) << 23) + 0x3f800000u);
+  f2_unpack(f2_mul(p, f2_pack(s0, s1)), e0, e1);
+}
+
 // Programmatic dependent launch: a grid launched with that attribute may start before the grid in front of it in the
 // stream has ended. griddep_wait() holds a thread until that grid has completed and its memory is visible;
 // griddep_launch() (once per CTA) lets the grid behind this one start where SMs are free. Both do nothing in a grid
@@ -331,6 +353,31 @@ __device__ __forceinline__ void umma_pv64(uint32_t d_tmem, uint32_t p_tmem, uint
       "}\n"
       :
       : "r"(d_tmem), "r"(p_tmem), "r"(v_lo), "r"(hi), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// D (+)= X B for 64 columns of X, which lie as two groups of 32 in the first 16 tensor-memory columns of every 32 (in the place
+// of the fp32 scores that they were made of); B as V above.
+__device__ __forceinline__ void umma_x64(uint32_t d_tmem, uint32_t x_tmem, uint32_t b_lo, uint32_t hi, uint32_t idesc,
+                                         uint32_t accumulate) {
+  asm volatile(
+      "{\n"
+      ".reg .pred lead, acc, yes;\n"
+      ".reg .b64 v;\n"
+      ".reg .b32 lo, p;\n"
+      "elect.sync _|lead, 0xffffffff;\n"
+      "setp.ne.b32 acc, %5, 0;\n"
+      "setp.eq.b32 yes, 0, 0;\n"
+      "mov.b64 v, {%2, %3};\n"
+      "@lead tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], v, %4, acc;\n"
+      "add.u32 lo, %2, 128;\n add.u32 p, %1, 8;\n mov.b64 v, {lo, %3};\n"
+      "@lead tcgen05.mma.cta_group::1.kind::f16 [%0], [p], v, %4, yes;\n"
+      "add.u32 lo, %2, 256;\n add.u32 p, %1, 32;\n mov.b64 v, {lo, %3};\n"
+      "@lead tcgen05.mma.cta_group::1.kind::f16 [%0], [p], v, %4, yes;\n"
+      "add.u32 lo, %2, 384;\n add.u32 p, %1, 40;\n mov.b64 v, {lo, %3};\n"
+      "@lead tcgen05.mma.cta_group::1.kind::f16 [%0], [p], v, %4, yes;\n"
+      "}\n"
+      :
+      : "r"(d_tmem), "r"(x_tmem), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate)
       : "memory");
 }
 // D += P V for 32 keys.

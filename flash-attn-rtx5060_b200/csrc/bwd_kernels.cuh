@@ -103,7 +103,7 @@ struct BwdCfg {
   static constexpr int kOffSecond = kOffFirst + kFirst * kTileBytes;
   static constexpr int kOffStats = kOffSecond + kSecond * kTileBytes;  // per slot float[2][128]
   static constexpr int kOffBars = kOffStats + kStats * 1024;
-  static constexpr int kNumBars = 2 * (kFirst + kSecond + kStats) + 9;
+  static constexpr int kNumBars = 2 * (kFirst + kSecond + kStats) + 10;
   static constexpr int kSmemBytes = kOffBars + kNumBars * 8 + 16;
   static constexpr uint32_t kTmemCols = 512;
   // Tensor memory: score regions of 128 columns, in which the fp16 operands of the second products take the place of the
@@ -175,6 +175,8 @@ struct Turn {
 struct BwdBars {
   uint64_t *first_full, *first_empty, *second_full, *second_empty, *stats_full, *own_full, *own_empty, *s_full, *dp_full,
       *acc_full;  // s_full: two
+  // p_ready: two, for even and odd tiles where S has two regions: a warp may then have handed over P of a tile before another
+  // has that of the tile before
   uint64_t *stats_empty, *p_ready, *ds_ready, *acc_empty;
   volatile int* abort_flag;
   volatile float* unit;  // of the items of even and odd turn
@@ -209,6 +211,8 @@ __device__ __forceinline__ bool bwd_softmax(const BwdParams& p, const BwdItem& i
   const uint64_t scale2 = f2_pack(p.scale_log2, p.scale_log2);
   const float slope = kAlibi ? p.alibi_slopes[it.bh % p.heads] * 1.4426950408889634f : 0.f;
   const int r_last = min(it.r0 + 127, p.seqlen - 1);
+  constexpr bool kTwoS = bwd_two_s<D>(kDq);
+  const uint32_t tS = tmem_addr(tmem_base, lane_base, Cfg::kColS + quarter * 32);
   const uint32_t tDp = tmem_addr(tmem_base, lane_base, Cfg::kColDp + quarter * 32);
   bool ok = true;  // (looked at once a tile: a vote behind each wait costs more than the wait)
   float unit = 1.f, nl = 0.f, nd = 0.f;
@@ -223,38 +227,37 @@ __device__ __forceinline__ bool bwd_softmax(const BwdParams& p, const BwdItem& i
     at.stats.advance();
   }
   for (int i = 0; i < it.tiles; ++i) {
-    const int odd = bwd_two_s<D>(kDq) ? i & 1 : 0;
-    const uint32_t tS = tmem_addr(tmem_base, lane_base, (odd ? Cfg::kColOdd : Cfg::kColS) + quarter * 32);
+    const uint32_t tS_i = tS + (kTwoS && (i & 1) ? Cfg::kColOdd - Cfg::kColS : 0u);
     const int c_tile = (it.begin + i) * 128, c0 = c_tile + quarter * 32;
     const float4* col_nl = reinterpret_cast<const float4*>(smem + Cfg::kOffStats + at.stats.slot * 1024 + quarter * 128);
     const float4* col_nd = col_nl + 32;
+    const bool cut = kv_tile_needs_mask(c_tile, it.r0, r_last, it.left, it.right, p.seqlen);
 
     if (!kDq) {
       ok &= mbar_wait(b.stats_full + at.stats.slot, at.stats.parity, b.abort_flag);
       if (i == 0) unit = b.unit[turn & 1];
     }
+    const int odd = kTwoS ? i & 1 : 0;
     ok &= mbar_wait(b.s_full + odd, at.s >> odd & 1u, b.abort_flag);
     at.s ^= 1u << odd;
     tc_fence_after();
+    uint32_t r[32];
+    tmem_ld32(tS_i, r);
+    tmem_wait_ld();
+    tmem_ld_fence(r);
     float e[32];
-    {
-      uint32_t r[32];
-      tmem_ld32(tS, r);
-      tmem_wait_ld();
-      tmem_ld_fence(r);
 #pragma unroll
-      for (int c = 0; c < 32; c += 4) {
-        const float4 n = kDq ? make_float4(nl, nl, nl, nl) : col_nl[c / 4];
-        f2_unpack(f2_fma(f2_pack(__uint_as_float(r[c]), __uint_as_float(r[c + 1])), scale2, f2_pack(n.x, n.y)), e[c], e[c + 1]);
-        f2_unpack(f2_fma(f2_pack(__uint_as_float(r[c + 2]), __uint_as_float(r[c + 3])), scale2, f2_pack(n.z, n.w)), e[c + 2],
-                  e[c + 3]);
-      }
+    for (int c = 0; c < 32; c += 4) {
+      const float4 n = kDq ? make_float4(nl, nl, nl, nl) : col_nl[c / 4];
+      f2_unpack(f2_fma(f2_pack(__uint_as_float(r[c]), __uint_as_float(r[c + 1])), scale2, f2_pack(n.x, n.y)), e[c], e[c + 1]);
+      f2_unpack(f2_fma(f2_pack(__uint_as_float(r[c + 2]), __uint_as_float(r[c + 3])), scale2, f2_pack(n.z, n.w)), e[c + 2],
+                e[c + 3]);
     }
     if (kAlibi) {
 #pragma unroll
       for (int c = 0; c < 32; ++c) e[c] = fmaf(-slope, fabsf(static_cast<float>(row - c0 - c)), e[c]);
     }
-    if (kv_tile_needs_mask(c_tile, it.r0, r_last, it.left, it.right, p.seqlen)) {
+    if (cut) {
       const int c_lo = it.left >= 0 ? row - it.left - c0 : -1;
       const int c_hi = min(it.right >= 0 ? row + it.right : p.seqlen - 1, p.seqlen - 1) - c0;
 #pragma unroll
@@ -270,39 +273,36 @@ __device__ __forceinline__ bool bwd_softmax(const BwdParams& p, const BwdItem& i
         e[c + 1] = ex2_approx(e[c + 1]);
       }
     }
+    uint32_t pk[16];
     if (!kDq) {
-      uint32_t pk[16];
 #pragma unroll
       for (int c = 0; c < 16; ++c) pk[c] = pack_f16x2(e[2 * c], e[2 * c + 1]);
-      tmem_st16(tS, pk);
+      tmem_st16(tS_i, pk);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      mbar_arrive_lane0(b.p_ready, lane);
+      mbar_arrive_lane0(b.p_ready + odd, lane);
     }
     ok &= mbar_wait(b.dp_full, at.dp, b.abort_flag);
     at.dp ^= 1;
     tc_fence_after();
-    {
-      uint32_t r[32], pk[16];
-      tmem_ld32(tDp, r);
-      tmem_wait_ld();
-      tmem_ld_fence(r);
-      const uint64_t unit2 = f2_pack(unit, unit);
+    tmem_ld32(tDp, r);
+    tmem_wait_ld();
+    tmem_ld_fence(r);
+    const uint64_t unit2 = f2_pack(unit, unit);
 #pragma unroll
-      for (int c = 0; c < 32; c += 4) {
-        const float4 n = kDq ? make_float4(nd, nd, nd, nd) : col_nd[c / 4];
+    for (int c = 0; c < 32; c += 4) {
+      const float4 n = kDq ? make_float4(nd, nd, nd, nd) : col_nd[c / 4];
 #pragma unroll
-        for (int k = 0; k < 4; k += 2) {
-          float d0, d1;
-          const uint64_t t = f2_fma(f2_pack(__uint_as_float(r[c + k]), __uint_as_float(r[c + k + 1])), unit2,
-                                    k ? f2_pack(n.z, n.w) : f2_pack(n.x, n.y));
-          f2_unpack(f2_mul(t, f2_pack(e[c + k], e[c + k + 1])), d0, d1);
-          pk[(c + k) / 2] = pack_f16x2(d0, d1);
-        }
+      for (int k = 0; k < 4; k += 2) {
+        float d0, d1;
+        const uint64_t t = f2_fma(f2_pack(__uint_as_float(r[c + k]), __uint_as_float(r[c + k + 1])), unit2,
+                                  k ? f2_pack(n.z, n.w) : f2_pack(n.x, n.y));
+        f2_unpack(f2_mul(t, f2_pack(e[c + k], e[c + k + 1])), d0, d1);
+        pk[(c + k) / 2] = pack_f16x2(d0, d1);
       }
-      tmem_st16(kDq ? tS : tDp, pk);
     }
+    tmem_st16(kDq ? tS_i : tDp, pk);
     tmem_wait_st();
     tc_fence_before();
     __syncwarp();
@@ -384,7 +384,7 @@ __device__ __forceinline__ bool bwd_issue(const BwdParams& p, const BwdBars& b, 
   };
   Turn<Cfg::kFirst> f_scores, f_acc;  // first tiles: whose scores come next, whose product comes next
   Turn<Cfg::kSecond> s_scores, s_acc;
-  uint32_t p_at = 0, ds_at = 0, own_at = 0, acc_at = 1;  // (the accumulators are free at the start)
+  uint32_t p_at = 0, ds_at = 0, own_at = 0, acc_at = 1;  // parities, p_at of either p_ready (the accumulators are free at the start)
   for (int k = 0, index; (index = bwd_index(k)) < 2 * p.tiles * p.bh && ok; ++k) {
     const BwdItem it = bwd_item(p, index);
     const int n = it.tiles;
@@ -429,8 +429,9 @@ __device__ __forceinline__ bool bwd_issue(const BwdParams& p, const BwdBars& b, 
       }
     } else {
       for (int i = 0; i < n && ok; ++i) {
-        wait(b.p_ready, p_at);
-        p_at ^= 1;
+        const int odd = two_s ? i & 1 : 0;
+        wait(b.p_ready + odd, p_at >> odd & 1u);
+        p_at ^= 1u << odd;
         accumulate(Cfg::kColDv, s_col(i), second + s_acc.slot * kTile, i > 0);
         umma_commit_warp(b.second_empty + s_acc.slot);
         s_acc.advance();
@@ -491,6 +492,7 @@ __device__ __forceinline__ void bwd_stats(const BwdParams& p, const BwdBars& b, 
   using Cfg = BwdCfg<D>;
   Turn<Cfg::kStats> at;
   at.parity = 1;
+  griddep_wait();
   for (int k = 0, index; (index = bwd_index(k)) < 2 * p.tiles * p.bh; ++k) {
     const BwdItem it = bwd_item(p, index);
     const float unit = bwd_unit(p, it.bh, lane);
@@ -541,8 +543,8 @@ bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
   b.s_full = b.own_full + 4;
   b.stats_empty = b.own_full + 6;  // from here on it is the softmax warps that arrive
   b.p_ready = b.stats_empty + Cfg::kStats;
-  b.ds_ready = b.p_ready + 1;
-  b.acc_empty = b.p_ready + 2;
+  b.ds_ready = b.p_ready + 2;
+  b.acc_empty = b.p_ready + 3;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + Cfg::kNumBars);
   b.abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   b.unit = reinterpret_cast<volatile float*>(tmem_slot + 2);
@@ -564,7 +566,9 @@ bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  griddep_wait();
+  // bwd_rows_kernel lets this kernel in only behind its own griddep_wait(): whatever came before the two of them is complete,
+  // and only the warp that reads what bwd_rows_kernel writes has to wait for it. (Every CTA has one, so whoever waits for this
+  // kernel has waited for both.)
   griddep_launch();
 
   if (warp < Cfg::kSoftmaxWarps) {

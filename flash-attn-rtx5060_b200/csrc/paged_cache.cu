@@ -133,8 +133,8 @@ int flash_cache_append(const fa_paged_cache* cache, const fa_rows* k, const fa_r
     if (reinterpret_cast<uintptr_t>(rotary) & 15) return fail(FA_INVALID_ARG, "rotary must be 16-byte aligned");
   }
   const long long row_units = (2ll * cache->kv_heads + q_heads) * (cache->head_dim / 16);  // of a token
-  if (static_cast<double>(batch) * tokens * row_units >= 256.0 * 0x7fffffff) return fail(FA_INVALID_ARG, "too many rows");
-  const long long units = static_cast<long long>(batch) * tokens * row_units;
+  if (static_cast<long long>(batch) * tokens > 0x7fffffffLL || row_units > 65535ll * 128)
+    return fail(FA_INVALID_ARG, "too many rows");
 
   DeviceState* s = nullptr;
   bool captured = false;
@@ -155,11 +155,12 @@ int flash_cache_append(const fa_paged_cache* cache, const fa_rows* k, const fa_r
   p.rotary_dim = rotary ? rotary_dim : 0;
   p.positions = rotary_positions;
   p.interleaved = interleaved ? 1 : 0;
-  p.units = units;
+  p.row_units = static_cast<int>(row_units);
   const bool half = cache->dtype == FA_FP16, d64 = cache->head_dim == 64;
   const auto kernel = half ? (d64 ? fa::cache_append_kernel<__half, 64> : fa::cache_append_kernel<__half, 128>)
                            : (d64 ? fa::cache_append_kernel<__nv_bfloat16, 64> : fa::cache_append_kernel<__nv_bfloat16, 128>);
-  cudaError_t e = launch_early(kernel, dim3(static_cast<unsigned>((units + 255) / 256)), 256, 0, st, !captured, p);
+  const dim3 grid(static_cast<unsigned>(batch) * tokens, static_cast<unsigned>((row_units + 127) / 128));
+  cudaError_t e = launch_early(kernel, grid, 128, 0, st, !captured, p);
   if (e != cudaSuccess) return fail_cuda("launch cache_append_kernel", e);
   return FA_OK;
 }

@@ -12,6 +12,10 @@ namespace {
 // Two CTAs on each of a B200's 148 SMs: three (head_dim 64: six) stages of 32 KB (16 KB) each keep up to 192 KB a SM in
 // flight. On a device with fewer SMs they run one after the other.
 constexpr int kDecodeCtas = 296;
+constexpr long long kJoinBlocks = 148 * 6;
+// Keys and values that a CTA reads in about the time that a second launch and the join take: a sequence that cannot be longer
+// is not cut.
+constexpr long long kDirectBytes = 256 * 1024;
 
 int check_cache(const fa_paged_cache* c, int batch, int tokens, int q_heads) {
   if (!c) return fail(FA_INVALID_ARG, "cache is null");
@@ -92,11 +96,17 @@ int launch_decode(const CUtensorMap& mk, const CUtensorMap& mv, const fa::Decode
   constexpr auto kernel = fa::decode_kernel<T, D, kRowWarps>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes);
   if (e != cudaSuccess) return fail_cuda("cudaFuncSetAttribute(MaxDynamicSharedMemorySize)", e);
-  e = launch_early(kernel, dim3(p.ctas), Cfg::kThreads, Cfg::kSmemBytes, st, early, mk, mv, p);
+  const unsigned grid = p.direct ? static_cast<unsigned>(p.cache.batch) * p.cache.kv_heads * p.row_tiles : p.ctas;
+  e = launch_early(kernel, dim3(grid), Cfg::kThreads, Cfg::kSmemBytes, st, early, mk, mv, p);
   if (e != cudaSuccess) return fail_cuda("launch decode_kernel", e);
+  if (p.direct) return FA_OK;
   const long long rows = static_cast<long long>(p.cache.batch) * p.q_heads * p.cache.tokens;
-  e = launch_early(fa::decode_join_kernel<T, D>, dim3(static_cast<unsigned>((rows + 3) / 4)), 128, 0, st, early, p,
-                   static_cast<int>(Cfg::kRows));
+  // a row by the four warps of a block while that is one wave of blocks
+  e = rows <= kJoinBlocks
+          ? launch_early(fa::decode_join_kernel<T, D, 4>, dim3(static_cast<unsigned>(rows)), 128, 0, st, early, p,
+                         static_cast<int>(Cfg::kRows))
+          : launch_early(fa::decode_join_kernel<T, D, 1>, dim3(static_cast<unsigned>((rows + 3) / 4)), 128, 0, st, early, p,
+                         static_cast<int>(Cfg::kRows));
   if (e != cudaSuccess) return fail_cuda("launch decode_join_kernel", e);
   return FA_OK;
 }
@@ -212,6 +222,10 @@ int flash_decode(const fa_paged_cache* cache, const fa_rows* q, void* o, float* 
   if (p.box_rows > fa::kDecodeKeys) p.box_rows = fa::kDecodeKeys;
   p.row_tiles = static_cast<int>((rows + tile - 1) / tile);
   p.ctas = kDecodeCtas;
+  long long longest = static_cast<long long>(cache->max_pages) * cache->page_size;  // keys that an item may have
+  if (window_left >= 0 && longest > static_cast<long long>(window_left) + tokens)
+    longest = static_cast<long long>(window_left) + tokens;
+  p.direct = longest * cache->head_dim * 4 <= kDirectBytes;
   p.part_o = static_cast<float*>(workspace);
   p.part_ml = p.part_o + static_cast<size_t>(kDecodeCtas) * 2 * tile * cache->head_dim;
   p.status = s->status;

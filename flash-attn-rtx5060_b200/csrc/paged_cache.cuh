@@ -180,6 +180,7 @@ struct DecodeParams {
   int box_rows;   // rows of a page that one TMA box brings: the largest power of two that divides page_size, 64 at most
   int row_tiles;  // of the group * tokens rows of a key head
   int ctas;
+  int direct;      // 1: a CTA an item, nothing is cut and nothing joined (short sequences)
   float* part_o;   // [ctas][2][rows of a tile][head_dim]
   float* part_ml;  // [ctas][2][rows of a tile][2]: running maximum (log2 units) and sum
   int* status;
@@ -224,6 +225,13 @@ struct DecodeWalk {
   int b, first, tiles, length, count;
 
   __device__ void start(const DecodeParams& p, int cta, int lane) {
+    if (p.direct) {  // one item: `at` and `end` count items
+      b = cta / (p.cache.kv_heads * p.row_tiles);
+      DecodeLine::tiles_of(p, b, first, tiles, length, count);
+      at = begin = 0;
+      end = 1;
+      return;
+    }
     long long all, before;
     DecodeLine::sum(p, 0, all, before, lane);
     const long long share = DecodeLine::share_of(p, all), total = all * p.cache.kv_heads * p.row_tiles;
@@ -260,6 +268,15 @@ struct DecodeWalk {
   // The item at `at`: key head, row tile, and its tiles [t0, t1) of [0, tiles). Moves on behind them.
   __device__ bool next(const DecodeParams& p, int& kv_head, int& row_tile, int& t0, int& t1) {
     if (at >= end) return false;
+    if (p.direct) {
+      const int item = blockIdx.x % (p.cache.kv_heads * p.row_tiles);
+      kv_head = item / p.row_tiles;
+      row_tile = item % p.row_tiles;
+      t0 = 0;
+      t1 = tiles;
+      at = end;
+      return true;
+    }
     const long long per = static_cast<long long>(p.cache.kv_heads) * p.row_tiles;
     while (at >= b_start + tiles * per) {
       b_start += tiles * per;
@@ -282,6 +299,7 @@ struct DecodeCfg {
   static constexpr int kRows = 16 * kRowWarps;
   static constexpr int kKeyWarps = 4 / kRowWarps;
   static constexpr int kWarpKeys = kDecodeKeys / kKeyWarps;  // of a tile, a warp's
+  static constexpr int kChunk = D == 128 || kWarpKeys < 32 ? 16 : 32;  // of them at a time: more spill
   static constexpr int kHalfBytes = kDecodeKeys * D * 2;     // K or V of a tile
   static constexpr int kStages = D == 128 ? 3 : 6;
   static constexpr int kOffJoin = kStages * 2 * kHalfBytes;
@@ -447,10 +465,15 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
       if (ok) {
         const int key0 = (walk.first + t) * kDecodeKeys;
         const uint32_t k_smem = smem_u32(smem + stage * 2 * Cfg::kHalfBytes), v_smem = k_smem + Cfg::kHalfBytes;
-        float s[Cfg::kWarpKeys / 8][4];
+        // does every row see every key of the tile?
+        const bool cut = key0 + kDecodeKeys > first_query + 1 ||
+                         (p.window_left >= 0 && key0 < walk.length - 1 - p.window_left);
+#pragma unroll 1
+        for (int chunk = 0; chunk < Cfg::kWarpKeys; chunk += Cfg::kChunk) {
+        float s[Cfg::kChunk / 8][4];
 #pragma unroll
-        for (int n = 0; n < Cfg::kWarpKeys / 16; ++n) {
-          const uint32_t base = k_smem + row_base(k_row + 16 * n);
+        for (int n = 0; n < Cfg::kChunk / 16; ++n) {
+          const uint32_t base = k_smem + row_base(k_row + chunk + 16 * n);
 #pragma unroll
           for (int i = 0; i < 4; ++i) s[2 * n][i] = s[2 * n + 1][i] = 0.f;
 #pragma unroll
@@ -461,13 +484,10 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
             mma16816<T>(s[2 * n + 1], qf[k], b[2], b[3]);
           }
         }
-        // does every row see every key of the tile?
-        const bool cut = key0 + kDecodeKeys > first_query + 1 ||
-                         (p.window_left >= 0 && key0 < walk.length - 1 - p.window_left);
-        const int warp_key = key0 + key_warp * Cfg::kWarpKeys + 2 * in_quad;
+        const int warp_key = key0 + key_warp * Cfg::kWarpKeys + chunk + 2 * in_quad;
         float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-        for (int n = 0; n < Cfg::kWarpKeys / 8; ++n)
+        for (int n = 0; n < Cfg::kChunk / 8; ++n)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int key = warp_key + 8 * n + (i & 1), r = i >> 1;
@@ -501,7 +521,7 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
         }
         const float off[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
 #pragma unroll
-        for (int n = 0; n < Cfg::kWarpKeys / 16; ++n) {
+        for (int n = 0; n < Cfg::kChunk / 16; ++n) {
           uint32_t pf[4];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
@@ -513,7 +533,7 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
             pf[2 * h] = from_floats<T>(x[0], x[1]);
             pf[2 * h + 1] = from_floats<T>(x[2], x[3]);
           }
-          const uint32_t base = v_smem + row_base(v_row + 16 * n);
+          const uint32_t base = v_smem + row_base(v_row + chunk + 16 * n);
           if (cut) {
             // what lies behind the last token, or in pages in front of the window, is not the sequence's: any bits at all,
             // and 0 * NaN is NaN
@@ -541,6 +561,7 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
               mma16816<T>(o[2 * d + 1], pf, b[2], b[3]);
             }
           }
+        }
         }
       }
       __syncwarp();
@@ -633,47 +654,85 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
   if (!ok && lane == 0) atomicExch(p.status, 1);
 }
 
-// A warp a row: nothing to do where one CTA had the whole item; else the parts are joined in the order of the line. Rows
-// of sequences without keys, and rows of padding, are set to O = 0 and a log-sum-exp of -infinity.
-template <typename T, int D>
-__global__ void __launch_bounds__(128) decode_join_kernel(const __grid_constant__ DecodeParams p, int tile_rows) {
-  const int lane = threadIdx.x & 31;
-  const long long row = blockIdx.x * 4ll + (threadIdx.x >> 5);
-  griddep_wait();
+// kWarps warps a row: nothing to do where one CTA had the whole item; else the parts are joined, every warp those of its turn
+// in the order of the line, then the warps in their order. Rows of sequences without keys, and rows of padding, are set to
+// O = 0 and a log-sum-exp of -infinity.
+template <typename T, int D, int kWarps>
+__global__ void __launch_bounds__(128, 6) decode_join_kernel(const __grid_constant__ DecodeParams p, int tile_rows) {
+  constexpr int kOwn = D / 32;  // elements of a lane
+  __shared__ float s_o[kWarps][D];
+  __shared__ float2 s_ml[kWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, turn = warp % kWarps;
+  const long long row = kWarps == 4 ? blockIdx.x : blockIdx.x * 4ll + warp;
   if (row >= static_cast<long long>(p.cache.batch) * p.q_heads * p.cache.tokens) return;
   const int t = static_cast<int>(row % p.cache.tokens);
   const int bh = static_cast<int>(row / p.cache.tokens), head = bh % p.q_heads, b = bh / p.q_heads;
+  // decode_kernel lets this kernel in only behind its own griddep_wait(), so the lengths are there already
   int first, tiles, length, count;
   DecodeLine::tiles_of(p, b, first, tiles, length, count);
-  constexpr int kOwn = D / 32;  // elements of a lane
+  const bool real = tiles > 0 && t < count;
+  long long c0 = 0, c1 = -1, start = 0, share = 1;
+  const int r = t * p.group + head % p.group;
+  if (real) {
+    long long all, before;
+    DecodeLine::sum(p, b, all, before, lane);
+    const int item = head / p.group * p.row_tiles + r / tile_rows;
+    share = DecodeLine::share_of(p, all);
+    start = before * p.cache.kv_heads * p.row_tiles + static_cast<long long>(item) * tiles;
+    c0 = start / share;
+    c1 = (start + tiles - 1) / share;
+  }
+  griddep_wait();
+  if (real && c0 == c1) return;
+  auto part = [&](long long c) { return (2 * c + (c == c0 && start != c * share ? 1 : 0)) * tile_rows + r % tile_rows; };
   float o[kOwn], m = -INFINITY, l = 0.f;
 #pragma unroll
   for (int i = 0; i < kOwn; ++i) o[i] = 0.f;
-  if (tiles > 0 && t < count) {
-    long long all, before;
-    DecodeLine::sum(p, b, all, before, lane);
-    const int r = t * p.group + head % p.group, item = head / p.group * p.row_tiles + r / tile_rows;
-    const long long share = DecodeLine::share_of(p, all);
-    const long long s = before * p.cache.kv_heads * p.row_tiles + static_cast<long long>(item) * tiles;
-    const long long c0 = s / share, c1 = (s + tiles - 1) / share;
-    if (c0 == c1) return;
-    auto part = [&](long long c) { return (2 * c + (c == c0 && s != c * share ? 1 : 0)) * tile_rows + r % tile_rows; };
-    for (long long c = c0 + lane; c <= c1; c += 32) m = fmaxf(m, p.part_ml[2 * part(c)]);
+  for (long long base = c0 + turn; base <= c1; base += 32 * kWarps) {  // 32 parts at a time, one a lane
+    const long long mine = base + lane * kWarps;
+    const float2 ml = mine <= c1 ? *reinterpret_cast<const float2*>(p.part_ml + 2 * part(mine)) : make_float2(-INFINITY, 0.f);
+    float top = ml.x;
 #pragma unroll
-    for (int i = 16; i > 0; i >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, i));
-    const float off = m == -INFINITY ? 0.f : m;
+    for (int i = 16; i > 0; i >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, i));
+    top = fmaxf(top, m);
+    const float off = top == -INFINITY ? 0.f : top;
+    const float old = ex2_approx(m - off), scale = ex2_approx(ml.x - off);
+    m = top;
+    l *= old;
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) o[i] *= old;
+    const int n = static_cast<int>(c1 - base < 31ll * kWarps ? (c1 - base) / kWarps + 1 : 32);
 #pragma unroll 4
-    for (long long c = c0; c <= c1; ++c) {
-      const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + 2 * part(c));
-      const float scale = ex2_approx(ml.x - off);
-      const float* from = p.part_o + part(c) * D + lane * kOwn;
-      l = fmaf(ml.y, scale, l);
+    for (int k = 0; k < n; ++k) {
+      const float s = __shfl_sync(0xffffffffu, scale, k);
+      const float* from = p.part_o + part(base + k * kWarps) * D + lane * kOwn;
+      l = fmaf(__shfl_sync(0xffffffffu, ml.y, k), s, l);
 #pragma unroll
       for (int i = 0; i < kOwn; i += 2) {
         const float2 x = *reinterpret_cast<const float2*>(from + i);
-        o[i] = fmaf(x.x, scale, o[i]);
-        o[i + 1] = fmaf(x.y, scale, o[i + 1]);
+        o[i] = fmaf(x.x, s, o[i]);
+        o[i + 1] = fmaf(x.y, s, o[i + 1]);
       }
+    }
+  }
+  if constexpr (kWarps > 1) {
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) s_o[turn][lane * kOwn + i] = o[i];
+    if (lane == 0) s_ml[turn] = make_float2(m, l);
+    __syncthreads();
+    if (turn > 0) return;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) m = fmaxf(m, s_ml[w].x);
+    const float off = m == -INFINITY ? 0.f : m;
+    l = 0.f;
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) o[i] = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float s = ex2_approx(s_ml[w].x - off);
+      l = fmaf(s_ml[w].y, s, l);
+#pragma unroll
+      for (int i = 0; i < kOwn; ++i) o[i] = fmaf(s_o[w][lane * kOwn + i], s, o[i]);
     }
   }
   const float inv = l != 0.f ? 1.f / l : 0.f;

@@ -9,13 +9,17 @@ using namespace fa_host;
 
 namespace {
 
-// Two CTAs on each of a B200's 148 SMs: three (head_dim 64: six) stages of 32 KB (16 KB) each keep up to 192 KB a SM in
-// flight. On a device with fewer SMs they run one after the other.
-constexpr int kDecodeCtas = 296;
+// CTAs of a call on a B200's 148 SMs: two a SM for tiles of 16 rows, else one (their rings of tiles keep 192 KB a SM in flight
+// either way). On a device with fewer SMs they run one after the other.
+int decode_ctas(int tile_rows) { return tile_rows == 16 ? 296 : 148; }
 constexpr long long kJoinBlocks = 148 * 6;
-// Keys and values that a CTA reads in about the time that a second launch and the join take: a sequence that cannot be longer
-// is not cut.
-constexpr long long kDirectBytes = 256 * 1024;
+// Whether sequences of up to `longest` keys get a CTA each (and key head and tile of rows) instead of being cut: where they are
+// so short that a second launch and the join would take longer than the two tiles, or are short and fill the SMs by their number.
+// us, cut -> not cut: 128 sequences of up to 400 tokens on 8 key heads of 128 48.5 -> 36.5; 1 x 512 tokens on 4 heads of 64
+// 9.0 -> 9.5 (so that is cut).
+bool decode_direct(long long longest, int tile_keys, long long items, int ctas) {
+  return longest <= 2 * tile_keys || (longest <= 8 * tile_keys && items >= ctas);
+}
 
 int check_cache(const fa_paged_cache* c, int batch, int tokens, int q_heads) {
   if (!c) return fail(FA_INVALID_ARG, "cache is null");
@@ -177,8 +181,8 @@ int flash_cache_append(const fa_paged_cache* cache, const fa_rows* k, const fa_r
 
 size_t flash_decode_workspace_bytes(int tokens, int q_heads, int kv_heads, int head_dim) {
   if (tokens <= 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads != 0 || head_dim <= 0) return 0;
-  return static_cast<size_t>(kDecodeCtas) * 2 * tile_rows(static_cast<long long>(q_heads / kv_heads) * tokens) *
-         (head_dim + 2) * sizeof(float);
+  const int rows = tile_rows(static_cast<long long>(q_heads / kv_heads) * tokens);
+  return static_cast<size_t>(2) * decode_ctas(rows) * rows * (head_dim + 2) * sizeof(float);
 }
 
 int flash_decode(const fa_paged_cache* cache, const fa_rows* q, void* o, float* lse, int batch, int tokens, int q_heads,
@@ -219,15 +223,19 @@ int flash_decode(const fa_paged_cache* cache, const fa_rows* q, void* o, float* 
   p.window_left = window_left;
   p.alibi_slopes = alibi_slopes;
   p.box_rows = cache->page_size & -cache->page_size;
-  if (p.box_rows > fa::kDecodeKeys) p.box_rows = fa::kDecodeKeys;
+  const int tile_keys = cache->head_dim == 128 ? fa::kDecodeKeys<128> : fa::kDecodeKeys<64>;
+  if (p.box_rows > tile_keys) p.box_rows = tile_keys;
+  p.tile_shift = cache->head_dim == 128 ? 6 : 7;
   p.row_tiles = static_cast<int>((rows + tile - 1) / tile);
-  p.ctas = kDecodeCtas;
+  p.ctas = decode_ctas(tile);
   long long longest = static_cast<long long>(cache->max_pages) * cache->page_size;  // keys that an item may have
   if (window_left >= 0 && longest > static_cast<long long>(window_left) + tokens)
     longest = static_cast<long long>(window_left) + tokens;
-  p.direct = longest * cache->head_dim * 4 <= kDirectBytes;
+  const double tiles = static_cast<double>(batch) * cache->kv_heads * p.row_tiles * ((longest + tile_keys - 1) / tile_keys + 1);
+  if (tiles > 0x7fffffff - 512) return fail(FA_INVALID_ARG, "more tiles of keys than 31 bits count");
+  p.direct = decode_direct(longest, tile_keys, static_cast<long long>(batch) * cache->kv_heads * p.row_tiles, p.ctas);
   p.part_o = static_cast<float*>(workspace);
-  p.part_ml = p.part_o + static_cast<size_t>(kDecodeCtas) * 2 * tile * cache->head_dim;
+  p.part_ml = p.part_o + static_cast<size_t>(2) * p.ctas * tile * cache->head_dim;
   p.status = s->status;
   CUtensorMap mk, mv;
   if ((rc = make_page_map(&mk, cache, cache->k, p.box_rows)) != FA_OK) return rc;

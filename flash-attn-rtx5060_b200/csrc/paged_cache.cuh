@@ -166,7 +166,9 @@ __global__ void __launch_bounds__(128) cache_append_kernel(const __grid_constant
 // ---------------------------------------------------------------------------------------------------------------------
 // attention of the newest tokens
 // ---------------------------------------------------------------------------------------------------------------------
-constexpr int kDecodeKeys = 64;  // keys of a tile
+// Keys of a tile: 32 KB of keys and values.
+template <int D>
+constexpr int kDecodeKeys = D == 128 ? 64 : 128;
 
 struct DecodeParams {
   CacheView cache;
@@ -177,7 +179,8 @@ struct DecodeParams {
   float scale_log2;
   int window_left;  // < 0: unbounded
   const float* alibi_slopes;
-  int box_rows;   // rows of a page that one TMA box brings: the largest power of two that divides page_size, 64 at most
+  int tile_shift;  // a tile has 2^tile_shift keys
+  int box_rows;   // rows of a page that one TMA box brings: the largest power of two that divides page_size, a tile at most
   int row_tiles;  // of the group * tokens rows of a key head
   int ctas;
   int direct;      // 1: a CTA an item, nothing is cut and nothing joined (short sequences)
@@ -194,11 +197,11 @@ struct DecodeLine {
   __device__ static void tiles_of(const DecodeParams& p, int b, int& first, int& tiles, int& length, int& count) {
     sequence_of(p.cache, b, length, count);
     const int lo = p.window_left >= 0 && length - count > p.window_left ? length - count - p.window_left : 0;
-    first = lo / kDecodeKeys;
-    tiles = count > 0 ? (length + kDecodeKeys - 1) / kDecodeKeys - first : 0;
+    first = lo >> p.tile_shift;
+    tiles = count > 0 ? ((length - 1) >> p.tile_shift) + 1 - first : 0;
   }
   // Sums the tiles of one key head over all sequences and over those in front of `upto`. All lanes of a warp call it.
-  __device__ static void sum(const DecodeParams& p, int upto, long long& all, long long& before, int lane) {
+  __device__ static void sum(const DecodeParams& p, int upto, int& all, int& before, int lane) {
     all = before = 0;
     for (int b = lane; b < p.cache.batch; b += 32) {
       int first, tiles, length, count;
@@ -212,16 +215,15 @@ struct DecodeLine {
       before += __shfl_xor_sync(0xffffffffu, before, s);
     }
   }
-  __device__ static long long share_of(const DecodeParams& p, long long all) {
-    const long long total = all * p.cache.kv_heads * p.row_tiles;
-    return (total + p.ctas - 1) / p.ctas;
+  __device__ static int share_of(const DecodeParams& p, int all) {
+    return static_cast<int>((static_cast<unsigned>(all) * p.cache.kv_heads * p.row_tiles + p.ctas - 1) / p.ctas);
   }
 };
 
 // A stretch of the line, walked item by item; every role of a CTA walks it for itself.
 struct DecodeWalk {
-  long long at, begin, end;  // of the line
-  long long b_start;   // where sequence b starts
+  int at, begin, end;  // of the line
+  int b_start;         // where sequence b starts
   int b, first, tiles, length, count;
 
   __device__ void start(const DecodeParams& p, int cta, int lane) {
@@ -232,22 +234,22 @@ struct DecodeWalk {
       end = 1;
       return;
     }
-    long long all, before;
+    int all, before;
     DecodeLine::sum(p, 0, all, before, lane);
-    const long long share = DecodeLine::share_of(p, all), total = all * p.cache.kv_heads * p.row_tiles;
-    at = begin = cta * share;
-    end = at + share < total ? at + share : total;
+    const int share = DecodeLine::share_of(p, all), total = all * p.cache.kv_heads * p.row_tiles;
+    at = begin = min(cta * share, total);  // (ctas * share exceeds the total by less than ctas)
+    end = min(at + share, total);
     b = 0;
     b_start = 0;
     // the sequence that holds `at`, 32 at a time
-    const long long per = static_cast<long long>(p.cache.kv_heads) * p.row_tiles;
+    const int per = p.cache.kv_heads * p.row_tiles;
     for (int b0 = 0; at < end; b0 += 32) {
       int f = 0, n = 0, len = 0, cnt = 0;
       if (b0 + lane < p.cache.batch) DecodeLine::tiles_of(p, b0 + lane, f, n, len, cnt);
-      long long upto = n;
+      int upto = n;
 #pragma unroll
       for (int s = 1; s < 32; s <<= 1) {
-        const long long v = __shfl_up_sync(0xffffffffu, upto, s);
+        const int v = __shfl_up_sync(0xffffffffu, upto, s);
         if (lane >= s) upto += v;
       }
       upto = b_start + upto * per;
@@ -277,36 +279,40 @@ struct DecodeWalk {
       at = end;
       return true;
     }
-    const long long per = static_cast<long long>(p.cache.kv_heads) * p.row_tiles;
+    const int per = p.cache.kv_heads * p.row_tiles;
     while (at >= b_start + tiles * per) {
       b_start += tiles * per;
       ++b;
       DecodeLine::tiles_of(p, b, first, tiles, length, count);
     }
-    const int item = static_cast<int>((at - b_start) / tiles);
+    const int item = (at - b_start) / tiles;
     kv_head = item / p.row_tiles;
     row_tile = item % p.row_tiles;
-    t0 = static_cast<int>((at - b_start) % tiles);
-    t1 = static_cast<int>(end - at < tiles - t0 ? t0 + (end - at) : tiles);
+    t0 = at - b_start - item * tiles;
+    t1 = min(t0 + end - at, tiles);
     at += t1 - t0;
     return true;
   }
 };
 
+// 16 rows: four warps that compute and two CTAs a SM. More rows: eight warps and one CTA a SM, whose threads have the registers
+// for 32 keys' scores at a time (a warp's work on a tile is one chain of latencies: 16 keys or 32 take it about as long).
 template <int D, int kRowWarps>
 struct DecodeCfg {
-  static constexpr int kThreads = 160;  // four warps that compute, one that loads
+  static constexpr int kWarps = kRowWarps == 1 ? 4 : 8;
+  static constexpr int kThreads = kWarps * 32 + 32;  // and one that loads
+  static constexpr int kCtasPerSm = kRowWarps == 1 ? 2 : 1;
   static constexpr int kRows = 16 * kRowWarps;
-  static constexpr int kKeyWarps = 4 / kRowWarps;
-  static constexpr int kWarpKeys = kDecodeKeys / kKeyWarps;  // of a tile, a warp's
-  static constexpr int kChunk = D == 128 || kWarpKeys < 32 ? 16 : 32;  // of them at a time: more spill
-  static constexpr int kHalfBytes = kDecodeKeys * D * 2;     // K or V of a tile
-  static constexpr int kStages = D == 128 ? 3 : 6;
+  static constexpr int kKeys = kDecodeKeys<D>;
+  static constexpr int kKeyWarps = kWarps / kRowWarps;
+  static constexpr int kWarpKeys = kKeys / kKeyWarps;  // of a tile, a warp's
+  static constexpr int kChunk = kWarpKeys < 32 ? kWarpKeys : 32;  // of them at a time
+  static constexpr int kHalfBytes = kKeys * D * 2;  // K or V of a tile
+  static constexpr int kStages = 6 / kCtasPerSm;
   static constexpr int kOffJoin = kStages * 2 * kHalfBytes;
-  // O of two warps a row group (four key warps), or of one (two); with the maxima and sums of all
-  static constexpr int kJoinBytes = kKeyWarps == 1 ? 0 : (kKeyWarps / 2) * kRows * D * 4;
-  static constexpr int kOffMl = kOffJoin + kJoinBytes;
-  static constexpr int kOffBars = kOffMl + 4 * 16 * 8;
+  static constexpr int kJoinBytes = (kKeyWarps / 2) * kRows * D * 4;  // O of half of the key warps
+  static constexpr int kOffMl = kOffJoin + kJoinBytes;  // maxima and sums of all warps' rows
+  static constexpr int kOffBars = kOffMl + kWarps * 16 * 8;
   static constexpr int kSmemBytes = kOffBars + kStages * 16 + 16;
 };
 
@@ -343,17 +349,20 @@ __device__ __forceinline__ void tma_load_5d(void* smem_dst, const CUtensorMap* m
         "r"(c3), "r"(c4)
       : "memory");
 }
-// barrier of the four warps that compute
-__device__ __forceinline__ void compute_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+// barrier of the warps that compute
+template <int kThreads>
+__device__ __forceinline__ void compute_sync() {
+  asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory");
+}
 
-// A CTA's four compute warps take 16 * kRowWarps rows (a row: one query head of the key head's group and one new token)
-// and share a tile's keys where the rows are fewer than 64. The products run as m16n8k16 matrix instructions: a step of
+// A CTA's warps take 16 * kRowWarps rows (a row: one query head of the key head's group and one new token) and share a tile's
+// keys. The products run as m16n8k16 matrix instructions: a step of
 // generation reads every key for a handful of rows, so HBM is what bounds it (at 16 rows a tile of 64 keys is 32 KB and
 // 128 instructions of the SM's warps), and rows that are padding cost nothing that matters. Scores, maxima, sums and O
 // are fp32; P is rounded to the cache's type for the second product, as the operand has to be, against a maximum that
 // is exact for the warp's own keys.
 template <typename T, int D, int kRowWarps>
-__global__ void __launch_bounds__(160, 2)
+__global__ void __launch_bounds__(DecodeCfg<D, kRowWarps>::kThreads, DecodeCfg<D, kRowWarps>::kCtasPerSm)
 decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
               const __grid_constant__ DecodeParams p) {
   using Cfg = DecodeCfg<D, kRowWarps>;
@@ -365,7 +374,7 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
   if (threadIdx.x == 0) {
     for (int i = 0; i < Cfg::kStages; ++i) {
       mbar_init(full + i, 1);
-      mbar_init(empty + i, 4);
+      mbar_init(empty + i, Cfg::kWarps);
     }
     *abort_flag = 0;
     fence_mbar_init();
@@ -378,9 +387,9 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
   int kv_head, row_tile, t0, t1, stage = 0;
   uint32_t phase = 0;
 
-  if (warp == 4) {
+  if (warp == Cfg::kWarps) {
     // ---- loads: lane i brings box i of the tile's keys and of its values ----
-    const int boxes = kDecodeKeys / p.box_rows;
+    const int boxes = Cfg::kKeys / p.box_rows;
     const uint32_t box_bytes = p.box_rows * D * 2;
     bool ok = true;
     while (ok && walk.next(p, kv_head, row_tile, t0, t1)) {
@@ -388,7 +397,7 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
                          ? walk.length - walk.count - p.window_left : 0;
       const int* table = p.cache.page_table + walk.b * p.cache.table_stride;
       auto page_of = [&](int tile) {  // -1: the box holds nothing that is seen
-        const int key = (walk.first + tile) * kDecodeKeys + lane * p.box_rows;
+        const int key = (walk.first + tile) * Cfg::kKeys + lane * p.box_rows;
         if (lane >= boxes || tile >= t1 || key >= walk.length || key + p.box_rows <= lo) return -1;
         const int page = table[key / p.cache.page_size];
         if (page >= 0 && page < p.cache.num_pages) return page;
@@ -405,7 +414,7 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
         __syncwarp();
         if (page >= 0) {
           uint8_t* dst = smem + stage * 2 * Cfg::kHalfBytes + lane * box_bytes;
-          const int row = ((walk.first + t) * kDecodeKeys + lane * p.box_rows) % p.cache.page_size;
+          const int row = ((walk.first + t) * Cfg::kKeys + lane * p.box_rows) % p.cache.page_size;
           tma_load_5d(dst, &map_k, full + stage, 0, row, 0, kv_head, page);
           tma_load_5d(dst + Cfg::kHalfBytes, &map_v, full + stage, 0, row, 0, kv_head, page);
         }
@@ -432,7 +441,7 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
     return (row >> box_shift) * (p.box_rows * D * 2) + (row & (p.box_rows - 1)) * 128;
   };
   const uint32_t panel = p.box_rows * 128;
-  bool ok = true;  // once a wait has run out, the warp goes on without its tiles: the others may wait for it
+  bool ok = true;  // once a wait has run out, the warp goes on with whatever is there: the others may wait for it
 
   while (walk.next(p, kv_head, row_tile, t0, t1)) {
     // this thread's two rows
@@ -461,12 +470,12 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
     for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
 
     for (int t = t0; t < t1; ++t) {
-      ok = ok && mbar_wait_warp(full + stage, phase, abort_flag);
-      if (ok) {
-        const int key0 = (walk.first + t) * kDecodeKeys;
+      ok &= mbar_wait(full + stage, phase, abort_flag);  // (looked at once an item: a vote costs more than the wait)
+      {
+        const int key0 = (walk.first + t) * Cfg::kKeys;
         const uint32_t k_smem = smem_u32(smem + stage * 2 * Cfg::kHalfBytes), v_smem = k_smem + Cfg::kHalfBytes;
         // does every row see every key of the tile?
-        const bool cut = key0 + kDecodeKeys > first_query + 1 ||
+        const bool cut = key0 + Cfg::kKeys > first_query + 1 ||
                          (p.window_left >= 0 && key0 < walk.length - 1 - p.window_left);
 #pragma unroll 1
         for (int chunk = 0; chunk < Cfg::kWarpKeys; chunk += Cfg::kChunk) {
@@ -474,15 +483,20 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
 #pragma unroll
         for (int n = 0; n < Cfg::kChunk / 16; ++n) {
           const uint32_t base = k_smem + row_base(k_row + chunk + 16 * n);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) s[2 * n][i] = s[2 * n + 1][i] = 0.f;
+          // (two partial sums each where a warp has 16 keys only: four chains of products instead of two)
+          constexpr int kSplit = Cfg::kChunk == 16 ? 2 : 1;
+          float part[kSplit][2][4] = {};
 #pragma unroll
           for (int k = 0; k < D / 16; ++k) {
             uint32_t b[4];
             ldsm4(base + (k / 4) * panel + ((((k % 4) * 2 + k_chunk) ^ (k_row & 7)) << 4), b);
-            mma16816<T>(s[2 * n], qf[k], b[0], b[1]);
-            mma16816<T>(s[2 * n + 1], qf[k], b[2], b[3]);
+            mma16816<T>(part[k % kSplit][0], qf[k], b[0], b[1]);
+            mma16816<T>(part[k % kSplit][1], qf[k], b[2], b[3]);
           }
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) s[2 * n + h][i] = kSplit == 2 ? part[0][h][i] + part[kSplit - 1][h][i] : part[0][h][i];
         }
         const int warp_key = key0 + key_warp * Cfg::kWarpKeys + chunk + 2 * in_quad;
         float top[2] = {-INFINITY, -INFINITY};
@@ -569,6 +583,7 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
       if (++stage == Cfg::kStages) stage = 0, phase ^= 1;
     }
 
+    ok = __all_sync(0xffffffffu, ok);
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
@@ -581,7 +596,7 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
         ml[warp * 16 + quad] = make_float2(m[0], l[0]);
         ml[warp * 16 + quad + 8] = make_float2(m[1], l[1]);
       }
-      compute_sync();
+      compute_sync<Cfg::kWarps * 32>();
       float scale[2];
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
@@ -610,7 +625,7 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
             buf[(2 * n + 1) * 32] = make_float2(o[n][2] * c1, o[n][3] * c1);
           }
         }
-        compute_sync();
+        compute_sync<Cfg::kWarps * 32>();
         if (key_warp < step) {
 #pragma unroll
           for (int n = 0; n < D / 8; ++n) {
@@ -622,7 +637,7 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
             o[n][3] = fmaf(o[n][3], c1, c.y);
           }
         }
-        compute_sync();
+        compute_sync<Cfg::kWarps * 32>();
       }
     }
     if (key_warp == 0) {
@@ -671,25 +686,27 @@ __global__ void __launch_bounds__(128, 6) decode_join_kernel(const __grid_consta
   int first, tiles, length, count;
   DecodeLine::tiles_of(p, b, first, tiles, length, count);
   const bool real = tiles > 0 && t < count;
-  long long c0 = 0, c1 = -1, start = 0, share = 1;
+  int c0 = 0, c1 = -1, start = 0, share = 1;
   const int r = t * p.group + head % p.group;
   if (real) {
-    long long all, before;
+    int all, before;
     DecodeLine::sum(p, b, all, before, lane);
     const int item = head / p.group * p.row_tiles + r / tile_rows;
     share = DecodeLine::share_of(p, all);
-    start = before * p.cache.kv_heads * p.row_tiles + static_cast<long long>(item) * tiles;
+    start = before * p.cache.kv_heads * p.row_tiles + item * tiles;
     c0 = start / share;
     c1 = (start + tiles - 1) / share;
   }
   griddep_wait();
   if (real && c0 == c1) return;
-  auto part = [&](long long c) { return (2 * c + (c == c0 && start != c * share ? 1 : 0)) * tile_rows + r % tile_rows; };
+  auto part = [&](int c) {
+    return (2ll * c + (c == c0 && start != c * share ? 1 : 0)) * tile_rows + r % tile_rows;
+  };
   float o[kOwn], m = -INFINITY, l = 0.f;
 #pragma unroll
   for (int i = 0; i < kOwn; ++i) o[i] = 0.f;
-  for (long long base = c0 + turn; base <= c1; base += 32 * kWarps) {  // 32 parts at a time, one a lane
-    const long long mine = base + lane * kWarps;
+  for (int base = c0 + turn; base <= c1; base += 32 * kWarps) {  // 32 parts at a time, one a lane
+    const int mine = base + lane * kWarps;
     const float2 ml = mine <= c1 ? *reinterpret_cast<const float2*>(p.part_ml + 2 * part(mine)) : make_float2(-INFINITY, 0.f);
     float top = ml.x;
 #pragma unroll
@@ -701,7 +718,7 @@ __global__ void __launch_bounds__(128, 6) decode_join_kernel(const __grid_consta
     l *= old;
 #pragma unroll
     for (int i = 0; i < kOwn; ++i) o[i] *= old;
-    const int n = static_cast<int>(c1 - base < 31ll * kWarps ? (c1 - base) / kWarps + 1 : 32);
+    const int n = min((c1 - base) / kWarps + 1, 32);
 #pragma unroll 4
     for (int k = 0; k < n; ++k) {
       const float s = __shfl_sync(0xffffffffu, scale, k);

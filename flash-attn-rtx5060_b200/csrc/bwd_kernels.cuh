@@ -44,8 +44,9 @@ __global__ void __launch_bounds__(256) bwd_rows_kernel(const BwdParams p) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const size_t head = blockIdx.y;
   float top[3] = {0.f, 0.f, 0.f};
-#pragma unroll 2
-  for (int r = blockIdx.x * 128 + warp * 16 + lane / kLanes, i = 0; i < 16 / kRows; ++i, r += kRows) {
+#pragma unroll 4
+  for (int i = 0; i < 16 / kRows; ++i) {
+    const int r = blockIdx.x * 128 + warp * 16 + i * kRows + lane / kLanes;
     float dot = 0.f, gg = 0.f, vv = 0.f;
     if (r < p.seqlen) {
       const size_t at = (head * p.seqlen + r) * D + (lane % kLanes) * 8;
@@ -554,12 +555,10 @@ bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
     tmem_alloc(tmem_slot, Cfg::kTmemCols);
     tmem_relinquish();
   }
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < Cfg::kNumBars; ++i) {
-      uint64_t* bar = bars + i;
-      mbar_init(bar, bar >= b.stats_empty ? Cfg::kSoftmaxWarps : 1);
-    }
-    *b.abort_flag = 0;
+  static_assert(Cfg::kNumBars <= 64);
+  if (warp == 0) {  // (a thread for one barrier or two: one after the other they cost a short call 0.2 us)
+    for (int i = lane; i < Cfg::kNumBars; i += 32) mbar_init(bars + i, bars + i >= b.stats_empty ? Cfg::kSoftmaxWarps : 1);
+    if (lane == 0) *b.abort_flag = 0;
     fence_mbar_init();
   }
   tc_fence_before();

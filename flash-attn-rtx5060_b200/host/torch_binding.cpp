@@ -13,6 +13,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/PythonTorchFunctionTLS.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_like.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
@@ -178,8 +179,13 @@ bool lies_on(const at::Tensor& t, int64_t device, at::ScalarType type) {
   return t.is_cuda() && t.get_device() == device && t.scalar_type() == type;
 }
 void* data_of(const at::Tensor* t) { return t ? t->data_ptr() : nullptr; }
+// at::empty() of a contiguous CUDA tensor without the dispatcher, which no mode is active to hear of (modes() is asked first):
+// 0.4 us less each
+at::Tensor new_tensor(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor& like) {
+  return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt);
+}
 at::Tensor workspace_of(size_t bytes, const at::Tensor& like) {
-  return at::empty({static_cast<int64_t>(bytes)}, like.options().dtype(at::kByte));
+  return new_tensor({static_cast<int64_t>(bytes)}, at::kByte, like);
 }
 // false (and no error) for what is not a number that the C entry points take
 bool scale_of(PyObject* o, float* scale) {
@@ -216,7 +222,7 @@ PyObject* backward(PyObject* self, PyObject* const* a, Py_ssize_t n) {
   if (slopes && (!lies_on(*slopes, device, at::kFloat) || !slopes->is_contiguous() || slopes->numel() != H)) return not_here();
   const Operators& lib = operators(self);
   at::Tensor grads[3];
-  for (int i = 0; i < 3; ++i) grads[i] = given[i] ? *given[i] : at::empty_like(*q);
+  for (int i = 0; i < 3; ++i) grads[i] = given[i] ? *given[i] : new_tensor(q->sizes(), at::kHalf, *q);
   const int b = static_cast<int>(B), h = static_cast<int>(H), s = static_cast<int>(N), d = static_cast<int>(q->size(3));
   const size_t bytes = lib.backward_bytes(b, h, s);
   const at::Tensor ws = workspace_of(bytes, *q);
@@ -295,7 +301,7 @@ PyObject* append(PyObject* self, PyObject* const* a, Py_ssize_t n) {
     return not_here();
   if (given && !cache.output(*given, *q)) return not_here();
   at::Tensor q_out;
-  if (q) q_out = given ? *given : at::empty(q->sizes(), q->options());
+  if (q) q_out = given ? *given : new_tensor(q->sizes(), q->scalar_type(), *q);
   void* stream = c10::cuda::getCurrentCUDAStream(k->get_device()).stream();
   const int b = static_cast<int>(B), t = static_cast<int>(T), q_heads = q ? static_cast<int>(q->size(1)) : 0;
   const int dim = rotary ? static_cast<int>(rotary->size(1)) : 0, positions = rotary ? static_cast<int>(rotary->size(0)) : 0;
@@ -329,9 +335,9 @@ PyObject* decode(PyObject* self, PyObject* const* a, Py_ssize_t n) {
     return not_here();
   if (given && !cache.output(*given, *q)) return not_here();
   const bool want_lse = a[9] == Py_True;
-  const at::Tensor out = given ? *given : at::empty(q->sizes(), q->options());
+  const at::Tensor out = given ? *given : new_tensor(q->sizes(), q->scalar_type(), *q);
   at::Tensor lse;
-  if (want_lse) lse = at::empty({B, H, T}, q->options().dtype(at::kFloat));
+  if (want_lse) lse = new_tensor({B, H, T}, at::kFloat, *q);
   const Operators& lib = operators(self);
   const int b = static_cast<int>(B), h = static_cast<int>(H), t = static_cast<int>(T), wl = low_int(a[7]);
   const size_t bytes = lib.decode_bytes(t, h, cache.c.kv_heads, cache.c.head_dim);

@@ -193,6 +193,25 @@ def test_append_without_rotation_and_in_place(pkg):
     assert same is q and torch.equal(q, apart)
 
 
+def test_append_of_many_tokens_and_of_keys_alone(pkg):
+    """More tokens than blocks that run at once (a block then has a whole token), and a rotation without queries."""
+    lengths = [700, 333, 640]
+    b = oracle.Batch(32, lengths, [640, 200, 640], 640, 2, 128, 16, "fp16")
+    k, v, q = b.rows(2), b.rows(2), b.rows(6)
+    rotary = oracle.angles(700, 64)
+    want = oracle.append(b, k, v, q, rotary)
+    args = b.cuda()
+    turned = pkg.cache_append(k.cuda(), v.cuda(), *args, counts=b.cuda_counts(), q=q.cuda(), rotary=rotary.cuda())
+    alone = b.cuda()
+    assert pkg.cache_append(k.cuda(), v.cuda(), *alone, counts=b.cuda_counts(), rotary=rotary.cuda()) is None
+    pkg.check(torch.cuda.current_stream().cuda_stream)
+    assert torch.equal(args[0], alone[0]) and torch.equal(args[1], alone[1])
+    assert torch.equal(args[1].cpu().double(), want[1])
+    # |a| + |b| of normal values is below 12
+    for got, w in ((args[0].cpu(), want[0]), (turned.cpu(), want[2])):
+        assert ((got.double() - w).abs() <= 2.0 ** -11 * w.abs() + 3 * 2.0 ** -24 * 12 + 2.0 ** -24).all()
+
+
 def test_bad_indices_are_reported(pkg):
     """Pages, lengths, counts and positions outside their ranges become a status; the other sequences are unharmed."""
     stream = torch.cuda.current_stream().cuda_stream

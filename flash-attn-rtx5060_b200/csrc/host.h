@@ -79,19 +79,27 @@ int check_scale(float softmax_scale);
 // graph: two such launches in a row would leave a programmatic edge there, and cudaGraphGetEdges and the like, which
 // report plain edges only, would answer cudaErrorLossyQuery for the caller's whole graph.
 template <typename... Params, typename... Args>
-cudaError_t launch_early(void (*kernel)(Params...), dim3 grid, int threads, int smem, cudaStream_t st, bool early,
-                         Args&&... args) {
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = early ? 1 : 0;
+cudaError_t launch_early_in_clusters(void (*kernel)(Params...), int cluster, dim3 grid, int threads, int smem, cudaStream_t st,
+                                     bool early, Args&&... args) {
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = early ? 1 : 0;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+template <typename... Params, typename... Args>
+cudaError_t launch_early(void (*kernel)(Params...), dim3 grid, int threads, int smem, cudaStream_t st, bool early,
+                         Args&&... args) {
+  return launch_early_in_clusters(kernel, 1, grid, threads, smem, st, early, args...);
 }
 
 }  // namespace fa_host

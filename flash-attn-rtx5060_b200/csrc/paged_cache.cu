@@ -13,12 +13,16 @@ namespace {
 // either way). On a device with fewer SMs they run one after the other.
 int decode_ctas(int tile_rows) { return tile_rows == 16 ? 296 : 148; }
 constexpr long long kJoinBlocks = 148 * 6;
-// Whether sequences of up to `longest` keys get a CTA each (and key head and tile of rows) instead of being cut: where they are
-// so short that a second launch and the join would take longer than the two tiles, or are short and fill the SMs by their number.
-// us, cut -> not cut: 128 sequences of up to 400 tokens on 8 key heads of 128 48.5 -> 36.5; 1 x 512 tokens on 4 heads of 64
-// 9.0 -> 9.5 (so that is cut).
-bool decode_direct(long long longest, int tile_keys, long long items, int ctas) {
-  return longest <= 2 * tile_keys || (longest <= 8 * tile_keys && items >= ctas);
+// CTAs of a cluster that takes an item (a sequence, key head and tile of rows) of up to `tiles` tiles of keys as a whole, 1 for
+// a CTA alone, or 0 where the items are cut by the line and joined by a second launch (which takes as long as four tiles or
+// five). An item of two tiles has a CTA; short items of a large batch fill the SMs by their number; fewer items have clusters of
+// up to eight CTAs, where a CTA's tiles are not many more than if the line had cut them, and uneven lengths cannot cost much.
+// us, cut -> not cut (sequences x longest, key heads, head_dim): 1 x 512, 4, 64 8.6 -> 6.5; 1 x 512, 8, 128 8.2 -> 6.8;
+// 1 x 2048, 8, 128 9.5 -> 9.1; 4 x 2048, 8, 128 11.7 -> 10.2; 128 x 400, 8, 128 48.5 -> 34.5; but 1 x 4096, 4, 64 8.8 -> 9.7.
+int decode_cluster(long long tiles, long long items, int ctas) {
+  if (tiles <= 2 || (tiles <= 8 && items >= ctas)) return 1;
+  if (8 * items > ctas || tiles > 64 || tiles * (ctas - 8 * items) > 26ll * ctas) return 0;
+  return tiles <= 4 ? 4 : 8;
 }
 
 int check_cache(const fa_paged_cache* c, int batch, int tokens, int q_heads) {
@@ -100,10 +104,12 @@ int launch_decode(const CUtensorMap& mk, const CUtensorMap& mv, const fa::Decode
   constexpr auto kernel = fa::decode_kernel<T, D, kRowWarps>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes);
   if (e != cudaSuccess) return fail_cuda("cudaFuncSetAttribute(MaxDynamicSharedMemorySize)", e);
-  const unsigned grid = p.direct ? static_cast<unsigned>(p.cache.batch) * p.cache.kv_heads * p.row_tiles : p.ctas;
-  e = launch_early(kernel, dim3(grid), Cfg::kThreads, Cfg::kSmemBytes, st, early, mk, mv, p);
+  const unsigned grid =
+      p.cluster > 0 ? static_cast<unsigned>(p.cluster) * p.cache.batch * p.cache.kv_heads * p.row_tiles : p.ctas;
+  e = launch_early_in_clusters(kernel, p.cluster > 0 ? p.cluster : 1, dim3(grid), Cfg::kThreads, Cfg::kSmemBytes, st, early, mk, mv,
+                               p);
   if (e != cudaSuccess) return fail_cuda("launch decode_kernel", e);
-  if (p.direct) return FA_OK;
+  if (p.cluster > 0) return FA_OK;
   const long long rows = static_cast<long long>(p.cache.batch) * p.q_heads * p.cache.tokens;
   // a row by the four warps of a block while that is one wave of blocks
   e = rows <= kJoinBlocks
@@ -231,9 +237,11 @@ int flash_decode(const fa_paged_cache* cache, const fa_rows* q, void* o, float* 
   long long longest = static_cast<long long>(cache->max_pages) * cache->page_size;  // keys that an item may have
   if (window_left >= 0 && longest > static_cast<long long>(window_left) + tokens)
     longest = static_cast<long long>(window_left) + tokens;
-  const double tiles = static_cast<double>(batch) * cache->kv_heads * p.row_tiles * ((longest + tile_keys - 1) / tile_keys + 1);
-  if (tiles > 0x7fffffff - 512) return fail(FA_INVALID_ARG, "more tiles of keys than 31 bits count");
-  p.direct = decode_direct(longest, tile_keys, static_cast<long long>(batch) * cache->kv_heads * p.row_tiles, p.ctas);
+  const long long tiles = (longest + tile_keys - 1) / tile_keys + (window_left >= 0);
+  const long long items = static_cast<long long>(batch) * cache->kv_heads * p.row_tiles;
+  if (static_cast<double>(items) * (tiles + 1) > 0x7fffffff - 512)
+    return fail(FA_INVALID_ARG, "more tiles of keys than 31 bits count");
+  p.cluster = decode_cluster(tiles, items, p.ctas);
   p.part_o = static_cast<float*>(workspace);
   p.part_ml = p.part_o + static_cast<size_t>(2) * p.ctas * tile * cache->head_dim;
   p.status = s->status;

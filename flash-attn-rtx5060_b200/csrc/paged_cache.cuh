@@ -183,7 +183,7 @@ struct DecodeParams {
   int box_rows;   // rows of a page that one TMA box brings: the largest power of two that divides page_size, a tile at most
   int row_tiles;  // of the group * tokens rows of a key head
   int ctas;
-  int direct;      // 1: a CTA an item, nothing is cut and nothing joined (short sequences)
+  int cluster;     // CTAs of a cluster that share an item and join it themselves (1: a CTA an item), or 0: the line below
   float* part_o;   // [ctas][2][rows of a tile][head_dim]
   float* part_ml;  // [ctas][2][rows of a tile][2]: running maximum (log2 units) and sum
   int* status;
@@ -192,7 +192,8 @@ struct DecodeParams {
 // The work is one line of tiles of 64 keys: sequence by sequence, in each key head by key head (and row tile by row
 // tile), the tiles that the new tokens see. Every CTA takes an equal stretch of the line. A (sequence, key head, row tile)
 // that lies within one stretch is finished there; one that is cut has its parts written as (maximum, sum, unnormalised
-// output) and joined by decode_join_kernel in the order of the line, so the results depend on the lengths alone.
+// output) and joined by decode_join_kernel in the order of the line, so the results depend on the lengths alone. Where few
+// items are short, or many are very short, an item has a cluster of CTAs, or one CTA, to itself instead, and no second launch.
 struct DecodeLine {
   __device__ static void tiles_of(const DecodeParams& p, int b, int& first, int& tiles, int& length, int& count) {
     sequence_of(p.cache, b, length, count);
@@ -227,8 +228,8 @@ struct DecodeWalk {
   int b, first, tiles, length, count;
 
   __device__ void start(const DecodeParams& p, int cta, int lane) {
-    if (p.direct) {  // one item: `at` and `end` count items
-      b = cta / (p.cache.kv_heads * p.row_tiles);
+    if (p.cluster > 0) {  // one item: `at` and `end` count items
+      b = cta / (p.cluster * p.cache.kv_heads * p.row_tiles);
       DecodeLine::tiles_of(p, b, first, tiles, length, count);
       at = begin = 0;
       end = 1;
@@ -270,12 +271,13 @@ struct DecodeWalk {
   // The item at `at`: key head, row tile, and its tiles [t0, t1) of [0, tiles). Moves on behind them.
   __device__ bool next(const DecodeParams& p, int& kv_head, int& row_tile, int& t0, int& t1) {
     if (at >= end) return false;
-    if (p.direct) {
-      const int item = blockIdx.x % (p.cache.kv_heads * p.row_tiles);
+    if (p.cluster > 0) {
+      const int item = blockIdx.x / p.cluster % (p.cache.kv_heads * p.row_tiles);
       kv_head = item / p.row_tiles;
       row_tile = item % p.row_tiles;
-      t0 = 0;
-      t1 = tiles;
+      const int share = (tiles + p.cluster - 1) / p.cluster, rank = blockIdx.x % p.cluster;
+      t0 = min(rank * share, tiles);
+      t1 = min(t0 + share, tiles);
       at = end;
       return true;
     }
@@ -348,6 +350,15 @@ __device__ __forceinline__ void tma_load_5d(void* smem_dst, const CUtensorMap* m
       : "r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2),
         "r"(c3), "r"(c4)
       : "memory");
+}
+// Two floats from the shared memory of CTA `rank` of the cluster, at the place of `here` in this CTA's.
+__device__ __forceinline__ float2 dsmem_ld2(const void* here, uint32_t rank) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];"
+               : "=f"(v.x), "=f"(v.y)
+               : "r"(mapa_u32(smem_u32(here), rank))
+               : "memory");
+  return v;
 }
 // barrier of the warps that compute
 template <int kThreads>
@@ -425,6 +436,11 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
     if (!ok && lane == 0) {
       atomicExch(p.status, 1);
       for (int i = 0; i < 64; ++i) __nanosleep(2000);  // loads in flight land before the CTA retires
+    }
+    if (p.cluster > 1) {  // the barriers of the join below
+      __syncwarp();
+      cluster_sync_all();
+      cluster_sync_all();
     }
     return;
   }
@@ -640,6 +656,21 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
         compute_sync<Cfg::kWarps * 32>();
       }
     }
+    if (p.cluster > 1) {
+      // this CTA's part of every row, for the CTA of the cluster that finishes it
+      if (key_warp == 0) {
+        float* part_o = reinterpret_cast<float*>(smem + Cfg::kOffJoin) + (row_warp * 16 + quad) * D + 2 * in_quad;
+        float2* part_ml = reinterpret_cast<float2*>(smem + Cfg::kOffMl) + row_warp * 16 + quad;
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+#pragma unroll
+          for (int n = 0; n < D / 8; ++n)
+            *reinterpret_cast<float2*>(part_o + 8 * r * D + 8 * n) = make_float2(o[n][2 * r], o[n][2 * r + 1]);
+          if (in_quad == 0) part_ml[8 * r] = make_float2(m[r], l[r]);
+        }
+      }
+      break;  // a cluster has one item
+    }
     if (key_warp == 0) {
       const bool whole = t0 == 0 && t1 == walk.tiles;
       const long long part =
@@ -665,6 +696,47 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
         }
       }
     }
+  }
+  if (p.cluster > 1) {
+    // CTA `rank` finishes the rows rank, rank + cluster, ...: a warp a row, the parts in the order of their keys
+    cluster_sync_all();
+    constexpr int kOwn = D / 32;  // elements of a lane
+    const int rank = blockIdx.x % p.cluster;
+    for (int tile_row = rank + p.cluster * warp; tile_row < Cfg::kRows; tile_row += p.cluster * Cfg::kWarps) {
+      const int r = row_tile * Cfg::kRows + tile_row;
+      if (r >= rows) break;
+      const int t = r / p.group, head = kv_head * p.group + r % p.group;
+      const bool real = t < walk.count;
+      float2 ml = make_float2(-INFINITY, 0.f);
+      if (lane < p.cluster) ml = dsmem_ld2(smem + Cfg::kOffMl + tile_row * 8, lane);
+      float top = ml.x;
+#pragma unroll
+      for (int i = 4; i > 0; i >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, i));
+      const float off = top == -INFINITY ? 0.f : top, scale = ex2_approx(ml.x - off);
+      float sum = 0.f, out[kOwn];
+#pragma unroll
+      for (int i = 0; i < kOwn; ++i) out[i] = 0.f;
+#pragma unroll 8
+      for (int c = 0; c < p.cluster; ++c) {
+        const float s = __shfl_sync(0xffffffffu, scale, c);
+        sum = fmaf(__shfl_sync(0xffffffffu, ml.y, c), s, sum);
+#pragma unroll
+        for (int i = 0; i < kOwn; i += 2) {
+          const float2 x = dsmem_ld2(smem + Cfg::kOffJoin + (tile_row * D + lane * kOwn + i) * 4, c);
+          out[i] = fmaf(x.x, s, out[i]);
+          out[i + 1] = fmaf(x.y, s, out[i + 1]);
+        }
+      }
+      top = __shfl_sync(0xffffffffu, top, 0);  // (lanes from the eighth on have seen no part)
+      const long long row = (static_cast<long long>(walk.b) * p.q_heads + head) * p.cache.tokens + t;
+      const float inv = real && sum != 0.f ? 1.f / sum : 0.f;
+      T* to = static_cast<T*>(p.o) + row * D + lane * kOwn;
+#pragma unroll
+      for (int i = 0; i < kOwn; i += 2)
+        *reinterpret_cast<uint32_t*>(to + i) = real ? from_floats<T>(out[i] * inv, out[i + 1] * inv) : 0u;
+      if (p.lse && lane == 0) p.lse[row] = real ? (top + log2f(sum)) * 0.6931471805599453f : -INFINITY;
+    }
+    cluster_sync_all();  // the others may still read here
   }
   if (!ok && lane == 0) atomicExch(p.status, 1);
 }

@@ -47,6 +47,10 @@ def check_decode(pkg, batch, q, dtype_eps=None, counts=False, **kw):
     (7, 1, 3, 32, [3, 4, 200]),                      # several tokens, sequences that hold nothing else
     (16, 4, 8, 256, [600, 8]),
     (1, 1, 1, 16, [4100]),                           # cut among many CTAs
+    (4, 4, 1, 16, [700, 0, 1, 130]),                 # clusters of CTAs with and without tiles
+    (36, 4, 2, 64, [1000, 64]),                      # clusters, 18 rows
+    (64, 2, 2, 64, [900]),                           # clusters, 64 rows
+    (4, 2, 1, 16, [31 * i % 129 for i in range(90)]),  # a CTA for each of many short sequences
 ])
 def test_decode(pkg, dtype, head_dim, q_heads, kv_heads, tokens, page, lengths):
     b = oracle.Batch(len(lengths) + head_dim, lengths, [min(tokens, n) for n in lengths], tokens, kv_heads, head_dim, page,

@@ -239,7 +239,7 @@ int flash_decode(const fa_paged_cache* cache, const fa_rows* q, void* o, float* 
     longest = static_cast<long long>(window_left) + tokens;
   const long long tiles = (longest + tile_keys - 1) / tile_keys + (window_left >= 0);
   const long long items = static_cast<long long>(batch) * cache->kv_heads * p.row_tiles;
-  if (static_cast<double>(items) * (tiles + 1) > 0x7fffffff - 512)
+  if (static_cast<double>(items) * (tiles + 2) > 0x7fffffff - 512)
     return fail(FA_INVALID_ARG, "more tiles of keys than 31 bits count");
   p.cluster = decode_cluster(tiles, items, p.ctas);
   p.part_o = static_cast<float*>(workspace);

@@ -190,7 +190,7 @@ struct DecodeParams {
 };
 
 // The work is one line of tiles of 64 keys: sequence by sequence, in each key head by key head (and row tile by row
-// tile), the tiles that the new tokens see. Every CTA takes an equal stretch of the line. A (sequence, key head, row tile)
+// tile), the tiles that the new tokens see. Every CTA takes an equal stretch of the line, to within a tile. A (sequence, key head, row tile)
 // that lies within one stretch is finished there; one that is cut has its parts written as (maximum, sum, unnormalised
 // output) and joined by decode_join_kernel in the order of the line, so the results depend on the lengths alone. Where few
 // items are short, or many are very short, an item has a cluster of CTAs, or one CTA, to itself instead, and no second launch.
@@ -201,14 +201,17 @@ struct DecodeLine {
     first = lo >> p.tile_shift;
     tiles = count > 0 ? ((length - 1) >> p.tile_shift) + 1 - first : 0;
   }
-  // Sums the tiles of one key head over all sequences and over those in front of `upto`. All lanes of a warp call it.
+  // What an item takes up on the line: a tile for its beginning and end (Q, the join of the warps and the output take a CTA about
+  // as long as a tile does), then its tiles.
+  __device__ static int units_of(int tiles) { return tiles > 0 ? tiles + 1 : 0; }
+  // Sums the units of an item of every sequence, and of those in front of `upto`. All lanes of a warp call it.
   __device__ static void sum(const DecodeParams& p, int upto, int& all, int& before, int lane) {
     all = before = 0;
     for (int b = lane; b < p.cache.batch; b += 32) {
       int first, tiles, length, count;
       tiles_of(p, b, first, tiles, length, count);
-      all += tiles;
-      if (b < upto) before += tiles;
+      all += units_of(tiles);
+      if (b < upto) before += units_of(tiles);
     }
 #pragma unroll
     for (int s = 16; s > 0; s >>= 1) {
@@ -216,42 +219,53 @@ struct DecodeLine {
       before += __shfl_xor_sync(0xffffffffu, before, s);
     }
   }
-  __device__ static int share_of(const DecodeParams& p, int all) {
-    return static_cast<int>((static_cast<unsigned>(all) * p.cache.kv_heads * p.row_tiles + p.ctas - 1) / p.ctas);
+
+  // CTA c has the units [start(c), start(c + 1)).
+  int base, more;  // units of a CTA; CTAs that have one more
+  __device__ DecodeLine(const DecodeParams& p, int all) {
+    const int total = all * p.cache.kv_heads * p.row_tiles;
+    base = total / p.ctas;
+    more = total - base * p.ctas;
+  }
+  __device__ int start(int c) const { return c * base + min(c, more); }
+  __device__ int cta_of(int unit) const {
+    const int in_more = more * (base + 1);
+    return unit < in_more ? unit / (base + 1) : more + (unit - in_more) / base;
   }
 };
 
 // A stretch of the line, walked item by item; every role of a CTA walks it for itself.
 struct DecodeWalk {
-  int at, begin, end;  // of the line
-  int b_start;         // where sequence b starts
+  int at, end;  // of the line
+  int b_start;  // where sequence b starts
   int b, first, tiles, length, count;
 
   __device__ void start(const DecodeParams& p, int cta, int lane) {
     if (p.cluster > 0) {  // one item: `at` and `end` count items
       b = cta / (p.cluster * p.cache.kv_heads * p.row_tiles);
       DecodeLine::tiles_of(p, b, first, tiles, length, count);
-      at = begin = 0;
+      at = 0;
       end = 1;
       return;
     }
-    int all, before;
-    DecodeLine::sum(p, 0, all, before, lane);
-    const int share = DecodeLine::share_of(p, all), total = all * p.cache.kv_heads * p.row_tiles;
-    at = begin = min(cta * share, total);  // (ctas * share exceeds the total by less than ctas)
-    end = min(at + share, total);
-    b = 0;
-    b_start = 0;
-    // the sequence that holds `at`, 32 at a time
     const int per = p.cache.kv_heads * p.row_tiles;
-    for (int b0 = 0; at < end; b0 += 32) {
+    b = b_start = at = end = 0;
+    // the sequence that holds the start, 32 at a time
+    for (int b0 = 0; b0 < p.cache.batch; b0 += 32) {
       int f = 0, n = 0, len = 0, cnt = 0;
       if (b0 + lane < p.cache.batch) DecodeLine::tiles_of(p, b0 + lane, f, n, len, cnt);
-      int upto = n;
+      int upto = DecodeLine::units_of(n);
 #pragma unroll
       for (int s = 1; s < 32; s <<= 1) {
         const int v = __shfl_up_sync(0xffffffffu, upto, s);
         if (lane >= s) upto += v;
+      }
+      if (b0 == 0) {
+        int all = __shfl_sync(0xffffffffu, upto, 31), before;
+        if (p.cache.batch > 32) DecodeLine::sum(p, 0, all, before, lane);
+        const DecodeLine line(p, all);
+        at = line.start(cta);
+        end = line.start(cta + 1);
       }
       upto = b_start + upto * per;
       const unsigned found = __ballot_sync(0xffffffffu, upto > at);
@@ -262,16 +276,17 @@ struct DecodeWalk {
         tiles = __shfl_sync(0xffffffffu, n, src);
         length = __shfl_sync(0xffffffffu, len, src);
         count = __shfl_sync(0xffffffffu, cnt, src);
-        b_start = __shfl_sync(0xffffffffu, upto, src) - tiles * per;
+        b_start = __shfl_sync(0xffffffffu, upto, src) - DecodeLine::units_of(tiles) * per;
         return;
       }
       b_start = __shfl_sync(0xffffffffu, upto, 31);
     }
+    at = end;  // (nothing is left for this CTA)
   }
-  // The item at `at`: key head, row tile, and its tiles [t0, t1) of [0, tiles). Moves on behind them.
+  // The next item of which the stretch holds tiles: key head, row tile, and its tiles [t0, t1) of [0, tiles).
   __device__ bool next(const DecodeParams& p, int& kv_head, int& row_tile, int& t0, int& t1) {
-    if (at >= end) return false;
     if (p.cluster > 0) {
+      if (at >= end) return false;
       const int item = blockIdx.x / p.cluster % (p.cache.kv_heads * p.row_tiles);
       kv_head = item / p.row_tiles;
       row_tile = item % p.row_tiles;
@@ -282,18 +297,22 @@ struct DecodeWalk {
       return true;
     }
     const int per = p.cache.kv_heads * p.row_tiles;
-    while (at >= b_start + tiles * per) {
-      b_start += tiles * per;
-      ++b;
-      DecodeLine::tiles_of(p, b, first, tiles, length, count);
+    while (at < end) {
+      while (at >= b_start + DecodeLine::units_of(tiles) * per) {
+        b_start += DecodeLine::units_of(tiles) * per;
+        ++b;
+        DecodeLine::tiles_of(p, b, first, tiles, length, count);
+      }
+      const int units = DecodeLine::units_of(tiles), item = (at - b_start) / units, from = at - b_start - item * units;
+      const int to = min(from + end - at, units);
+      at += to - from;
+      t0 = max(from - 1, 0);
+      t1 = to - 1;
+      kv_head = item / p.row_tiles;
+      row_tile = item % p.row_tiles;
+      if (t1 > t0) return true;
     }
-    const int item = (at - b_start) / tiles;
-    kv_head = item / p.row_tiles;
-    row_tile = item % p.row_tiles;
-    t0 = at - b_start - item * tiles;
-    t1 = min(t0 + end - at, tiles);
-    at += t1 - t0;
-    return true;
+    return false;
   }
 };
 
@@ -674,7 +693,7 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
     if (key_warp == 0) {
       const bool whole = t0 == 0 && t1 == walk.tiles;
       const long long part =
-          (2ll * blockIdx.x + (walk.at - (t1 - t0) == walk.begin ? 0 : 1)) * Cfg::kRows + row_warp * 16 + quad;
+          (2ll * blockIdx.x + (t0 == 0 ? 1 : 0)) * Cfg::kRows + row_warp * 16 + quad;  // of the first part, or a later one
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         if (out_row[r] < 0) continue;
@@ -758,22 +777,20 @@ __global__ void __launch_bounds__(128, 6) decode_join_kernel(const __grid_consta
   int first, tiles, length, count;
   DecodeLine::tiles_of(p, b, first, tiles, length, count);
   const bool real = tiles > 0 && t < count;
-  int c0 = 0, c1 = -1, start = 0, share = 1;
+  int c0 = 0, c1 = -1;  // the CTAs of the row's item
   const int r = t * p.group + head % p.group;
   if (real) {
     int all, before;
     DecodeLine::sum(p, b, all, before, lane);
     const int item = head / p.group * p.row_tiles + r / tile_rows;
-    share = DecodeLine::share_of(p, all);
-    start = before * p.cache.kv_heads * p.row_tiles + item * tiles;
-    c0 = start / share;
-    c1 = (start + tiles - 1) / share;
+    const DecodeLine line(p, all);
+    const int from = before * p.cache.kv_heads * p.row_tiles + item * DecodeLine::units_of(tiles) + 1;
+    c0 = line.cta_of(from);
+    c1 = line.cta_of(from + tiles - 1);
   }
   griddep_wait();
   if (real && c0 == c1) return;
-  auto part = [&](int c) {
-    return (2ll * c + (c == c0 && start != c * share ? 1 : 0)) * tile_rows + r % tile_rows;
-  };
+  auto part = [&](int c) { return (2ll * c + (c == c0 ? 1 : 0)) * tile_rows + r % tile_rows; };
   float o[kOwn], m = -INFINITY, l = 0.f;
 #pragma unroll
   for (int i = 0; i < kOwn; ++i) o[i] = 0.f;

@@ -14,7 +14,7 @@ size_t align256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
 template <int D, bool kAlibi>
 int launch(const CUtensorMap (&maps)[4], const fa::BwdParams& p, int num_sms, cudaStream_t st, bool early) {
   using Cfg = fa::BwdCfg<D>;
-  cudaError_t e = launch_early(fa::bwd_rows_kernel<D>, dim3(p.tiles, p.bh), 256, 0, st, early, p);
+  cudaError_t e = launch_early(fa::bwd_rows_kernel<D>, dim3(p.tiles, p.bh), 1024, 0, st, early, p);
   if (e != cudaSuccess) return fail_cuda("launch bwd_rows_kernel", e);
   constexpr auto kernel = fa::bwd_kernel<D, kAlibi>;
   e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes);

@@ -27,6 +27,7 @@ struct BwdParams {
   __half *dq, *dk, *dv;
   int seqlen, bh, heads, tiles;  // tiles: ceil(seqlen / 128)
   int head_group;                // heads whose work items are interleaved
+  int kinds_apart;               // in such a group all items of dK and dV come first, not those of one rank
   float scale, scale_log2;
   int causal, window_left, window_right;
   const float* alibi_slopes;
@@ -132,10 +133,21 @@ __device__ __forceinline__ BwdItem bwd_item(const BwdParams& p, int index) {
   const int per_group = 2 * p.tiles * p.head_group;
   const int first_head = index / per_group * p.head_group;
   const int heads = min(p.head_group, p.bh - first_head);
-  const int in = index % per_group, rank = in / (2 * heads), rest = in % (2 * heads);
+  const int in = index % per_group;
+  int rank, head;
   BwdItem it;
-  it.is_dq = rest >= heads;
-  it.bh = first_head + rest % heads;
+  if (p.kinds_apart) {
+    const int of_kind = in % (p.tiles * heads);
+    it.is_dq = in >= p.tiles * heads;
+    rank = of_kind / heads;
+    head = of_kind % heads;
+  } else {
+    const int of_rank = in % (2 * heads);
+    it.is_dq = of_rank >= heads;
+    rank = in / (2 * heads);
+    head = of_rank % heads;
+  }
+  it.bh = first_head + head;
   const int wr = eff_window_right(p.causal, p.window_right);
   it.left = it.is_dq ? p.window_left : wr;
   it.right = it.is_dq ? wr : p.window_left;

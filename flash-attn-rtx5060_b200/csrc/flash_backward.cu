@@ -85,6 +85,12 @@ int backward(const void* q, const void* k, const void* v, const void* o, const v
   const long long group = (64ll << 20) / (4ll * seqlen * head_dim * 2);
   p.head_group = static_cast<int>(group < 1 ? 1 : group > bh ? bh : group);
 
+  // Items come in falling order of their time. A mask that bounds one side only makes them unequal, so there the order is by
+  // rank; else they differ by their kind: dK and dV take a fifth longer than dQ. us, by rank -> kinds apart: 8 heads x 2048 d64,
+  // 256 items on 148 CTAs 46.9 -> 41.4, 37 x 4096 d128 866 -> 835; but causal 8 x 2048 d128 35.8 -> 41.9.
+  const bool left = p.window_left >= 0, right = p.causal || p.window_right >= 0;
+  p.kinds_apart = left == right;
+
   CUtensorMap maps[4];
   const void* tensors[4] = {q, k, v, d_o};
   for (int i = 0; i < 4; ++i)

@@ -5,7 +5,7 @@
 //   dQ_i  = scale * sum_j dS_ij k_j,   dK_j = scale * sum_i dS_ij q_i,   dV_j = sum_i P_ij dO_i
 //
 // bwd_rows_kernel computes delta and the norms that the scaling of dS needs; bwd_kernel has a work item for every 128 rows
-// of dQ and one for every 128 rows of dK and dV. Both kinds take the probabilities again (seven products a tile pair where
+// of dQ and one for every 128 rows of dK and dV (few short heads: one launch, bwd_own_rows). Both kinds take the probabilities again (seven products a tile pair where
 // one pass that also adds dQ up in global memory would have five), so that every sum stays in tensor memory, in one order:
 // no atomics, no fp32 copy of dQ in HBM, the same bits every time.
 //
@@ -19,7 +19,7 @@
 namespace fa {
 
 struct BwdParams {
-  const __half *o, *d_o, *v;  // bwd_rows_kernel
+  const __half *o, *d_o, *v;  // for delta and the norms
   const float* lse;           // [bh][seqlen]
   const float* d_lse;         // the same, or nullptr
   float* delta;               // [bh][seqlen]
@@ -35,11 +35,46 @@ struct BwdParams {
   int withhold;  // test build only: work item 0 leaves out a tile, so that a wait runs out
 };
 
-// 128 rows of a head a CTA, D / 8 lanes a row. Reads O, dO and V once: bound by bytes where rows are many (B1 H16 N8192 d128:
-// 101 MB in 21 us under ncu, caches flushed), else by one round of loads and two reductions.
+// delta of row r of a head, and |dO_r|^2 and |v_r|^2: D / 8 lanes a row, all of which get the sums. All lanes of a warp.
+template <int D>
+__device__ __forceinline__ void bwd_row(const BwdParams& p, size_t head, int r, int lane, float& delta, float& gg, float& vv) {
+  constexpr int kLanes = D / 8;
+  delta = gg = vv = 0.f;
+  if (r < p.seqlen) {
+    const size_t at = (head * p.seqlen + r) * D + (lane % kLanes) * 8;
+    const uint4 a = *reinterpret_cast<const uint4*>(p.o + at), g = *reinterpret_cast<const uint4*>(p.d_o + at),
+                v = *reinterpret_cast<const uint4*>(p.v + at);
+    const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, gw[4] = {g.x, g.y, g.z, g.w}, vw[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float2 x = __half22float2(*reinterpret_cast<const __half2*>(aw + k));
+      const float2 y = __half22float2(*reinterpret_cast<const __half2*>(gw + k));
+      const float2 z = __half22float2(*reinterpret_cast<const __half2*>(vw + k));
+      delta = fmaf(x.x, y.x, fmaf(x.y, y.y, delta));
+      gg = fmaf(y.x, y.x, fmaf(y.y, y.y, gg));
+      vv = fmaf(z.x, z.x, fmaf(z.y, z.y, vv));
+    }
+  }
+#pragma unroll
+  for (int s = kLanes / 2; s > 0; s >>= 1) {
+    delta += __shfl_xor_sync(0xffffffffu, delta, s);
+    gg += __shfl_xor_sync(0xffffffffu, gg, s);
+    vv += __shfl_xor_sync(0xffffffffu, vv, s);
+  }
+  if (p.d_lse && r < p.seqlen) delta -= p.d_lse[head * p.seqlen + r];
+}
+
+__device__ __forceinline__ float warp_max(float x) {
+#pragma unroll
+  for (int s = 16; s > 0; s >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, s));
+  return x;
+}
+
+// 128 rows of a head a CTA. Reads O, dO and V once: bound by bytes where rows are many (B1 H16 N8192 d128: 101 MB in 21 us under
+// ncu, caches flushed), else by one round of loads and two reductions.
 template <int D>
 __global__ void __launch_bounds__(1024) bwd_rows_kernel(const BwdParams p) {
-  constexpr int kLanes = D / 8, kRows = 32 / kLanes;  // of a warp at a time
+  constexpr int kRows = 32 / (D / 8);  // of a warp at a time
   __shared__ float s_max[32][3];
   griddep_wait();
   griddep_launch();
@@ -48,48 +83,22 @@ __global__ void __launch_bounds__(1024) bwd_rows_kernel(const BwdParams p) {
   float top[3] = {0.f, 0.f, 0.f};
 #pragma unroll
   for (int i = 0; i < 4 / kRows; ++i) {
-    const int r = blockIdx.x * 128 + warp * 4 + i * kRows + lane / kLanes;
-    float dot = 0.f, gg = 0.f, vv = 0.f;
-    if (r < p.seqlen) {
-      const size_t at = (head * p.seqlen + r) * D + (lane % kLanes) * 8;
-      const uint4 a = *reinterpret_cast<const uint4*>(p.o + at), g = *reinterpret_cast<const uint4*>(p.d_o + at),
-                  v = *reinterpret_cast<const uint4*>(p.v + at);
-      const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, gw[4] = {g.x, g.y, g.z, g.w}, vw[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float2 x = __half22float2(*reinterpret_cast<const __half2*>(aw + k));
-        const float2 y = __half22float2(*reinterpret_cast<const __half2*>(gw + k));
-        const float2 z = __half22float2(*reinterpret_cast<const __half2*>(vw + k));
-        dot = fmaf(x.x, y.x, fmaf(x.y, y.y, dot));
-        gg = fmaf(y.x, y.x, fmaf(y.y, y.y, gg));
-        vv = fmaf(z.x, z.x, fmaf(z.y, z.y, vv));
-      }
-    }
-#pragma unroll
-    for (int s = kLanes / 2; s > 0; s >>= 1) {
-      dot += __shfl_xor_sync(0xffffffffu, dot, s);
-      gg += __shfl_xor_sync(0xffffffffu, gg, s);
-      vv += __shfl_xor_sync(0xffffffffu, vv, s);
-    }
-    if (r < p.seqlen) {
-      if (p.d_lse) dot -= p.d_lse[head * p.seqlen + r];
-      if (lane % kLanes == 0) p.delta[head * p.seqlen + r] = dot;
-      top[0] = fmaxf(top[0], gg);
-      top[1] = fmaxf(top[1], vv);
-      top[2] = fmaxf(top[2], fabsf(dot));
-    }
+    const int r = blockIdx.x * 128 + warp * 4 + i * kRows + lane / (D / 8);
+    float delta, gg, vv;
+    bwd_row<D>(p, head, r, lane, delta, gg, vv);
+    if (r < p.seqlen && lane % (D / 8) == 0) p.delta[head * p.seqlen + r] = delta;
+    top[0] = fmaxf(top[0], gg);
+    top[1] = fmaxf(top[1], vv);
+    top[2] = fmaxf(top[2], fabsf(delta));
   }
 #pragma unroll
-  for (int k = 0; k < 3; ++k)
-#pragma unroll
-    for (int s = 16; s > 0; s >>= 1) top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], s));
-  if (lane == 0)
-    for (int k = 0; k < 3; ++k) s_max[warp][k] = top[k];
+  for (int k = 0; k < 3; ++k) {
+    const float m = warp_max(top[k]);
+    if (lane == 0) s_max[warp][k] = m;
+  }
   __syncthreads();
   if (warp < 3) {  // warp k: the largest of norm k
-    float m = s_max[lane][warp];
-#pragma unroll
-    for (int k = 16; k > 0; k >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
+    const float m = warp_max(s_max[lane][warp]);
     if (lane == 0) p.norms[(head * p.tiles + blockIdx.x) * 3 + warp] = warp < 2 ? sqrtf(m) : m;
   }
 }
@@ -109,6 +118,13 @@ struct BwdCfg {
   static constexpr int kOffBars = kOffStats + kStats * 1024;
   static constexpr int kNumBars = 2 * (kFirst + kSecond + kStats) + 10;
   static constexpr int kSmemBytes = kOffBars + kNumBars * 8 + 16;
+  // kOwnRows: delta of all rows, 16 warps' three norms and a barrier. At head_dim 128, where there is no other room, they lie in
+  // the first ring's third slot, which the single tile of 128 rows does not reach.
+  static constexpr int kMaxOwnRows = 16384 / D;
+  static constexpr int kOffOwnRows = D == 128 ? kOffFirst + 2 * kTileBytes : (kSmemBytes + 15) / 16 * 16;
+  static constexpr int kOwnRowsBytes = kMaxOwnRows * 4 + 16 * 3 * 4 + 8;
+  static constexpr int kSmemBytesOwnRows = D == 128 ? kSmemBytes : kOffOwnRows + kOwnRowsBytes;
+  static_assert(D == 64 || kFirst * 128 > kMaxOwnRows);
   static constexpr uint32_t kTmemCols = 512;
   // Tensor memory: score regions of 128 columns, in which the fp16 operands of the second products take the place of the
   // scores that they are made of (32 columns' operand in the first 16 of the 32), and the accumulators. S has two regions for
@@ -157,22 +173,11 @@ __device__ __forceinline__ BwdItem bwd_item(const BwdParams& p, int index) {
   return it;
 }
 
-// 2^-e: see the top of this file. A bound that is zero, infinite or NaN leaves dS as it is. All lanes of a warp.
-__device__ __forceinline__ float bwd_unit(const BwdParams& p, int bh, int lane) {
-  float g = 0.f, v = 0.f, d = 0.f;
-  for (int t = lane; t < p.tiles; t += 32) {
-    const float* n = p.norms + (static_cast<size_t>(bh) * p.tiles + t) * 3;
-    g = fmaxf(g, n[0]);
-    v = fmaxf(v, n[1]);
-    d = fmaxf(d, n[2]);
-  }
-#pragma unroll
-  for (int s = 16; s > 0; s >>= 1) {
-    g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, s));
-    v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, s));
-    d = fmaxf(d, __shfl_xor_sync(0xffffffffu, d, s));
-  }
-  const int exponent = static_cast<int>(__float_as_uint(fmaf(g, v, d)) >> 23 & 255u);  // of the bound, biased by 127
+// 2^-e (see the top of this file) from a lane's norms. A bound that is zero, infinite or NaN leaves dS as it is. All lanes of a
+// warp.
+__device__ __forceinline__ float bwd_unit(float g, float v, float d) {
+  const float bound = fmaf(warp_max(g), warp_max(v), warp_max(d));
+  const int exponent = static_cast<int>(__float_as_uint(bound) >> 23 & 255u);  // biased by 127
   if (exponent == 0 || exponent == 255) return 1.f;
   return __uint_as_float(static_cast<uint32_t>(min(max(127 - (exponent - 126), 27), 227)) << 23);
 }
@@ -529,13 +534,42 @@ __device__ __forceinline__ bool bwd_load(const CUtensorMap& map_q, const CUtenso
   return true;
 }
 
-// The warp that brings the statistics: for dK and dV those of every column tile, for dQ those of the item's own rows.
+// What bwd_rows_kernel computes, by the softmax warps of a CTA for all rows of its one item's head.
 template <int D>
+__device__ __forceinline__ void bwd_own_rows(const BwdParams& p, int bh, uint8_t* smem, int warp, int lane) {
+  using Cfg = BwdCfg<D>;
+  constexpr int kRows = 32 / (D / 8);  // of a warp at a time
+  float* delta_of = reinterpret_cast<float*>(smem + Cfg::kOffOwnRows);
+  float* norms = delta_of + Cfg::kMaxOwnRows;
+  float top[3] = {0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int r0 = warp * kRows; r0 < p.seqlen; r0 += 16 * kRows) {
+    const int r = r0 + lane / (D / 8);
+    float delta, gg, vv;
+    bwd_row<D>(p, bh, r, lane, delta, gg, vv);
+    if (r < p.seqlen && lane % (D / 8) == 0) delta_of[r] = delta;
+    top[0] = fmaxf(top[0], gg);
+    top[1] = fmaxf(top[1], vv);
+    top[2] = fmaxf(top[2], fabsf(delta));
+  }
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    const float m = warp_max(top[k]);
+    if (lane == 0) norms[warp * 3 + k] = k < 2 ? sqrtf(m) : m;
+  }
+  __syncwarp();
+  mbar_arrive_lane0(reinterpret_cast<uint64_t*>(norms + 48), lane);
+}
+
+// The warp that brings the statistics: for dK and dV those of every column tile, for dQ those of the item's own rows.
+template <int D, bool kOwnRows>
 __device__ __forceinline__ void bwd_stats(const BwdParams& p, const BwdBars& b, uint8_t* smem, int lane) {
   using Cfg = BwdCfg<D>;
   Turn<Cfg::kStats> at;
   at.parity = 1;
   griddep_wait();
+  const float* delta_here = reinterpret_cast<const float*>(smem + Cfg::kOffOwnRows);
+  const float* norms_here = delta_here + Cfg::kMaxOwnRows;
   for (int k = 0, index; (index = bwd_index(k)) < 2 * p.tiles * p.bh; ++k) {
     const BwdItem it = bwd_item(p, index);
     const int c0 = it.is_dq ? it.r0 : it.begin * 128;
@@ -546,15 +580,27 @@ __device__ __forceinline__ void bwd_stats(const BwdParams& p, const BwdBars& b, 
         const int c = c0 + i * 128 + j * 32 + lane;
         const size_t from = static_cast<size_t>(it.bh) * p.seqlen + c;
         nl[j] = c < p.seqlen ? fmaf(p.lse[from], -1.4426950408889634f, 14.f) : -INFINITY;
-        nd[j] = c < p.seqlen ? -p.delta[from] : 0.f;
+        if (!kOwnRows) nd[j] = c < p.seqlen ? -p.delta[from] : 0.f;
       }
     };
     load(0);  // (on its way while the norms are read)
-    const float unit = bwd_unit(p, it.bh, lane);
+    float norm[3] = {0.f, 0.f, 0.f};
+    if (kOwnRows) {
+      if (!mbar_wait_warp(reinterpret_cast<uint64_t*>(const_cast<float*>(norms_here + 48)), 0, b.abort_flag)) return;
+      for (int j = 0; j < 3; ++j) norm[j] = lane < 16 ? norms_here[lane * 3 + j] : 0.f;
+    } else {
+      for (int t = lane; t < p.tiles; t += 32)
+        for (int j = 0; j < 3; ++j) norm[j] = fmaxf(norm[j], p.norms[(static_cast<size_t>(it.bh) * p.tiles + t) * 3 + j]);
+    }
+    const float unit = bwd_unit(norm[0], norm[1], norm[2]);
     for (int i = 0; i < (it.is_dq ? 1 : it.tiles); ++i) {
       if (i > 0) load(i);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) nd[j] *= unit;
+      for (int j = 0; j < 4; ++j) {
+        const int c = c0 + i * 128 + j * 32 + lane;
+        if (kOwnRows) nd[j] = c < p.seqlen ? -delta_here[c] : 0.f;
+        nd[j] *= unit;
+      }
       if (!mbar_wait_warp(b.stats_empty + at.slot, at.parity, b.abort_flag)) return;
       float* to = reinterpret_cast<float*>(smem + Cfg::kOffStats + at.slot * 1024);
 #pragma unroll
@@ -573,9 +619,11 @@ __device__ __forceinline__ void bwd_stats(const BwdParams& p, const BwdBars& b, 
 // One CTA a SM walks the work items bwd_index(0), bwd_index(1), ... (a CTA an item, started by the hardware, took 7 us an item
 // for its start and end: window 1024 2576 -> 2153 us with all that came with it). Bound by the tensor pipe at head_dim 128: 4890
 // clocks a pair of tiles for 3584 of products, 73 % busy at 1.4-1.5 GHz under the power cap; B2 H32 N8192 causal 3370-3660 us,
-// 750-815 TFLOP/s of the five products that the gradient has; B2 H16 N4096 d64 causal 280-365 us. 20 warps: 0-15 softmax and epilogue, 16 issues
-// the products, 17 loads tiles, 18 brings the statistics, 19 only donates registers.
-template <int D, bool kAlibi>
+// 750-815 TFLOP/s of the five products that the gradient has; B2 H16 N4096 d64 causal 280-365 us. 20 warps: 0-15 softmax and
+// epilogue, 16 issues the products, 17 loads tiles, 18 brings the statistics, 19 only donates registers.
+// kOwnRows: short heads, an item a CTA, no bwd_rows_kernel: the softmax warps, idle until the first products, do its work for
+// their CTA, each CTA for all rows of its head.
+template <int D, bool kAlibi, bool kOwnRows>
 __global__ void __launch_bounds__(640, 1)
 bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
            const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do,
@@ -610,13 +658,17 @@ bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
   static_assert(Cfg::kNumBars <= 64);
   if (warp == 0) {  // (a thread for one barrier or two: one after the other they cost a short call 0.2 us)
     for (int i = lane; i < Cfg::kNumBars; i += 32) mbar_init(bars + i, bars + i >= b.stats_empty ? Cfg::kSoftmaxWarps : 1);
-    if (lane == 0) *b.abort_flag = 0;
+    if (lane == 0) {
+      *b.abort_flag = 0;
+      if (kOwnRows) mbar_init(reinterpret_cast<uint64_t*>(smem + Cfg::kOffOwnRows + Cfg::kOwnRowsBytes - 8), Cfg::kSoftmaxWarps);
+    }
     fence_mbar_init();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  if (kOwnRows) griddep_wait();
   // bwd_rows_kernel lets this kernel in only behind its own griddep_wait(): whatever came before the two of them is complete,
   // and only the warp that reads what bwd_rows_kernel writes has to wait for it. (Every CTA has one, so whoever waits for this
   // kernel has waited for both.)
@@ -624,6 +676,7 @@ bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
 
   if (warp < Cfg::kSoftmaxWarps) {
     reg_inc<Cfg::kRegSoftmax>();
+    if (kOwnRows) bwd_own_rows<D>(p, bwd_item(p, blockIdx.x).bh, smem, warp, lane);
     SoftmaxTurns<D> at;
     bool ok = true;
     for (int k = 0, index; (index = bwd_index(k)) < 2 * p.tiles * p.bh && ok; ++k) {
@@ -641,7 +694,7 @@ bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
         for (int i = 0; i < 64; ++i) __nanosleep(2000);
       __syncwarp();
     } else if (warp == 18) {
-      bwd_stats<D>(p, b, smem, lane);
+      bwd_stats<D, kOwnRows>(p, b, smem, lane);
     }
   }
 

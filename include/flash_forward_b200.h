@@ -122,8 +122,8 @@ int flash_forward_dropout(const void* q, const void* k, const void* v, void* o, 
  * gradients cost precision; all sums are fp32. dK, dV and dQ are summed in one order: two calls with the same arguments give
  * the same bits.
  * workspace: flash_backward_workspace_bytes() bytes of device memory, 256-byte aligned, with any contents; calls that may
- * overlap on the GPU need one each. Asynchronous on `stream`, two launches; may be captured into a CUDA graph once a call of
- * this library has been made on the device. batch*heads up to 65535. flash_forward_check() reports a wait that ran out. */
+ * overlap on the GPU need one each. Asynchronous on `stream`, one launch or two; may be captured into a CUDA graph once a call
+ * of this library has been made on the device. batch*heads up to 65535. flash_forward_check() reports a wait that ran out. */
 int flash_backward(const void* q, const void* k, const void* v, const void* o, const void* d_o, const float* lse,
                    const float* d_lse, void* dq, void* dk, void* dv, int batch, int heads, int seqlen, int head_dim,
                    float softmax_scale, int is_causal, int window_left, int window_right, const float* alibi_slopes,
@@ -323,7 +323,7 @@ int flash_cache_append(const fa_paged_cache* cache, const fa_rows* k, const fa_r
  *   lse  NULL, or float [batch][q_heads][tokens]: the log-sum-exp as in flash_forward_lse()
  * Rows of padding, and of sequences without keys, are O = 0 and lse = -infinity.
  * workspace: flash_decode_workspace_bytes() bytes of device memory, 16-byte aligned, with any contents; calls that may
- * overlap on the GPU need one each. Asynchronous on `stream`, two launches; may be captured into a CUDA graph once a call
+ * overlap on the GPU need one each. Asynchronous on `stream`, one launch or two; may be captured into a CUDA graph once a call
  * has been made on the device. Two calls with the same arguments give the same bits; how a sequence's keys are shared out
  * depends on the lengths of the whole batch. */
 int flash_decode(const fa_paged_cache* cache, const fa_rows* q, void* o, float* lse, int batch, int tokens, int q_heads,

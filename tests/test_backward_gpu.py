@@ -159,6 +159,28 @@ def test_many_items_again_and_again(pkg, d):
     pkg.check(torch.cuda.current_stream().cuda_stream)
 
 
+@pytest.mark.parametrize("kw", [dict(causal=True), dict(window_left=30, window_right=50), dict(causal=True, alibi=True)])
+@pytest.mark.parametrize("N,d", [(1, 64), (128, 64), (200, 64), (256, 64), (257, 64), (3, 128), (100, 128), (128, 128), (129, 128)])
+def test_short_heads_alone_and_among_many(pkg, N, d, kw):
+    """A few short heads find their delta and norms in the kernel that uses them, many have a kernel for it: the same bits, and
+    for the few the formula's gradient, with one of the log-sum-exp."""
+    H = 5
+    kw = dict(kw)
+    if kw.pop("alibi", False):
+        kw["alibi_slopes"] = torch.tensor([0.5, 0.1, 1.0, 0.02, 0.0])
+    q, k, v, dout = tensors(40 + N + d, 31, H, N, d)
+    dout[::2] *= 2.0 ** -10
+    dlse = torch.randn((31, H, N), generator=torch.Generator().manual_seed(41))
+    check(pkg, *(x[:2] for x in (q, k, v, dout)), dlse=dlse[:2], **kw)
+    gq, gk, gv, gd, gl = (x.cuda() for x in (q, k, v, dout, dlse))
+    gkw = gpu_kwargs(kw)
+    out, lse = pkg.attention_forward(gq, gk, gv, return_lse=True, **gkw)
+    many = pkg.attention_backward(gq, gk, gv, out, lse, gd, dlse=gl, **gkw)
+    few = pkg.attention_backward(*(x[:2] for x in (gq, gk, gv, out, lse, gd)), dlse=gl[:2], **gkw)
+    for x, y in zip(many, few):
+        assert torch.equal(x[:2], y)
+
+
 def test_two_streams_and_capture(pkg):
     q, k, v, dout = (x.cuda() for x in tensors(13, 1, 4, 600, 64))
     out, lse = pkg.attention_forward(q, k, v, return_lse=True)
@@ -235,3 +257,25 @@ def test_wait_gives_up_and_the_device_stays_usable(pkg):
         assert L.flash_forward_check(stream) == pkg.FA_OK
         for x, y in zip(grads, want):
             assert torch.equal(x, y)
+
+
+def test_wait_gives_up_in_a_short_head(pkg):
+    """The same where delta and the norms are found by the kernel itself."""
+    L = load_waittest()
+    vp, i = ctypes.c_void_p, ctypes.c_int
+    L.flash_backward_test_withhold.argtypes = [vp] * 9 + [i] * 4 + [vp, ctypes.c_size_t, vp]
+    for d, N in ((64, 200), (128, 70)):
+        q, k, v, dout = (x.cuda() for x in tensors(31, 1, 2, N, d))
+        out, lse = pkg.attention_forward(q, k, v, return_lse=True)
+        want = pkg.attention_backward(q, k, v, out, lse, dout)
+        stream = torch.cuda.current_stream().cuda_stream
+        pkg.check(stream)
+        grads = [torch.zeros_like(q) for _ in range(3)]
+        nbytes = pkg.lib().flash_backward_workspace_bytes(1, 2, N)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device="cuda")
+        ptrs = [x.data_ptr() for x in (q, k, v, out, dout, lse, *grads)]
+        assert L.flash_backward_test_withhold(*ptrs, 1, 2, N, d, ws.data_ptr(), nbytes, stream) == pkg.FA_OK
+        assert L.flash_forward_check(stream) == pkg.FA_DEVICE_TIMEOUT
+        again = pkg.attention_backward(q, k, v, out, lse, dout)
+        pkg.check(stream)
+        assert all(torch.equal(x, y) for x, y in zip(again, want))

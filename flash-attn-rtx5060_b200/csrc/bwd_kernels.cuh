@@ -5,9 +5,9 @@
 //   dQ_i  = scale * sum_j dS_ij k_j,   dK_j = scale * sum_i dS_ij q_i,   dV_j = sum_i P_ij dO_i
 //
 // bwd_rows_kernel computes delta and the norms that the scaling of dS needs; bwd_kernel has a work item for every 128 rows
-// of dQ and one for every 128 rows of dK and dV (few short heads: one launch, bwd_own_rows). Both kinds take the probabilities again (seven products a tile pair where
-// one pass that also adds dQ up in global memory would have five), so that every sum stays in tensor memory, in one order:
-// no atomics, no fp32 copy of dQ in HBM, the same bits every time.
+// of dQ and one for every 128 rows of dK and dV (few short heads: one launch, bwd_own_rows). Both kinds take the
+// probabilities again (seven products a tile pair where one pass that also adds dQ up in global memory would have five), so
+// that every sum stays in tensor memory, in one order: no atomics, no fp32 copy of dQ in HBM, the same bits every time.
 //
 // The operands of the second products are fp16, and P and dS of a long row are far below 1: P is kept as 2^14 P, and dS as
 // 2^14 P * (dO.v - delta) / 2^e with 2^e above the head's bound max|dO_i| max|v_j| + max|delta_i|, so that neither overflows
@@ -117,7 +117,7 @@ struct BwdCfg {
   static constexpr int kOffStats = kOffSecond + kSecond * kTileBytes;  // per slot float[2][128]
   static constexpr int kOffBars = kOffStats + kStats * 1024;
   static constexpr int kNumBars = 2 * (kFirst + kSecond + kStats) + 10;
-  static constexpr int kSmemBytes = kOffBars + kNumBars * 8 + 16;
+  static constexpr int kSmemBytes = kOffBars + kNumBars * 8 + 24;
   // kOwnRows: delta of all rows, 16 warps' three norms and a barrier. At head_dim 128, where there is no other room, they lie in
   // the first ring's third slot, which the single tile of 128 rows does not reach.
   static constexpr int kMaxOwnRows = 16384 / D;
@@ -146,23 +146,18 @@ struct BwdItem {
 };
 
 __device__ __forceinline__ BwdItem bwd_item(const BwdParams& p, int index) {
-  const int per_group = 2 * p.tiles * p.head_group;
-  const int first_head = index / per_group * p.head_group;
-  const int heads = min(p.head_group, p.bh - first_head);
-  const int in = index % per_group;
-  int rank, head;
+  const unsigned per_group = 2 * p.tiles * p.head_group, group = static_cast<unsigned>(index) / per_group;
+  const int first_head = group * p.head_group;
+  const unsigned heads = min(p.head_group, p.bh - first_head);
+  unsigned in = index - group * per_group;  // kinds apart: [kind][rank][head], else [rank][kind][head]
+  const unsigned of_kind = p.tiles * heads;
+  const bool second_kind = p.kinds_apart && in >= of_kind;
+  if (second_kind) in -= of_kind;
+  int rank = in / heads;
+  const int head = in - rank * heads;
   BwdItem it;
-  if (p.kinds_apart) {
-    const int of_kind = in % (p.tiles * heads);
-    it.is_dq = in >= p.tiles * heads;
-    rank = of_kind / heads;
-    head = of_kind % heads;
-  } else {
-    const int of_rank = in % (2 * heads);
-    it.is_dq = of_rank >= heads;
-    rank = in / (2 * heads);
-    head = of_rank % heads;
-  }
+  it.is_dq = p.kinds_apart ? second_kind : rank & 1;
+  if (!p.kinds_apart) rank >>= 1;
   it.bh = first_head + head;
   const int wr = eff_window_right(p.causal, p.window_right);
   it.left = it.is_dq ? p.window_left : wr;
@@ -171,6 +166,12 @@ __device__ __forceinline__ BwdItem bwd_item(const BwdParams& p, int index) {
   it.begin = kv_tile_begin(it.r0, it.left);
   it.tiles = kv_tile_end(min(it.r0 + 127, p.seqlen - 1), it.right, p.seqlen) - it.begin;
   return it;
+}
+
+// The k-th work item of a CTA, or an index past the last: every other round of CTAs is dealt backwards, so that the CTAs'
+// sums are alike although the items of a group of heads get shorter under a causal mask.
+__device__ __forceinline__ int bwd_index(int k) {
+  return k * static_cast<int>(gridDim.x) + static_cast<int>(k & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
 }
 
 // 2^-e (see the top of this file) from a lane's norms. A bound that is zero, infinite or NaN leaves dS as it is. All lanes of a
@@ -199,7 +200,7 @@ struct BwdBars {
   // has that of the tile before
   uint64_t *stats_empty, *p_ready, *ds_ready, *acc_empty;
   volatile int* abort_flag;
-  volatile float* unit;  // of the items of even and odd turn
+  volatile float *unit, *slope;  // of the items of even and odd turn
 };
 
 // dK and dV at head_dim 128 have one region for S.
@@ -220,8 +221,8 @@ struct SoftmaxTurns {
 
 // Stores 32 rows of kPieces * 16 bytes, `rows` of which exist, from lanes that hold a row each. Written as they lie, a store
 // instruction touches 32 lines for 16 bytes each, 5300 clocks for the dK and dV of an item at head_dim 128 (2700 this way), in the
-// load/store unit that all warps share: B1 H4 N512 d128 16.8 -> 13.9 us, window 1024 2373 -> 2253. So groups of kPieces lanes first exchange their pieces: lane l gets piece l % kPieces of each of the
-// group's rows, and an instruction writes whole rows.
+// load/store unit that all warps share: B1 H4 N512 d128 16.8 -> 13.9 us, window 1024 2373 -> 2253. So groups of kPieces lanes
+// first exchange their pieces: lane l gets piece l % kPieces of each of the group's rows, and an instruction writes whole rows.
 template <int kPieces>
 __device__ __forceinline__ void bwd_store_rows(__half* to, int stride, int rows, uint4 (&piece)[kPieces], int lane) {
 #pragma unroll
@@ -251,26 +252,27 @@ __device__ __forceinline__ void bwd_store_rows(__half* to, int stride, int rows,
 // kDq: the statistics (14 - log2(e) * lse and -delta / 2^e) are the row's, P is not needed further; else they are the
 // columns', and P goes to the tensor cores too. Returns false once a wait has run out.
 template <int D, bool kAlibi, bool kDq>
-__device__ __forceinline__ bool bwd_softmax(const BwdParams& p, const BwdItem& it, const BwdBars& b, const uint8_t* smem,
-                                            uint32_t tmem_base, int warp, int lane, int turn, SoftmaxTurns<D>& at) {
+__device__ __forceinline__ bool bwd_softmax(const BwdParams& p, const BwdItem& it, BwdItem& next, const BwdBars& b,
+                                            const uint8_t* smem, uint32_t tmem_base, int warp, int lane, int turn,
+                                            SoftmaxTurns<D>& at) {
   using Cfg = BwdCfg<D>;
   const int quarter = warp >> 2;
   const uint32_t lane_base = (warp & 3) * 32u;
   const int row = it.r0 + static_cast<int>(lane_base) + lane;
   const uint64_t scale2 = f2_pack(p.scale_log2, p.scale_log2);
-  const float slope = kAlibi ? p.alibi_slopes[it.bh % p.heads] * 1.4426950408889634f : 0.f;
   const int r_last = min(it.r0 + 127, p.seqlen - 1);
   constexpr bool kTwoS = bwd_two_s<D>(kDq);
   const uint32_t tS = tmem_addr(tmem_base, lane_base, Cfg::kColS + quarter * 32);
   const uint32_t tDp = tmem_addr(tmem_base, lane_base, Cfg::kColDp + quarter * 32);
   bool ok = true;  // (looked at once a tile: a vote behind each wait costs more than the wait)
-  float unit = 1.f, nl = 0.f, nd = 0.f;
+  float unit = 1.f, slope = 0.f, nl = 0.f, nd = 0.f;
   if (kDq) {
     ok &= mbar_wait(b.stats_full + at.stats.slot, at.stats.parity, b.abort_flag);
     const float* stats = reinterpret_cast<const float*>(smem + Cfg::kOffStats + at.stats.slot * 1024);
     nl = stats[lane_base + lane];
     nd = stats[128 + lane_base + lane];
     unit = b.unit[turn & 1];
+    if (kAlibi) slope = b.slope[turn & 1];
     __syncwarp();
     mbar_arrive_lane0(b.stats_empty + at.stats.slot, lane);
     at.stats.advance();
@@ -284,7 +286,10 @@ __device__ __forceinline__ bool bwd_softmax(const BwdParams& p, const BwdItem& i
 
     if (!kDq) {
       ok &= mbar_wait(b.stats_full + at.stats.slot, at.stats.parity, b.abort_flag);
-      if (i == 0) unit = b.unit[turn & 1];
+      if (i == 0) {
+        unit = b.unit[turn & 1];
+        if (kAlibi) slope = b.slope[turn & 1];
+      }
     }
     const int odd = kTwoS ? i & 1 : 0;
     ok &= mbar_wait(b.s_full + odd, at.s >> odd & 1u, b.abort_flag);
@@ -364,6 +369,8 @@ __device__ __forceinline__ bool bwd_softmax(const BwdParams& p, const BwdItem& i
   }
 
   // ---- epilogue: dQ a quarter of the columns a warp; dV the first eight warps, dK the others, half of the columns each ----
+  // (the next item's place is worked out while the last product runs: after the epilogue it cost 1000 clocks)
+  if (bwd_index(turn + 1) < 2 * p.tiles * p.bh) next = bwd_item(p, bwd_index(turn + 1));
   ok &= mbar_wait(b.acc_full, at.acc, b.abort_flag);
   at.acc ^= 1;
   tc_fence_after();
@@ -393,12 +400,6 @@ __device__ __forceinline__ bool bwd_softmax(const BwdParams& p, const BwdItem& i
   __syncwarp();
   mbar_arrive_lane0(b.acc_empty, lane);
   return __all_sync(0xffffffffu, ok);
-}
-
-// The k-th work item of a CTA, or an index past the last: every other round of CTAs is dealt backwards, so that the CTAs'
-// sums are alike although the items of a group of heads get shorter under a causal mask.
-__device__ __forceinline__ int bwd_index(int k) {
-  return k * static_cast<int>(gridDim.x) + static_cast<int>(k & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
 }
 
 // The warp that issues the products of all items.
@@ -433,8 +434,9 @@ __device__ __forceinline__ bool bwd_issue(const BwdParams& p, const BwdBars& b, 
   Turn<Cfg::kFirst> f_scores, f_acc;  // first tiles: whose scores come next, whose product comes next
   Turn<Cfg::kSecond> s_scores, s_acc;
   uint32_t p_at = 0, ds_at = 0, own_at = 0, acc_at = 1;  // parities, p_at of either p_ready (the accumulators are free at the start)
-  for (int k = 0, index; (index = bwd_index(k)) < 2 * p.tiles * p.bh && ok; ++k) {
-    const BwdItem it = bwd_item(p, index);
+  BwdItem it, next = bwd_item(p, bwd_index(0));
+  for (int k = 0; bwd_index(k) < 2 * p.tiles * p.bh && ok; ++k) {
+    it = next;
     const int n = it.tiles;
     const bool two_s = bwd_two_s<D>(it.is_dq);
     auto s_col = [&](int i) { return two_s && (i & 1) ? Cfg::kColOdd : Cfg::kColS; };
@@ -465,6 +467,7 @@ __device__ __forceinline__ bool bwd_issue(const BwdParams& p, const BwdBars& b, 
     wait(b.acc_empty, acc_at);  // (before the odd S, which may lie where an accumulator of the item before is)
     acc_at ^= 1;
     if (two_s && n > 1) scores_first(1);
+    if (bwd_index(k + 1) < 2 * p.tiles * p.bh) next = bwd_item(p, bwd_index(k + 1));
     if (it.is_dq) {
       for (int i = 0; i < n && ok; ++i) {
         wait(b.ds_ready, ds_at);
@@ -562,7 +565,7 @@ __device__ __forceinline__ void bwd_own_rows(const BwdParams& p, int bh, uint8_t
 }
 
 // The warp that brings the statistics: for dK and dV those of every column tile, for dQ those of the item's own rows.
-template <int D, bool kOwnRows>
+template <int D, bool kAlibi, bool kOwnRows>
 __device__ __forceinline__ void bwd_stats(const BwdParams& p, const BwdBars& b, uint8_t* smem, int lane) {
   using Cfg = BwdCfg<D>;
   Turn<Cfg::kStats> at;
@@ -584,6 +587,7 @@ __device__ __forceinline__ void bwd_stats(const BwdParams& p, const BwdBars& b, 
       }
     };
     load(0);  // (on its way while the norms are read)
+    const float slope = kAlibi ? p.alibi_slopes[it.bh % p.heads] * 1.4426950408889634f : 0.f;
     float norm[3] = {0.f, 0.f, 0.f};
     if (kOwnRows) {
       if (!mbar_wait_warp(reinterpret_cast<uint64_t*>(const_cast<float*>(norms_here + 48)), 0, b.abort_flag)) return;
@@ -608,7 +612,10 @@ __device__ __forceinline__ void bwd_stats(const BwdParams& p, const BwdBars& b, 
         to[j * 32 + lane] = nl[j];
         to[128 + j * 32 + lane] = nd[j];
       }
-      if (i == 0 && lane == 0) b.unit[k & 1] = unit;
+      if (i == 0 && lane == 0) {
+        b.unit[k & 1] = unit;
+        if (kAlibi) b.slope[k & 1] = slope;
+      }
       __syncwarp();
       mbar_arrive_lane0(b.stats_full + at.slot, lane);
       at.advance();
@@ -649,7 +656,12 @@ bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + Cfg::kNumBars);
   b.abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   b.unit = reinterpret_cast<volatile float*>(tmem_slot + 2);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  b.slope = b.unit + 2;
+  // The shuffles let the compiler see that the warp's number and the address in tensor memory are the same in all lanes: the
+  // issuer's branch then is one that a warp takes as a whole, and the operands of its products are computed in uniform registers,
+  // not moved there one by one. 17 -> 12 clocks for the instructions around a product, more where the softmax warps compete for
+  // the issue slots: 8 heads x 2048 d64 41.4 -> 38.2 us, B8 H12 N1000 d64 128 -> 119, B2 H32 N8192 d128 causal 3790 -> 3400.
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
   if (warp == 16) {
     tmem_alloc(tmem_slot, Cfg::kTmemCols);
@@ -667,7 +679,7 @@ bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem_base = *tmem_slot;
+  const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   if (kOwnRows) griddep_wait();
   // bwd_rows_kernel lets this kernel in only behind its own griddep_wait(): whatever came before the two of them is complete,
   // and only the warp that reads what bwd_rows_kernel writes has to wait for it. (Every CTA has one, so whoever waits for this
@@ -676,13 +688,14 @@ bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
 
   if (warp < Cfg::kSoftmaxWarps) {
     reg_inc<Cfg::kRegSoftmax>();
-    if (kOwnRows) bwd_own_rows<D>(p, bwd_item(p, blockIdx.x).bh, smem, warp, lane);
+    BwdItem next = bwd_item(p, bwd_index(0));
+    if (kOwnRows) bwd_own_rows<D>(p, next.bh, smem, warp, lane);
     SoftmaxTurns<D> at;
     bool ok = true;
-    for (int k = 0, index; (index = bwd_index(k)) < 2 * p.tiles * p.bh && ok; ++k) {
-      const BwdItem it = bwd_item(p, index);
-      ok = it.is_dq ? bwd_softmax<D, kAlibi, true>(p, it, b, smem, tmem_base, warp, lane, k, at)
-                    : bwd_softmax<D, kAlibi, false>(p, it, b, smem, tmem_base, warp, lane, k, at);
+    for (int k = 0; bwd_index(k) < 2 * p.tiles * p.bh && ok; ++k) {
+      const BwdItem it = next;
+      ok = it.is_dq ? bwd_softmax<D, kAlibi, true>(p, it, next, b, smem, tmem_base, warp, lane, k, at)
+                    : bwd_softmax<D, kAlibi, false>(p, it, next, b, smem, tmem_base, warp, lane, k, at);
     }
   } else {
     reg_dec<Cfg::kRegOthers>();
@@ -694,7 +707,7 @@ bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
         for (int i = 0; i < 64; ++i) __nanosleep(2000);
       __syncwarp();
     } else if (warp == 18) {
-      bwd_stats<D, kOwnRows>(p, b, smem, lane);
+      bwd_stats<D, kAlibi, kOwnRows>(p, b, smem, lane);
     }
   }
 

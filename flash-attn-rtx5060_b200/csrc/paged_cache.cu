@@ -4,14 +4,23 @@
 
 #include "host.h"
 #include "paged_cache.cuh"
+#include "paged_cache_wide.cuh"
 
 using namespace fa_host;
 
 namespace {
 
-// CTAs of a call on a B200's 148 SMs: two a SM for tiles of 16 rows, else one (their rings of tiles keep 192 KB a SM in flight
+// CTAs of a call on a B200's 148 SMs: two a SM for up to 16 rows, else one (their rings of tiles keep 192 KB a SM in flight
 // either way). On a device with fewer SMs they run one after the other.
-int decode_ctas(int tile_rows) { return tile_rows == 16 ? 296 : 148; }
+int decode_ctas(long long rows) { return rows <= 16 ? 296 : 148; }
+// Rows (query heads of a key head times new tokens) of a row tile, of which a tile of keys is read once.
+int part_rows(long long rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
+// Whether decode_wide_kernel takes a call: it starts and ends an item later by 5 us together, and takes half as long over a tile.
+// `work`: tiles of keys a CTA, if all sequences were as long as they may be. us, decode_kernel -> decode_wide_kernel, 16 sequences
+// on 8 key heads: 64 rows d128 x 512 26.6 -> 29.6, x 1024 (14 tiles a CTA) 36.8 -> 33.9, x 4096 93 -> 68, up to 32768 352 -> 209;
+// 32 rows d128 x 4096 (55) 58.8 -> 60.5, up to 32768 220 -> 198; 32 rows d64 x 4096 (28) 38.3 -> 36.7; and 2048 tokens of
+// 32 heads on 8 over 8192 keys 1270 -> 404, 4 x 256 tokens 395 -> 153.
+bool decode_wide(long long rows, long long work) { return rows > 64 || (rows > 16 && work >= (rows > 32 ? 10 : 48)); }
 constexpr long long kJoinBlocks = 148 * 6;
 // CTAs of a cluster that takes an item (a sequence, key head and tile of rows) of up to `tiles` tiles of keys as a whole, 1 for
 // a CTA alone, or 0 where the items are cut by the line and joined by a second launch (which takes as long as four tiles or
@@ -76,8 +85,8 @@ fa::CacheView view_of(const fa_paged_cache* c, int batch, int tokens, DeviceStat
 }
 
 // 5-D map over the pages of K or V: {64 contiguous elements, token of the page, 64-wide panel, head, page}. One box is
-// `box_rows` tokens of a head, [panel][token][64] in shared memory with the 128-byte swizzle.
-int make_page_map(CUtensorMap* map, const fa_paged_cache* c, void* base, int box_rows) {
+// `box_rows` tokens and `box_panels` panels of a head, [panel][token][64] in shared memory with the 128-byte swizzle.
+int make_page_map(CUtensorMap* map, const fa_paged_cache* c, void* base, int box_rows, int box_panels) {
   EncodeTiledFn enc = encode_tiled_fn();
   if (!enc) return fail(FA_CUDA_ERROR, "cuTensorMapEncodeTiled entry point not available");
   const cuuint64_t row = 2ull * c->head_dim;
@@ -85,7 +94,7 @@ int make_page_map(CUtensorMap* map, const fa_paged_cache* c, void* base, int box
                         (cuuint64_t)c->num_pages};
   cuuint64_t strides[4] = {2ull * c->token_stride, 128, c->kv_heads > 1 ? 2ull * c->head_stride : row,
                            c->num_pages > 1 ? 2ull * c->page_stride : row};
-  cuuint32_t box[5] = {64, (cuuint32_t)box_rows, (cuuint32_t)(c->head_dim / 64), 1, 1};
+  cuuint32_t box[5] = {64, (cuuint32_t)box_rows, (cuuint32_t)box_panels, 1, 1};
   cuuint32_t estr[5] = {1, 1, 1, 1, 1};
   CUresult r = enc(map, c->dtype == FA_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, base,
                    dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
@@ -94,39 +103,47 @@ int make_page_map(CUtensorMap* map, const fa_paged_cache* c, void* base, int box
   return FA_OK;
 }
 
-// Rows (query heads of a key head times new tokens) of a CTA's tile: 16 where they fit, else 32 or 64, so that a tile of
-// keys is read for as many rows as there are.
-int tile_rows(long long rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
-
-template <typename T, int D, int kRowWarps>
-int launch_decode(const CUtensorMap& mk, const CUtensorMap& mv, const fa::DecodeParams& p, cudaStream_t st, bool early) {
-  using Cfg = fa::DecodeCfg<D, kRowWarps>;
-  constexpr auto kernel = fa::decode_kernel<T, D, kRowWarps>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes);
-  if (e != cudaSuccess) return fail_cuda("cudaFuncSetAttribute(MaxDynamicSharedMemorySize)", e);
-  const unsigned grid =
-      p.cluster > 0 ? static_cast<unsigned>(p.cluster) * p.cache.batch * p.cache.kv_heads * p.row_tiles : p.ctas;
-  e = launch_early_in_clusters(kernel, p.cluster > 0 ? p.cluster : 1, dim3(grid), Cfg::kThreads, Cfg::kSmemBytes, st, early, mk, mv,
-                               p);
-  if (e != cudaSuccess) return fail_cuda("launch decode_kernel", e);
-  if (p.cluster > 0) return FA_OK;
+template <typename T, int D>
+int launch_join(const fa::DecodeParams& p, cudaStream_t st, bool early) {
   const long long rows = static_cast<long long>(p.cache.batch) * p.q_heads * p.cache.tokens;
   // a row by the four warps of a block while that is one wave of blocks
-  e = rows <= kJoinBlocks
-          ? launch_early(fa::decode_join_kernel<T, D, 4>, dim3(static_cast<unsigned>(rows)), 128, 0, st, early, p,
-                         static_cast<int>(Cfg::kRows))
-          : launch_early(fa::decode_join_kernel<T, D, 1>, dim3(static_cast<unsigned>((rows + 3) / 4)), 128, 0, st, early, p,
-                         static_cast<int>(Cfg::kRows));
+  cudaError_t e =
+      rows <= kJoinBlocks
+          ? launch_early(fa::decode_join_kernel<T, D, 4>, dim3(static_cast<unsigned>(rows)), 128, 0, st, early, p)
+          : launch_early(fa::decode_join_kernel<T, D, 1>, dim3(static_cast<unsigned>((rows + 3) / 4)), 128, 0, st, early, p);
   if (e != cudaSuccess) return fail_cuda("launch decode_join_kernel", e);
   return FA_OK;
 }
 
+using DecodeKernel = void (*)(CUtensorMap, CUtensorMap, fa::DecodeParams);
 template <typename T, int D>
-int launch_decode_rows(int rows, const CUtensorMap& mk, const CUtensorMap& mv, const fa::DecodeParams& p, cudaStream_t st,
-                       bool early) {
-  return rows == 16   ? launch_decode<T, D, 1>(mk, mv, p, st, early)
-         : rows == 32 ? launch_decode<T, D, 2>(mk, mv, p, st, early)
-                      : launch_decode<T, D, 4>(mk, mv, p, st, early);
+int launch_decode(DecodeKernel kernel, int threads, int smem, const fa_paged_cache* c, int box_panels, const fa::DecodeParams& p,
+                  cudaStream_t st, bool early) {
+  CUtensorMap mk, mv;
+  int rc = make_page_map(&mk, c, c->k, p.box_rows, box_panels);
+  if (rc != FA_OK || (rc = make_page_map(&mv, c, c->v, p.box_rows, box_panels)) != FA_OK) return rc;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return fail_cuda("cudaFuncSetAttribute(MaxDynamicSharedMemorySize)", e);
+  const unsigned grid =
+      p.cluster > 0 ? static_cast<unsigned>(p.cluster) * p.cache.batch * p.cache.kv_heads * p.row_tiles : p.ctas;
+  e = launch_early_in_clusters(kernel, p.cluster > 0 ? p.cluster : 1, dim3(grid), threads, smem, st, early, mk, mv, p);
+  if (e != cudaSuccess) return fail_cuda("launch of the decoding kernel", e);
+  return p.cluster > 0 ? FA_OK : launch_join<T, D>(p, st, early);
+}
+
+template <typename T, int D, int kRowWarps>
+int launch_narrow(const fa_paged_cache* c, const fa::DecodeParams& p, cudaStream_t st, bool early) {
+  using Cfg = fa::DecodeCfg<D, kRowWarps>;
+  return launch_decode<T, D>(fa::decode_kernel<T, D, kRowWarps>, Cfg::kThreads, Cfg::kSmemBytes, c, D / 64, p, st, early);
+}
+
+template <typename T, int D>
+int launch_rows(long long rows, bool wide, const fa_paged_cache* c, const fa::DecodeParams& p, cudaStream_t st, bool early) {
+  using Cfg = fa::WideCfg<D>;
+  if (wide) return launch_decode<T, D>(fa::decode_wide_kernel<T, D>, Cfg::kThreads, Cfg::kSmemBytes, c, 1, p, st, early);
+  return rows <= 16   ? launch_narrow<T, D, 1>(c, p, st, early)
+         : rows <= 32 ? launch_narrow<T, D, 2>(c, p, st, early)
+                      : launch_narrow<T, D, 4>(c, p, st, early);
 }
 
 }  // namespace
@@ -187,8 +204,8 @@ int flash_cache_append(const fa_paged_cache* cache, const fa_rows* k, const fa_r
 
 size_t flash_decode_workspace_bytes(int tokens, int q_heads, int kv_heads, int head_dim) {
   if (tokens <= 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads != 0 || head_dim <= 0) return 0;
-  const int rows = tile_rows(static_cast<long long>(q_heads / kv_heads) * tokens);
-  return static_cast<size_t>(2) * decode_ctas(rows) * rows * (head_dim + 2) * sizeof(float);
+  const long long rows = static_cast<long long>(q_heads / kv_heads) * tokens;
+  return static_cast<size_t>(2) * decode_ctas(rows) * part_rows(rows) * (head_dim + 2) * sizeof(float);
 }
 
 int flash_decode(const fa_paged_cache* cache, const fa_rows* q, void* o, float* lse, int batch, int tokens, int q_heads,
@@ -216,7 +233,6 @@ int flash_decode(const fa_paged_cache* cache, const fa_rows* q, void* o, float* 
   if (!s->is_sm100) return fail(FA_UNSUPPORTED, "this library runs on compute capability 10.x (B200) only");
   if (softmax_scale <= 0.f) softmax_scale = 1.0f / sqrtf(static_cast<float>(cache->head_dim));
 
-  const int tile = tile_rows(rows);
   fa::DecodeParams p;
   memset(&p, 0, sizeof(p));
   p.cache = view_of(cache, batch, tokens, s);
@@ -232,27 +248,28 @@ int flash_decode(const fa_paged_cache* cache, const fa_rows* q, void* o, float* 
   const int tile_keys = cache->head_dim == 128 ? fa::kDecodeKeys<128> : fa::kDecodeKeys<64>;
   if (p.box_rows > tile_keys) p.box_rows = tile_keys;
   p.tile_shift = cache->head_dim == 128 ? 6 : 7;
-  p.row_tiles = static_cast<int>((rows + tile - 1) / tile);
-  p.ctas = decode_ctas(tile);
+  p.part_rows = part_rows(rows);
+  p.row_tiles = static_cast<int>((rows + p.part_rows - 1) / p.part_rows);
+  p.ctas = decode_ctas(rows);
   long long longest = static_cast<long long>(cache->max_pages) * cache->page_size;  // keys that an item may have
   if (window_left >= 0 && longest > static_cast<long long>(window_left) + tokens)
     longest = static_cast<long long>(window_left) + tokens;
   const long long tiles = (longest + tile_keys - 1) / tile_keys + (window_left >= 0);
   const long long items = static_cast<long long>(batch) * cache->kv_heads * p.row_tiles;
-  if (static_cast<double>(items) * (tiles + 2) > 0x7fffffff - 512)
+  if (static_cast<double>(items) * (tiles + 8) > 0x7fffffff - 512)
     return fail(FA_INVALID_ARG, "more tiles of keys than 31 bits count");
   p.cluster = decode_cluster(tiles, items, p.ctas);
+  const bool wide = decode_wide(rows, items * tiles / p.ctas);
+  if (wide && p.cluster > 1) p.cluster = 0;
+  p.item_units = wide ? 4 : 1;
   p.part_o = static_cast<float*>(workspace);
-  p.part_ml = p.part_o + static_cast<size_t>(2) * p.ctas * tile * cache->head_dim;
+  p.part_ml = p.part_o + static_cast<size_t>(2) * p.ctas * p.part_rows * cache->head_dim;
   p.status = s->status;
-  CUtensorMap mk, mv;
-  if ((rc = make_page_map(&mk, cache, cache->k, p.box_rows)) != FA_OK) return rc;
-  if ((rc = make_page_map(&mv, cache, cache->v, p.box_rows)) != FA_OK) return rc;
   if (cache->dtype == FA_FP16)
-    return cache->head_dim == 64 ? launch_decode_rows<__half, 64>(tile, mk, mv, p, st, !captured)
-                                 : launch_decode_rows<__half, 128>(tile, mk, mv, p, st, !captured);
-  return cache->head_dim == 64 ? launch_decode_rows<__nv_bfloat16, 64>(tile, mk, mv, p, st, !captured)
-                               : launch_decode_rows<__nv_bfloat16, 128>(tile, mk, mv, p, st, !captured);
+    return cache->head_dim == 64 ? launch_rows<__half, 64>(rows, wide, cache, p, st, !captured)
+                                 : launch_rows<__half, 128>(rows, wide, cache, p, st, !captured);
+  return cache->head_dim == 64 ? launch_rows<__nv_bfloat16, 64>(rows, wide, cache, p, st, !captured)
+                               : launch_rows<__nv_bfloat16, 128>(rows, wide, cache, p, st, !captured);
 }
 
 }  // extern "C"

@@ -1,5 +1,6 @@
 // Kernels of the paged key-value cache: new keys and values enter it (cache_append_kernel), and the newest tokens of every
-// sequence attend to what it holds (decode_kernel, and decode_join_kernel for the sequences that several CTAs shared).
+// sequence attend to what it holds (decode_kernel here, decode_wide_kernel where there are many rows, and decode_join_kernel for
+// the sequences that several CTAs shared).
 //
 // The keys and values of a sequence lie in pages of `page_size` tokens that its row of the page table names in order:
 // token j is row j % page_size of page table[j / page_size]. Nothing of a page behind the sequence's last token, and no
@@ -184,14 +185,16 @@ struct DecodeParams {
   int row_tiles;  // of the group * tokens rows of a key head
   int ctas;
   int cluster;     // CTAs of a cluster that share an item and join it themselves (1: a CTA an item), or 0: the line below
-  float* part_o;   // [ctas][2][rows of a tile][head_dim]
-  float* part_ml;  // [ctas][2][rows of a tile][2]: running maximum (log2 units) and sum
+  float* part_o;   // [ctas][2][part_rows][head_dim]
+  float* part_ml;  // [ctas][2][part_rows][2]: running maximum (log2 units) and sum
+  int part_rows;   // rows of a row tile
+  int item_units;  // tiles of keys that an item's beginning and end take as long as
   int* status;
 };
 
-// The work is one line of tiles of 64 keys: sequence by sequence, in each key head by key head (and row tile by row
-// tile), the tiles that the new tokens see. Every CTA takes an equal stretch of the line, to within a tile. A (sequence, key head, row tile)
-// that lies within one stretch is finished there; one that is cut has its parts written as (maximum, sum, unnormalised
+// The work is one line of tiles of 32 KB: sequence by sequence, in each key head by key head (and row tile by row tile), the
+// tiles that the new tokens see. Every CTA takes an equal stretch of the line, to within a tile. A (sequence, key head, row
+// tile) that lies within one stretch is finished there; one that is cut has its parts written as (maximum, sum, unnormalised
 // output) and joined by decode_join_kernel in the order of the line, so the results depend on the lengths alone. Where few
 // items are short, or many are very short, an item has a cluster of CTAs, or one CTA, to itself instead, and no second launch.
 struct DecodeLine {
@@ -201,17 +204,17 @@ struct DecodeLine {
     first = lo >> p.tile_shift;
     tiles = count > 0 ? ((length - 1) >> p.tile_shift) + 1 - first : 0;
   }
-  // What an item takes up on the line: a tile for its beginning and end (Q, the join of the warps and the output take a CTA about
-  // as long as a tile does), then its tiles.
-  __device__ static int units_of(int tiles) { return tiles > 0 ? tiles + 1 : 0; }
+  // What an item takes up on the line: p.item_units for its beginning and end (Q, the join of the warps and the output take a CTA
+  // about as long as so many tiles), then its tiles.
+  __device__ static int units_of(const DecodeParams& p, int tiles) { return tiles > 0 ? tiles + p.item_units : 0; }
   // Sums the units of an item of every sequence, and of those in front of `upto`. All lanes of a warp call it.
   __device__ static void sum(const DecodeParams& p, int upto, int& all, int& before, int lane) {
     all = before = 0;
     for (int b = lane; b < p.cache.batch; b += 32) {
       int first, tiles, length, count;
       tiles_of(p, b, first, tiles, length, count);
-      all += units_of(tiles);
-      if (b < upto) before += units_of(tiles);
+      all += units_of(p, tiles);
+      if (b < upto) before += units_of(p, tiles);
     }
 #pragma unroll
     for (int s = 16; s > 0; s >>= 1) {
@@ -254,7 +257,7 @@ struct DecodeWalk {
     for (int b0 = 0; b0 < p.cache.batch; b0 += 32) {
       int f = 0, n = 0, len = 0, cnt = 0;
       if (b0 + lane < p.cache.batch) DecodeLine::tiles_of(p, b0 + lane, f, n, len, cnt);
-      int upto = DecodeLine::units_of(n);
+      int upto = DecodeLine::units_of(p, n);
 #pragma unroll
       for (int s = 1; s < 32; s <<= 1) {
         const int v = __shfl_up_sync(0xffffffffu, upto, s);
@@ -276,7 +279,7 @@ struct DecodeWalk {
         tiles = __shfl_sync(0xffffffffu, n, src);
         length = __shfl_sync(0xffffffffu, len, src);
         count = __shfl_sync(0xffffffffu, cnt, src);
-        b_start = __shfl_sync(0xffffffffu, upto, src) - DecodeLine::units_of(tiles) * per;
+        b_start = __shfl_sync(0xffffffffu, upto, src) - DecodeLine::units_of(p, tiles) * per;
         return;
       }
       b_start = __shfl_sync(0xffffffffu, upto, 31);
@@ -298,16 +301,16 @@ struct DecodeWalk {
     }
     const int per = p.cache.kv_heads * p.row_tiles;
     while (at < end) {
-      while (at >= b_start + DecodeLine::units_of(tiles) * per) {
-        b_start += DecodeLine::units_of(tiles) * per;
+      while (at >= b_start + DecodeLine::units_of(p, tiles) * per) {
+        b_start += DecodeLine::units_of(p, tiles) * per;
         ++b;
         DecodeLine::tiles_of(p, b, first, tiles, length, count);
       }
-      const int units = DecodeLine::units_of(tiles), item = (at - b_start) / units, from = at - b_start - item * units;
+      const int units = DecodeLine::units_of(p, tiles), item = (at - b_start) / units, from = at - b_start - item * units;
       const int to = min(from + end - at, units);
       at += to - from;
-      t0 = max(from - 1, 0);
-      t1 = to - 1;
+      t0 = max(from - p.item_units, 0);
+      t1 = to - p.item_units;
       kv_head = item / p.row_tiles;
       row_tile = item % p.row_tiles;
       if (t1 > t0) return true;
@@ -388,9 +391,9 @@ __device__ __forceinline__ void compute_sync() {
 // A CTA's warps take 16 * kRowWarps rows (a row: one query head of the key head's group and one new token) and share a tile's
 // keys. The products run as m16n8k16 matrix instructions: a step of generation reads every key for a handful of rows, so HBM is
 // what bounds it (at 16 rows a tile of 32 KB is 128 such instructions of an SM), and rows that are padding cost nothing that
-// matters: 64 sequences of up to 32768 tokens, 32 heads on 8 of 128, 4.8 GB in 704-722 us; one of 131072 in 89 us (6.0 TB/s, 5 of
-// them start and join). More than 16 rows leave the warps latency-bound (16 x 8 tokens, 64 heads on 8, up to 8192 tokens: 108 us
-// for 306 MB). Scores, maxima, sums and O are fp32; P is rounded to the cache's type for the second product, as the operand has to
+// matters: 64 sequences of up to 32768 tokens, 32 heads on 8 of 128, 4.8 GB in 704-741 us; one of 131072 in 89 us (6.0 TB/s, 5 of
+// them start and join). More than 16 rows leave the warps latency-bound (16 x 8 tokens, 64 heads on 8, up to 32768 tokens: 352 us
+// for 1.2 GB), so there decode_wide_kernel takes all but short work. Scores, maxima, sums and O are fp32; P is rounded to the cache's type for the second product, as the operand has to
 // be, half a step relative to the element, and its sum is taken unrounded.
 template <typename T, int D, int kRowWarps>
 __global__ void __launch_bounds__(DecodeCfg<D, kRowWarps>::kThreads, DecodeCfg<D, kRowWarps>::kCtasPerSm)
@@ -765,7 +768,7 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
 // in the order of the line, then the warps in their order. Rows of sequences without keys, and rows of padding, are set to
 // O = 0 and a log-sum-exp of -infinity.
 template <typename T, int D, int kWarps>
-__global__ void __launch_bounds__(128, 6) decode_join_kernel(const __grid_constant__ DecodeParams p, int tile_rows) {
+__global__ void __launch_bounds__(128, 6) decode_join_kernel(const __grid_constant__ DecodeParams p) {
   constexpr int kOwn = D / 32;  // elements of a lane
   __shared__ float s_o[kWarps][D];
   __shared__ float2 s_ml[kWarps];
@@ -783,15 +786,15 @@ __global__ void __launch_bounds__(128, 6) decode_join_kernel(const __grid_consta
   if (real) {
     int all, before;
     DecodeLine::sum(p, b, all, before, lane);
-    const int item = head / p.group * p.row_tiles + r / tile_rows;
+    const int item = head / p.group * p.row_tiles + r / p.part_rows;
     const DecodeLine line(p, all);
-    const int from = before * p.cache.kv_heads * p.row_tiles + item * DecodeLine::units_of(tiles) + 1;
+    const int from = before * p.cache.kv_heads * p.row_tiles + item * DecodeLine::units_of(p, tiles) + p.item_units;
     c0 = line.cta_of(from);
     c1 = line.cta_of(from + tiles - 1);
   }
   griddep_wait();
   if (real && c0 == c1) return;
-  auto part = [&](int c) { return (2ll * c + (c == c0 ? 1 : 0)) * tile_rows + r % tile_rows; };
+  auto part = [&](int c) { return (2ll * c + (c == c0 ? 1 : 0)) * p.part_rows + r % p.part_rows; };
   float o[kOwn], m = -INFINITY, l = 0.f;
 #pragma unroll
   for (int i = 0; i < kOwn; ++i) o[i] = 0.f;

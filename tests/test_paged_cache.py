@@ -74,7 +74,8 @@ def test_workspace_bytes(pkg):
     size = pkg.lib().flash_decode_workspace_bytes
     assert size(1, 32, 8, 128) == 296 * 2 * 16 * 130 * 4
     assert size(4, 32, 8, 64) == size(1, 16, 1, 64) == 296 * 2 * 16 * 66 * 4
-    assert size(1, 17, 1, 64) == 148 * 2 * 32 * 66 * 4 and size(1, 33, 1, 64) == size(100, 8, 1, 64) == 148 * 2 * 64 * 66 * 4
+    assert size(1, 17, 1, 64) == 148 * 2 * 32 * 66 * 4 and size(1, 33, 1, 64) == size(8, 8, 1, 64) == 148 * 2 * 64 * 66 * 4
+    assert size(65, 1, 1, 64) == size(100, 8, 1, 64) == 148 * 2 * 128 * 66 * 4
     assert size(0, 8, 8, 64) == size(1, 8, 3, 64) == size(1, 8, 0, 64) == 0
 
 

@@ -58,6 +58,118 @@ def test_decode(pkg, dtype, head_dim, q_heads, kv_heads, tokens, page, lengths):
     check_decode(pkg, b, b.rows(q_heads))
 
 
+def with_room(batch, keys=1 << 19):
+    """The same batch with a page table that has room for long sequences: how a call is computed depends on that room."""
+    more = torch.full((len(batch.lengths), keys // batch.page_size), -7, dtype=torch.int32)
+    more[:, :batch.table.shape[1]] = batch.table
+    batch.table = more
+    return batch
+
+
+MANY_ROWS = [  # query heads, key heads, tokens, page, lengths
+    (24, 1, 1, 16, [1]),                         # 24 rows, one key
+    (8, 1, 3, 24, [3, 64, 65, 127, 128, 129]),   # around the ends of tiles
+    (32, 1, 1, 8, [192, 0, 193, 0, 256, 257]),   # 32 rows; one, two and three tiles; sequences without keys between others
+    (33, 1, 1, 64, [700, 41]),
+    (16, 2, 8, 128, [500, 8, 1100]),             # 64 rows of either key head
+    (65, 1, 1, 16, [330]),
+    (20, 2, 10, 32, [10, 11, 640]),              # 100 rows
+    (4, 1, 32, 16, [32, 150]),                   # 128 rows, a sequence that holds nothing else
+    (43, 1, 3, 16, [260]),                       # 129 rows: two row tiles
+    (4, 2, 150, 256, [150, 400]),                # 300 rows
+    (20, 1, 1, 16, [3000]),                      # cut among many CTAs
+    (40, 2, 1, 16, [37 * i * i % 300 for i in range(40)]),  # items that share CTAs
+]
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("head_dim", [64, 128])
+@pytest.mark.parametrize("q_heads,kv_heads,tokens,page,lengths", MANY_ROWS)
+def test_many_rows(pkg, dtype, head_dim, q_heads, kv_heads, tokens, page, lengths):
+    b = oracle.Batch(70 + len(lengths) + head_dim, lengths, [min(tokens, n) for n in lengths], tokens, kv_heads, head_dim, page,
+                     dtype)
+    q = b.rows(q_heads)
+    check_decode(pkg, b, q, counts=True)
+    long = check_decode(pkg, with_room(b), q, counts=True)
+    again = check_decode(pkg, b, q, counts=True)
+    for x, y in zip(long, again):
+        assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("head_dim", [64, 128])
+@pytest.mark.parametrize("window,alibi", [(0, False), (1, True), (63, False), (64, True), (200, False), (100000, True)])
+def test_many_rows_window_and_alibi(pkg, head_dim, window, alibi):
+    b = with_room(oracle.Batch(71, [5, 64, 133, 700, 0], [5, 6, 6, 2, 0], 6, 2, head_dim, 16, "fp16"))
+    slopes = torch.tensor([0.5, 0.01, -0.02, 0.0, 0.1, 0.2, 0.3, 0.003]) if alibi else None
+    check_decode(pkg, b, b.rows(8), counts=True, window_left=window, alibi_slopes=slopes)
+
+
+@pytest.mark.parametrize("head_dim,rows", [(64, 24), (64, 48), (64, 96), (128, 24), (128, 96)])
+@pytest.mark.parametrize("fill", [math.nan, math.inf])
+def test_many_rows_ignore_what_is_not_the_sequences(pkg, head_dim, rows, fill):
+    b = oracle.Batch(72, [1, 40, 200, 317], [1, 2, 2, 1], 2, 1, head_dim, 32, "bf16", fill=fill)
+    for window in (-1, 70):
+        if window >= 0:
+            for i, n in enumerate(b.lengths):
+                gone = max(0, n - b.counts[i] - window)
+                for j in range(gone):
+                    b.k_pages[b.table[i, j // 32], :, j % 32] = fill
+                    b.v_pages[b.table[i, j // 32], :, j % 32] = fill
+                b.table[i, :gone // 32] = -1
+        check_decode(pkg, with_room(b), b.rows(rows // 2), counts=True, window_left=window)
+
+
+@pytest.mark.parametrize("head_dim", [64, 128])
+@pytest.mark.parametrize("rows", [24, 60, 120])
+def test_many_rows_with_scores_that_grow(pkg, head_dim, rows):
+    """The maximum of a row rises from tile to tile: scores with a deviation of 6, and keys that grow along the sequence."""
+    b = oracle.Batch(73, [900, 400], [1, 1], 1, 1, head_dim, 16, "fp16")
+    for i, n in enumerate(b.lengths):
+        b.k[i] = (b.k[i] * torch.linspace(0.1, 1.5, n)[None, :, None]).half()
+        for j in range(n):
+            b.k_pages[b.table[i, j // 16], :, j % 16] = b.k[i][:, j]
+    check_decode(pkg, with_room(b), b.rows(rows, scale=4.0))
+
+
+def test_many_rows_bad_page_is_reported(pkg):
+    b = with_room(oracle.Batch(74, [200, 90], [1, 1], 1, 1, 128, 16, "fp16"))
+    q = b.rows(24)
+    args = b.cuda()
+    want = pkg.attention_decode(q.cuda(), *args)
+    stream = torch.cuda.current_stream().cuda_stream
+    pkg.check(stream)
+    for bad in (-1, b.k_pages.shape[0], 2 ** 31 - 1):
+        table = args[2].clone()
+        table[0, 3] = bad
+        out = pkg.attention_decode(q.cuda(), args[0], args[1], table, args[3])
+        with pytest.raises(Exception):
+            pkg.check(stream)
+        assert torch.equal(out[1], want[1])
+        pkg.check(stream)
+
+
+def test_many_rows_on_two_streams_and_captured(pkg):
+    b = with_room(oracle.Batch(75, [900, 130, 0, 77], [2, 2, 0, 1], 2, 2, 64, 16, "fp16"))
+    q, args, counts = b.rows(40).cuda(), b.cuda(), b.cuda_counts()
+    want = pkg.attention_decode(q, *args, counts=counts)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = []
+    for i in range(6):
+        with torch.cuda.stream(streams[i % 2]):
+            outs.append(pkg.attention_decode(q, *args, counts=counts))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = pkg.attention_decode(q, *args, counts=counts)
+    args[3].copy_(torch.tensor([500, 1, 0, 77], dtype=torch.int32))
+    counts.copy_(torch.tensor([2, 1, 0, 1], dtype=torch.int32))
+    graph.replay()
+    later = pkg.attention_decode(q, *args, counts=counts)
+    pkg.check(torch.cuda.current_stream().cuda_stream)
+    assert all(torch.equal(x, want) for x in outs) and torch.equal(captured, later)
+
+
 @pytest.mark.parametrize("window", [0, 1, 63, 64, 200, 100000, 2 ** 31 - 1])
 @pytest.mark.parametrize("alibi", [False, True])
 def test_decode_window_and_alibi(pkg, window, alibi):

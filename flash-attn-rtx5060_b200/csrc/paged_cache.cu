@@ -261,7 +261,7 @@ int flash_decode(const fa_paged_cache* cache, const fa_rows* q, void* o, float* 
   p.cluster = decode_cluster(tiles, items, p.ctas);
   const bool wide = decode_wide(rows, items * tiles / p.ctas);
   if (wide && p.cluster > 1) p.cluster = 0;
-  p.item_units = wide ? 4 : 1;
+  p.item_units = wide ? 6 : 1;
   p.part_o = static_cast<float*>(workspace);
   p.part_ml = p.part_o + static_cast<size_t>(2) * p.ctas * p.part_rows * cache->head_dim;
   p.status = s->status;

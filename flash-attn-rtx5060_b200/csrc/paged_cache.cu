@@ -17,9 +17,9 @@ int decode_ctas(long long rows) { return rows <= 16 ? 296 : 148; }
 int part_rows(long long rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
 // Whether decode_wide_kernel takes a call: it starts and ends an item later by 5 us together, and takes half as long over a tile.
 // `work`: tiles of keys a CTA, if all sequences were as long as they may be. us, decode_kernel -> decode_wide_kernel, 16 sequences
-// on 8 key heads: 64 rows d128 x 512 26.6 -> 29.6, x 1024 (14 tiles a CTA) 36.8 -> 33.9, x 4096 93 -> 68, up to 32768 352 -> 209;
+// on 8 key heads: 64 rows d128 x 512 26.6 -> 29.6, x 1024 (14 tiles a CTA) 36.1 -> 33.5, x 4096 93 -> 67, up to 32768 352 -> 209;
 // 32 rows d128 x 4096 (55) 58.8 -> 60.5, up to 32768 220 -> 198; 32 rows d64 x 4096 (28) 38.3 -> 36.7; and 2048 tokens of
-// 32 heads on 8 over 8192 keys 1270 -> 404, 4 x 256 tokens 395 -> 153.
+// 32 heads on 8 over 8192 keys 1271 -> 404, 4 x 256 tokens 395 -> 147.
 bool decode_wide(long long rows, long long work) { return rows > 64 || (rows > 16 && work >= (rows > 32 ? 10 : 48)); }
 constexpr long long kJoinBlocks = 148 * 6;
 // CTAs of a cluster that takes an item (a sequence, key head and tile of rows) of up to `tiles` tiles of keys as a whole, 1 for

@@ -11,15 +11,20 @@ struct WideCfg {
   static constexpr int kRows = 128;
   static constexpr int kKeys = kDecodeKeys<D>;
   static constexpr int kPanelBytes = kKeys * 128, kHalfBytes = kKeys * D * 2;  // 64 columns of a tile; K or V of a tile
+  // Tiles whose scores have a place. At head_dim 64 a third is worth 10-13 % (16 x 8 tokens, 64 heads on 8, up to 32768: 160 ->
+  // 138 us): the scores of a group's next tile are there before its P is done. At head_dim 128, where a tile's scores are half as
+  // many and each tile held back is one less on its way, three or four cost such calls 2-4 %, and looking for what can be done next
+  // costs more than it finds (2048 tokens over 8192 keys 404 -> 480).
+  static constexpr int kRegions = D == 128 ? 2 : 3;
   static constexpr int kQBytes = kRows * D * 2;
   static constexpr int kStages = D == 128 ? 5 : 6;
   static constexpr int kOffRing = 2 * kQBytes;  // behind Q of this item and of the next
   static constexpr int kOffMl = kOffRing + kStages * 2 * kHalfBytes;
   static constexpr int kOffBars = kOffMl + 2 * kRows * 8;
-  static constexpr int kNumBars = 2 * kStages + 9;
+  static constexpr int kNumBars = 2 * kStages + kRegions + 11;
   static constexpr int kSmemBytes = kOffBars + kNumBars * 8 + 16;
   // tensor memory: scores of either group of softmax warps, in which P takes their place, and its O
-  static constexpr uint32_t kColO = 256;
+  static constexpr uint32_t kColO = kRegions * kKeys;
   static constexpr float kLazy = 8.f;
   static constexpr int kMaxCopies = kKeys / 32;
 };
@@ -46,11 +51,12 @@ decode_wide_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + Cfg::kOffBars);
   uint64_t* empty = full + Cfg::kStages;
-  uint64_t* s_full = empty + Cfg::kStages;  // two, for either group
-  uint64_t* o_full = s_full + 2;
-  uint64_t* q_full = s_full + 3;            // two of each from here on
-  uint64_t* q_empty = s_full + 5;
-  uint64_t* p_ready = s_full + 7;
+  uint64_t* s_full = empty + Cfg::kStages;  // one a region
+  uint64_t* o_full = s_full + Cfg::kRegions;
+  uint64_t* o_done = o_full + 1;            // two, of either group: a product has been summed
+  uint64_t* q_full = o_full + 3;            // two
+  uint64_t* q_empty = o_full + 5;           // two
+  uint64_t* p_ready = o_full + 7;           // of tile i the (i % 4)th: a warp may be a tile of its group ahead of another
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(full + Cfg::kNumBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   // (shuffles: the compiler then sees that the issuing warp's operands are uniform)
@@ -84,10 +90,9 @@ decode_wide_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
     const int copies = rows <= Cfg::kRows / Cfg::kMaxCopies ? Cfg::kMaxCopies : rows <= Cfg::kRows / 2 ? 2 : 1;
     const int copy_rows = Cfg::kRows / copies, copy = in_tile / copy_rows;
     const int chunks = Cfg::kKeys / 32 / copies, first_chunk = copy * chunks;  // 32 keys of a tile each: this thread's
-    const uint32_t t_s = tmem_addr(tmem, (warp & 3) * 32, group * Cfg::kKeys);
     const uint32_t t_o = tmem_addr(tmem, (warp & 3) * 32, Cfg::kColO);  // of group 0
     float2* ml = reinterpret_cast<float2*>(smem + Cfg::kOffMl);         // [group][row]
-    uint32_t s_at = 0, o_at = 0, q_at = 0;
+    uint32_t s_at = 0, done_at = 0, o_at = 0, q_at = 0;  // parities at the start of the item; s_at: a bit a region
     int loaded = 0;  // tiles of the items before
     while (walk.next(p, kv_head, row_tile, t0, t1)) {
       const int n = t1 - t0, r = row_tile * Cfg::kRows + in_tile % copy_rows;
@@ -103,8 +108,9 @@ decode_wide_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         // does every row see every key of the tile?
         const bool cut = key0 + Cfg::kKeys > first_query + 1 ||
                          (p.window_left >= 0 && key0 < walk.length - 1 - p.window_left);
-        ok &= mbar_wait(s_full + group, s_at, abort_flag);
-        s_at ^= 1;
+        const int region = i % Cfg::kRegions;
+        const uint32_t t_s = tmem_addr(tmem, (warp & 3) * 32, region * Cfg::kKeys);
+        ok &= mbar_wait(s_full + region, (s_at >> region ^ i / Cfg::kRegions) & 1, abort_flag);
         tc_fence_after();
         if (cut) {
           // what lies behind the last token, or in pages in front of the window, is not the sequence's: any bits at all, and
@@ -163,7 +169,11 @@ decode_wide_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
             const float alpha = grown ? ex2_approx(m - top) : 1.f;
             if (grown) m = top;
             l *= alpha;
-            if (i >= 2) {  // (the product before has been summed: S came behind it)
+            if (i >= 2) {
+              if (Cfg::kRegions > 2) {  // the group's last product has to be summed (else S came behind it)
+                ok &= mbar_wait(o_done + group, (done_at ^ i / 2 ^ 1) & 1, abort_flag);
+                tc_fence_after();
+              }
 #pragma unroll 1
               for (int c = 0; c < D; c += 32) {
                 uint32_t o[32];
@@ -205,9 +215,12 @@ decode_wide_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         }
         tc_fence_before();
         __syncwarp();
-        mbar_arrive_lane0(p_ready + group, lane);
+        mbar_arrive_lane0(p_ready + i % 4, lane);
       }
       loaded += n;
+#pragma unroll
+      for (int r = 0; r < Cfg::kRegions; ++r) s_at ^= ((n + Cfg::kRegions - 1 - r) / Cfg::kRegions & 1) << r;
+      done_at ^= (n + 1 - group) / 2 & 1;
 
       const bool whole = t0 == 0 && t1 == walk.tiles;
       const long long out_row = (static_cast<long long>(walk.b) * p.q_heads + head) * p.cache.tokens + t;
@@ -319,18 +332,27 @@ decode_wide_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
       ok &= mbar_wait(bar, parity, abort_flag);
       tc_fence_after();
     };
-    int s_stage = 0, o_stage = 0;
+    int s_stage = 0, o_stage = 0, q_buffer = 0;
     uint32_t s_phase = 0, q_phase = 0, p_at = 0, q = q_first;
-    int q_buffer = 0;
-    auto scores = [&](int group) {
-      wait(full + s_stage, s_phase);
+    auto scores = [&](int region) {  // of the next tile, which is there
       const uint32_t k = ring + s_stage * (2 * Cfg::kHalfBytes >> 4);
 #pragma unroll
       for (int h = 0; h < D / 64; ++h)
-        umma_qk64(tmem + group * Cfg::kKeys, (q + h * (Cfg::kRows * 128 >> 4)) | kKMajor,
+        umma_qk64(tmem + region * Cfg::kKeys, (q + h * (Cfg::kRows * 128 >> 4)) | kKMajor,
                   (k + h * (Cfg::kPanelBytes >> 4)) | kKMajor, kDescHi, idesc_s, h);
-      umma_commit_warp(s_full + group);
+      umma_commit_warp(s_full + region);
       if (++s_stage == Cfg::kStages) s_stage = 0, s_phase ^= 1;
+    };
+    auto product = [&](int i, int region) {
+      const int group = i & 1;
+      const uint32_t v = ring + (o_stage * 2 * Cfg::kHalfBytes + Cfg::kHalfBytes >> 4);
+#pragma unroll
+      for (int c = 0; c < Cfg::kKeys / 64; ++c)
+        umma_x64(tmem + Cfg::kColO + group * D, tmem + region * Cfg::kKeys + 64 * c, (v + c * (64 * 128 >> 4)) | kMnMajor, kDescHi,
+                 idesc_o, i >= 2 || c > 0);
+      umma_commit_warp(empty + o_stage);
+      if (Cfg::kRegions > 2) umma_commit_warp(o_done + group);
+      if (++o_stage == Cfg::kStages) o_stage = 0;
     };
     while (ok && walk.next(p, kv_head, row_tile, t0, t1)) {
       const int n = t1 - t0;
@@ -338,21 +360,50 @@ decode_wide_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
       wait(q_full + q_buffer, q_phase);
       q = q_first + q_buffer * (Cfg::kQBytes >> 4);
       if (q_buffer ^= 1; q_buffer == 0) q_phase ^= 1;
-      scores(0);
-      if (n > 1) scores(1);
-      for (int i = 0; i < n && ok; ++i) {
-        const int group = i & 1;
-        wait(p_ready + group, p_at >> group & 1u);
-        p_at ^= 1u << group;
-        const uint32_t v = ring + (o_stage * 2 * Cfg::kHalfBytes + Cfg::kHalfBytes >> 4);
-#pragma unroll
-        for (int c = 0; c < Cfg::kKeys / 64; ++c)
-          umma_x64(tmem + Cfg::kColO + group * D, tmem + group * Cfg::kKeys + 64 * c, (v + c * (64 * 128 >> 4)) | kMnMajor, kDescHi,
-                   idesc_o, i >= 2 || c > 0);
-        umma_commit_warp(empty + o_stage);
-        if (++o_stage == Cfg::kStages) o_stage = 0;
-        if (i + 2 < n) scores(group);
-        ok = __all_sync(0xffffffffu, ok);
+      // (S goes where the P of a product in front of it was)
+      if constexpr (Cfg::kRegions == 2) {
+        for (int i = 0; i < 2 && i < n; ++i) {
+          wait(full + s_stage, s_phase);
+          scores(i);
+        }
+        for (int i = 0; i < n && ok; ++i) {
+          wait(p_ready + i % 4, p_at >> i % 4 & 1u);
+          p_at ^= 1u << i % 4;
+          product(i, i & 1);
+          if (i + 2 < n) {
+            wait(full + s_stage, s_phase);
+            scores(i & 1);
+          }
+          ok = __all_sync(0xffffffffu, ok);
+        }
+      } else {
+        // S of as many tiles ahead as there are regions, each once its tile is there; O in the tiles' order, each once its P is
+        // there; whichever can be done next
+        int s_next = 0, polls = 0;
+        for (int i = 0; i < n && ok;) {
+          const int p_bar = i % 4;
+          const bool ahead = s_next < min(n, i + Cfg::kRegions);
+          if (ahead && __all_sync(0xffffffffu, mbar_test(full + s_stage, s_phase))) {
+            tc_fence_after();
+            scores(s_next % Cfg::kRegions);
+            ++s_next;
+            polls = 0;
+          } else if (i < s_next && __all_sync(0xffffffffu, mbar_test(p_ready + p_bar, p_at >> p_bar & 1u))) {
+            tc_fence_after();
+            p_at ^= 1u << p_bar;
+            product(i, i % Cfg::kRegions);
+            ++i;
+            polls = 0;
+          } else if (!ahead) {  // only P can come
+            ok = mbar_wait_warp(p_ready + p_bar, p_at >> p_bar & 1u, abort_flag);
+          } else {
+            __nanosleep(40);  // (the softmax warps beside this one need the issue slots)
+            if ((++polls & 63) == 0) {
+              if (polls >= FA_WAIT_LIMIT_POLLS) *abort_flag = 1;
+              ok = __all_sync(0xffffffffu, *abort_flag == 0);
+            }
+          }
+        }
       }
       umma_commit_warp(o_full);
     }

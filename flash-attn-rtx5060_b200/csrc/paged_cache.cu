@@ -146,6 +146,71 @@ int launch_rows(long long rows, bool wide, const fa_paged_cache* c, const fa::De
                       : launch_narrow<T, D, 4>(c, p, st, early);
 }
 
+int decode(const fa_paged_cache* cache, const fa_rows* q, void* o, float* lse, int batch, int tokens, int q_heads,
+           float softmax_scale, int window_left, const float* alibi_slopes, void* workspace, size_t workspace_bytes, void* stream,
+           int withhold) {
+  int rc = check_cache(cache, batch, tokens, q_heads);
+  if (rc != FA_OK) return rc;
+  if (q_heads <= 0) return fail(FA_INVALID_ARG, "q_heads must be positive");
+  if ((rc = check_rows(q, batch, q_heads, tokens)) != FA_OK) return rc;
+  if (!o || (reinterpret_cast<uintptr_t>(o) & 15)) return fail(FA_INVALID_ARG, "o must be there and 16-byte aligned");
+  if ((reinterpret_cast<uintptr_t>(lse) | reinterpret_cast<uintptr_t>(alibi_slopes)) & 3)
+    return fail(FA_INVALID_ARG, "lse and alibi_slopes must be 4-byte aligned");
+  if ((rc = check_scale(softmax_scale)) != FA_OK) return rc;
+  const long long rows = static_cast<long long>(q_heads / cache->kv_heads) * tokens;
+  if (static_cast<double>(batch) * q_heads * tokens > 0x7fffffff - 256)  // (so are a key head's rows, filled up to row tiles)
+    return fail(FA_INVALID_ARG, "too many rows");
+  if (!workspace || workspace_bytes < flash_decode_workspace_bytes(tokens, q_heads, cache->kv_heads, cache->head_dim))
+    return fail(FA_INVALID_ARG, "workspace is null or smaller than flash_decode_workspace_bytes()");
+  if (reinterpret_cast<uintptr_t>(workspace) & 15) return fail(FA_INVALID_ARG, "workspace must be 16-byte aligned");
+
+  DeviceState* s = nullptr;
+  bool captured = false;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if ((rc = device_state_for(st, &s, &captured)) != FA_OK) return rc;
+  if (!s->is_sm100) return fail(FA_UNSUPPORTED, "this library runs on compute capability 10.x (B200) only");
+  if (softmax_scale <= 0.f) softmax_scale = 1.0f / sqrtf(static_cast<float>(cache->head_dim));
+
+  fa::DecodeParams p;
+  memset(&p, 0, sizeof(p));
+  p.cache = view_of(cache, batch, tokens, s);
+  p.q = rows_of(q);
+  p.o = o;
+  p.lse = lse;
+  p.q_heads = q_heads;
+  p.group = q_heads / cache->kv_heads;
+  p.scale_log2 = softmax_scale * 1.4426950408889634f;
+  p.window_left = window_left;
+  p.alibi_slopes = alibi_slopes;
+  p.box_rows = cache->page_size & -cache->page_size;
+  const int tile_keys = cache->head_dim == 128 ? fa::kDecodeKeys<128> : fa::kDecodeKeys<64>;
+  if (p.box_rows > tile_keys) p.box_rows = tile_keys;
+  p.tile_shift = cache->head_dim == 128 ? 6 : 7;
+  p.part_rows = part_rows(rows);
+  p.row_tiles = static_cast<int>((rows + p.part_rows - 1) / p.part_rows);
+  p.ctas = decode_ctas(rows);
+  long long longest = static_cast<long long>(cache->max_pages) * cache->page_size;  // keys that an item may have
+  if (window_left >= 0 && longest > static_cast<long long>(window_left) + tokens)
+    longest = static_cast<long long>(window_left) + tokens;
+  const long long tiles = (longest + tile_keys - 1) / tile_keys + (window_left >= 0);
+  const long long items = static_cast<long long>(batch) * cache->kv_heads * p.row_tiles;
+  if (static_cast<double>(items) * (tiles + 8) > 0x7fffffff - 512)
+    return fail(FA_INVALID_ARG, "more tiles of keys than 31 bits count");
+  p.cluster = decode_cluster(tiles, items, p.ctas);
+  const bool wide = decode_wide(rows, items * tiles / p.ctas);
+  if (wide && p.cluster > 1) p.cluster = 0;
+  p.item_units = wide ? 6 : 1;
+  p.part_o = static_cast<float*>(workspace);
+  p.part_ml = p.part_o + static_cast<size_t>(2) * p.ctas * p.part_rows * cache->head_dim;
+  p.status = s->status;
+  p.withhold = withhold;
+  if (cache->dtype == FA_FP16)
+    return cache->head_dim == 64 ? launch_rows<__half, 64>(rows, wide, cache, p, st, !captured)
+                                 : launch_rows<__half, 128>(rows, wide, cache, p, st, !captured);
+  return cache->head_dim == 64 ? launch_rows<__nv_bfloat16, 64>(rows, wide, cache, p, st, !captured)
+                               : launch_rows<__nv_bfloat16, 128>(rows, wide, cache, p, st, !captured);
+}
+
 }  // namespace
 
 extern "C" {
@@ -211,65 +276,18 @@ size_t flash_decode_workspace_bytes(int tokens, int q_heads, int kv_heads, int h
 int flash_decode(const fa_paged_cache* cache, const fa_rows* q, void* o, float* lse, int batch, int tokens, int q_heads,
                  float softmax_scale, int window_left, const float* alibi_slopes, void* workspace, size_t workspace_bytes,
                  void* stream) {
-  int rc = check_cache(cache, batch, tokens, q_heads);
-  if (rc != FA_OK) return rc;
-  if (q_heads <= 0) return fail(FA_INVALID_ARG, "q_heads must be positive");
-  if ((rc = check_rows(q, batch, q_heads, tokens)) != FA_OK) return rc;
-  if (!o || (reinterpret_cast<uintptr_t>(o) & 15)) return fail(FA_INVALID_ARG, "o must be there and 16-byte aligned");
-  if ((reinterpret_cast<uintptr_t>(lse) | reinterpret_cast<uintptr_t>(alibi_slopes)) & 3)
-    return fail(FA_INVALID_ARG, "lse and alibi_slopes must be 4-byte aligned");
-  if ((rc = check_scale(softmax_scale)) != FA_OK) return rc;
-  const long long rows = static_cast<long long>(q_heads / cache->kv_heads) * tokens;
-  if (static_cast<double>(batch) * q_heads * tokens > 0x7fffffff - 64)  // (so are the rows of a key head)
-    return fail(FA_INVALID_ARG, "too many rows");
-  if (!workspace || workspace_bytes < flash_decode_workspace_bytes(tokens, q_heads, cache->kv_heads, cache->head_dim))
-    return fail(FA_INVALID_ARG, "workspace is null or smaller than flash_decode_workspace_bytes()");
-  if (reinterpret_cast<uintptr_t>(workspace) & 15) return fail(FA_INVALID_ARG, "workspace must be 16-byte aligned");
-
-  DeviceState* s = nullptr;
-  bool captured = false;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if ((rc = device_state_for(st, &s, &captured)) != FA_OK) return rc;
-  if (!s->is_sm100) return fail(FA_UNSUPPORTED, "this library runs on compute capability 10.x (B200) only");
-  if (softmax_scale <= 0.f) softmax_scale = 1.0f / sqrtf(static_cast<float>(cache->head_dim));
-
-  fa::DecodeParams p;
-  memset(&p, 0, sizeof(p));
-  p.cache = view_of(cache, batch, tokens, s);
-  p.q = rows_of(q);
-  p.o = o;
-  p.lse = lse;
-  p.q_heads = q_heads;
-  p.group = q_heads / cache->kv_heads;
-  p.scale_log2 = softmax_scale * 1.4426950408889634f;
-  p.window_left = window_left;
-  p.alibi_slopes = alibi_slopes;
-  p.box_rows = cache->page_size & -cache->page_size;
-  const int tile_keys = cache->head_dim == 128 ? fa::kDecodeKeys<128> : fa::kDecodeKeys<64>;
-  if (p.box_rows > tile_keys) p.box_rows = tile_keys;
-  p.tile_shift = cache->head_dim == 128 ? 6 : 7;
-  p.part_rows = part_rows(rows);
-  p.row_tiles = static_cast<int>((rows + p.part_rows - 1) / p.part_rows);
-  p.ctas = decode_ctas(rows);
-  long long longest = static_cast<long long>(cache->max_pages) * cache->page_size;  // keys that an item may have
-  if (window_left >= 0 && longest > static_cast<long long>(window_left) + tokens)
-    longest = static_cast<long long>(window_left) + tokens;
-  const long long tiles = (longest + tile_keys - 1) / tile_keys + (window_left >= 0);
-  const long long items = static_cast<long long>(batch) * cache->kv_heads * p.row_tiles;
-  if (static_cast<double>(items) * (tiles + 8) > 0x7fffffff - 512)
-    return fail(FA_INVALID_ARG, "more tiles of keys than 31 bits count");
-  p.cluster = decode_cluster(tiles, items, p.ctas);
-  const bool wide = decode_wide(rows, items * tiles / p.ctas);
-  if (wide && p.cluster > 1) p.cluster = 0;
-  p.item_units = wide ? 6 : 1;
-  p.part_o = static_cast<float*>(workspace);
-  p.part_ml = p.part_o + static_cast<size_t>(2) * p.ctas * p.part_rows * cache->head_dim;
-  p.status = s->status;
-  if (cache->dtype == FA_FP16)
-    return cache->head_dim == 64 ? launch_rows<__half, 64>(rows, wide, cache, p, st, !captured)
-                                 : launch_rows<__half, 128>(rows, wide, cache, p, st, !captured);
-  return cache->head_dim == 64 ? launch_rows<__nv_bfloat16, 64>(rows, wide, cache, p, st, !captured)
-                               : launch_rows<__nv_bfloat16, 128>(rows, wide, cache, p, st, !captured);
+  return decode(cache, q, o, lse, batch, tokens, q_heads, softmax_scale, window_left, alibi_slopes, workspace, workspace_bytes,
+                stream, 0);
 }
+
+#ifdef FA_TEST_WITHHOLD_LOAD
+// Test build only: sequence 0 never gets its last tile.
+int flash_decode_test_withhold(const fa_paged_cache* cache, const fa_rows* q, void* o, float* lse, int batch, int tokens,
+                               int q_heads, float softmax_scale, int window_left, const float* alibi_slopes, void* workspace,
+                               size_t workspace_bytes, void* stream) {
+  return decode(cache, q, o, lse, batch, tokens, q_heads, softmax_scale, window_left, alibi_slopes, workspace, workspace_bytes,
+                stream, 1);
+}
+#endif
 
 }  // extern "C"

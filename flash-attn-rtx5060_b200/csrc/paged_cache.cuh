@@ -190,6 +190,7 @@ struct DecodeParams {
   int part_rows;   // rows of a row tile
   int item_units;  // tiles of keys that an item's beginning and end take as long as
   int* status;
+  int withhold;    // test build only: sequence 0 never gets its last tile
 };
 
 // The work is one line of tiles of 32 KB: sequence by sequence, in each key head by key head (and row tile by row tile), the
@@ -393,8 +394,9 @@ __device__ __forceinline__ void compute_sync() {
 // what bounds it (at 16 rows a tile of 32 KB is 128 such instructions of an SM), and rows that are padding cost nothing that
 // matters: 64 sequences of up to 32768 tokens, 32 heads on 8 of 128, 4.8 GB in 704-741 us; one of 131072 in 89 us (6.0 TB/s, 5 of
 // them start and join). More than 16 rows leave the warps latency-bound (16 x 8 tokens, 64 heads on 8, up to 32768 tokens: 352 us
-// for 1.2 GB), so there decode_wide_kernel takes all but short work. Scores, maxima, sums and O are fp32; P is rounded to the cache's type for the second product, as the operand has to
-// be, half a step relative to the element, and its sum is taken unrounded.
+// for 1.2 GB), so there decode_wide_kernel takes all but short work. Scores, maxima, sums and O are fp32; P is rounded to the
+// cache's type for the second product, as the operand has to be, half a step relative to the element, and its sum is taken
+// unrounded.
 template <typename T, int D, int kRowWarps>
 __global__ void __launch_bounds__(DecodeCfg<D, kRowWarps>::kThreads, DecodeCfg<D, kRowWarps>::kCtasPerSm)
 decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
@@ -446,6 +448,9 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
         const unsigned here = __ballot_sync(0xffffffffu, page >= 0);
         if (lane == 0) mbar_arrive_expect_tx(full + stage, 2 * box_bytes * __popc(here));
         __syncwarp();
+#ifdef FA_TEST_WITHHOLD_LOAD
+        if (p.withhold && walk.b == 0 && t == walk.tiles - 1) page = -1;
+#endif
         if (page >= 0) {
           uint8_t* dst = smem + stage * 2 * Cfg::kHalfBytes + lane * box_bytes;
           const int row = ((walk.first + t) * Cfg::kKeys + lane * p.box_rows) % p.cache.page_size;

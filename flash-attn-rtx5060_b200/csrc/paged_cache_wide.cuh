@@ -399,7 +399,7 @@ decode_wide_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
           } else {
             __nanosleep(40);  // (the softmax warps beside this one need the issue slots)
             if ((++polls & 63) == 0) {
-              if (polls >= FA_WAIT_LIMIT_POLLS) *abort_flag = 1;
+              if (polls >= 16 * FA_WAIT_LIMIT_POLLS) *abort_flag = 1;  // 0.4 s
               ok = __all_sync(0xffffffffu, *abort_flag == 0);
             }
           }
@@ -434,10 +434,13 @@ decode_wide_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         for (int j = 0; j < at_once && t + j < t1; ++j) {
           ok = mbar_wait_warp(empty + stage, phase ^ 1, abort_flag);
           if (!ok) break;
-          const bool mine = of_tile == j && page >= 0;
+          bool mine = of_tile == j && page >= 0;
           const unsigned here = __ballot_sync(0xffffffffu, mine);
           if (lane == 0) mbar_arrive_expect_tx(full + stage, 2 * (D / 64) * box_bytes * __popc(here));
           __syncwarp();
+#ifdef FA_TEST_WITHHOLD_LOAD
+          if (p.withhold && walk.b == 0 && t + j == walk.tiles - 1) mine = false;
+#endif
           if (mine) {
             uint8_t* dst = smem + Cfg::kOffRing + stage * 2 * Cfg::kHalfBytes + box * box_bytes;
             const int row = ((walk.first + t + j) * Cfg::kKeys + box * p.box_rows) % p.cache.page_size;
@@ -451,8 +454,6 @@ decode_wide_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         }
       }
     }
-    if (!ok)
-      for (int i = 0; i < 64; ++i) __nanosleep(2000);  // loads in flight land before the CTA retires
   } else {
     // ---- Q of the next item: two warps, neighbouring lanes neighbouring pieces of a row ----
     const int rows = p.group * p.cache.tokens;
@@ -491,6 +492,8 @@ decode_wide_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
   tc_fence_before();
   __syncthreads();
   if (warp == Cfg::kSoftmaxWarps) tmem_dealloc(tmem, 512);
+  if (*abort_flag)
+    for (int i = 0; i < 64; ++i) __nanosleep(2000);  // loads in flight land before the CTA retires
 }
 
 }  // namespace fa

@@ -436,3 +436,35 @@ def test_on_two_streams(pkg):
                 outs.append(pkg.attention_decode(q, *args))
     torch.cuda.synchronize()
     assert all(torch.equal(x, want) for x in outs)
+
+
+@pytest.mark.parametrize("head_dim", [64, 128])
+@pytest.mark.parametrize("heads,room", [(8, False), (8, True), (40, False), (40, True), (100, True)])
+def test_wait_gives_up_and_the_device_stays_usable(pkg, heads, room, head_dim):
+    """Test build: a sequence never gets its last tile. The launch returns, the check reports it, the next call is right.
+    With and without room for long sequences: clusters, or the line of tiles; and a row's warps, or products of 128 rows."""
+    import ctypes
+
+    from test_wait_runs_out import load_waittest
+
+    L = load_waittest()
+    L.flash_decode.argtypes = L.flash_decode_test_withhold.argtypes = pkg.lib().flash_decode.argtypes
+    b = oracle.Batch(80, [900, 400], [1, 1], 1, 1, head_dim, 16, "fp16")
+    if room:
+        b = with_room(b)
+    q, args = b.rows(heads).cuda(), b.cuda()
+    want = pkg.attention_decode(q, *args)
+    stream = torch.cuda.current_stream().cuda_stream
+    pkg.check(stream)
+    cache = pkg._cache_struct(torch, *args, None)
+    rows = pkg._rows_struct("q", q, args[0], heads, 2, 1)
+    out = torch.zeros((2, heads, 1, head_dim), device="cuda", dtype=q.dtype)
+    nbytes = pkg.lib().flash_decode_workspace_bytes(1, heads, 1, head_dim)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device="cuda")
+    call = (cache, rows, out.data_ptr(), None, 2, 1, heads, 0.0, -1, None, ws.data_ptr(), ctypes.c_size_t(nbytes), stream)
+    assert L.flash_decode_test_withhold(*call) == pkg.FA_OK
+    assert L.flash_forward_check(stream) == pkg.FA_DEVICE_TIMEOUT
+    assert L.flash_forward_check(stream) == pkg.FA_OK
+    assert L.flash_decode(*call) == pkg.FA_OK
+    assert L.flash_forward_check(stream) == pkg.FA_OK
+    assert torch.equal(out, want)

@@ -325,7 +325,8 @@ int flash_cache_append(const fa_paged_cache* cache, const fa_rows* k, const fa_r
  * workspace: flash_decode_workspace_bytes() bytes of device memory, 16-byte aligned, with any contents; calls that may
  * overlap on the GPU need one each. Asynchronous on `stream`, one launch or two; may be captured into a CUDA graph once a call
  * has been made on the device. Two calls with the same arguments give the same bits; how a sequence's keys are shared out
- * depends on the lengths of the whole batch. */
+ * depends on the lengths of the whole batch and on max_pages. More than 16 rows (q_heads / kv_heads * tokens) run as matrix
+ * products of 128, which pay where contexts are long: max_pages should be no larger than the longest sequence needs. */
 int flash_decode(const fa_paged_cache* cache, const fa_rows* q, void* o, float* lse, int batch, int tokens, int q_heads,
                  float softmax_scale, int window_left, const float* alibi_slopes, void* workspace, size_t workspace_bytes,
                  void* stream);

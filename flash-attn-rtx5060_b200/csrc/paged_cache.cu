@@ -13,14 +13,16 @@ namespace {
 // CTAs of a call on a B200's 148 SMs: two a SM for up to 16 rows, else one (their rings of tiles keep 192 KB a SM in flight
 // either way). On a device with fewer SMs they run one after the other.
 int decode_ctas(long long rows) { return rows <= 16 ? 296 : 148; }
-// Rows (query heads of a key head times new tokens) of a row tile, of which a tile of keys is read once.
-int part_rows(long long rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
+// Rows (query heads of a key head times new tokens) of a row tile, of which a tile of keys is read once: 64 at most in
+// decode_kernel, 128 in decode_wide_kernel.
+int part_rows(long long rows, bool wide) { return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 || !wide ? 64 : 128; }
 // Whether decode_wide_kernel takes a call: it starts and ends an item later by 5 us together, and takes half as long over a tile.
 // `work`: tiles of keys a CTA, if all sequences were as long as they may be. us, decode_kernel -> decode_wide_kernel, 16 sequences
 // on 8 key heads: 64 rows d128 x 512 26.6 -> 29.6, x 1024 (14 tiles a CTA) 36.1 -> 33.5, x 4096 93 -> 67, up to 32768 352 -> 209;
 // 32 rows d128 x 4096 (55) 58.8 -> 60.5, up to 32768 220 -> 198; 32 rows d64 x 4096 (28) 38.3 -> 36.7; and 2048 tokens of
-// 32 heads on 8 over 8192 keys 1271 -> 404, 4 x 256 tokens 395 -> 147.
-bool decode_wide(long long rows, long long work) { return rows > 64 || (rows > 16 && work >= (rows > 32 ? 10 : 48)); }
+// 32 heads on 8 over 8192 keys 1271 -> 404, 4 x 256 tokens 395 -> 147; but 128 rows d64 x 512 (3) 21.9 -> 28.8, 400 rows x 512 (1)
+// 12.7 -> 17.8.
+bool decode_wide(long long rows, long long work) { return rows > 16 && work >= (rows > 64 ? 5 : rows > 32 ? 10 : 48); }
 constexpr long long kJoinBlocks = 148 * 6;
 // CTAs of a cluster that takes an item (a sequence, key head and tile of rows) of up to `tiles` tiles of keys as a whole, 1 for
 // a CTA alone, or 0 where the items are cut by the line and joined by a second launch (which takes as long as four tiles or
@@ -186,18 +188,20 @@ int decode(const fa_paged_cache* cache, const fa_rows* q, void* o, float* lse, i
   const int tile_keys = cache->head_dim == 128 ? fa::kDecodeKeys<128> : fa::kDecodeKeys<64>;
   if (p.box_rows > tile_keys) p.box_rows = tile_keys;
   p.tile_shift = cache->head_dim == 128 ? 6 : 7;
-  p.part_rows = part_rows(rows);
-  p.row_tiles = static_cast<int>((rows + p.part_rows - 1) / p.part_rows);
   p.ctas = decode_ctas(rows);
   long long longest = static_cast<long long>(cache->max_pages) * cache->page_size;  // keys that an item may have
   if (window_left >= 0 && longest > static_cast<long long>(window_left) + tokens)
     longest = static_cast<long long>(window_left) + tokens;
   const long long tiles = (longest + tile_keys - 1) / tile_keys + (window_left >= 0);
-  const long long items = static_cast<long long>(batch) * cache->kv_heads * p.row_tiles;
+  const auto row_tiles = [&](int of) { return (rows + of - 1) / of; };
+  const long long heads = static_cast<long long>(batch) * cache->kv_heads;
+  const bool wide = decode_wide(rows, heads * row_tiles(128) * tiles / p.ctas);
+  p.part_rows = part_rows(rows, wide);
+  p.row_tiles = static_cast<int>(row_tiles(p.part_rows));
+  const long long items = heads * p.row_tiles;
   if (static_cast<double>(items) * (tiles + 8) > 0x7fffffff - 512)
     return fail(FA_INVALID_ARG, "more tiles of keys than 31 bits count");
   p.cluster = decode_cluster(tiles, items, p.ctas);
-  const bool wide = decode_wide(rows, items * tiles / p.ctas);
   if (wide && p.cluster > 1) p.cluster = 0;
   p.item_units = wide ? 6 : 1;
   p.part_o = static_cast<float*>(workspace);
@@ -270,7 +274,7 @@ int flash_cache_append(const fa_paged_cache* cache, const fa_rows* k, const fa_r
 size_t flash_decode_workspace_bytes(int tokens, int q_heads, int kv_heads, int head_dim) {
   if (tokens <= 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads != 0 || head_dim <= 0) return 0;
   const long long rows = static_cast<long long>(q_heads / kv_heads) * tokens;
-  return static_cast<size_t>(2) * decode_ctas(rows) * part_rows(rows) * (head_dim + 2) * sizeof(float);
+  return static_cast<size_t>(2) * decode_ctas(rows) * part_rows(rows, true) * (head_dim + 2) * sizeof(float);
 }
 
 int flash_decode(const fa_paged_cache* cache, const fa_rows* q, void* o, float* lse, int batch, int tokens, int q_heads,

@@ -2,6 +2,7 @@
 #include <cmath>
 #include <cstring>
 
+#include "decode_plan.h"
 #include "host.h"
 #include "paged_cache.cuh"
 #include "paged_cache_wide.cuh"
@@ -10,31 +11,7 @@ using namespace fa_host;
 
 namespace {
 
-// CTAs of a call on a B200's 148 SMs: two a SM for up to 16 rows, else one (their rings of tiles keep 192 KB a SM in flight
-// either way). On a device with fewer SMs they run one after the other.
-int decode_ctas(long long rows) { return rows <= 16 ? 296 : 148; }
-// Rows (query heads of a key head times new tokens) of a row tile, of which a tile of keys is read once: 64 at most in
-// decode_kernel, 128 in decode_wide_kernel.
-int part_rows(long long rows, bool wide) { return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 || !wide ? 64 : 128; }
-// Whether decode_wide_kernel takes a call: it starts and ends an item later by 5 us together, and takes half as long over a tile.
-// `work`: tiles of keys a CTA, if all sequences were as long as they may be. us, decode_kernel -> decode_wide_kernel, 16 sequences
-// on 8 key heads: 64 rows d128 x 512 26.6 -> 29.6, x 1024 (14 tiles a CTA) 36.1 -> 33.5, x 4096 93 -> 67, up to 32768 352 -> 209;
-// 32 rows d128 x 4096 (55) 58.8 -> 60.5, up to 32768 220 -> 198; 32 rows d64 x 4096 (28) 38.3 -> 36.7; and 2048 tokens of
-// 32 heads on 8 over 8192 keys 1271 -> 404, 4 x 256 tokens 395 -> 147; but 128 rows d64 x 512 (3) 21.9 -> 28.8, 400 rows x 512 (1)
-// 12.7 -> 17.8.
-bool decode_wide(long long rows, long long work) { return rows > 16 && work >= (rows > 64 ? 5 : rows > 32 ? 10 : 48); }
 constexpr long long kJoinBlocks = 148 * 6;
-// CTAs of a cluster that takes an item (a sequence, key head and tile of rows) of up to `tiles` tiles of keys as a whole, 1 for
-// a CTA alone, or 0 where the items are cut by the line and joined by a second launch (which takes as long as four tiles or
-// five). An item of two tiles has a CTA; short items of a large batch fill the SMs by their number; fewer items have clusters of
-// up to eight CTAs, where a CTA's tiles are not many more than if the line had cut them, and uneven lengths cannot cost much.
-// us, cut -> not cut (sequences x longest, key heads, head_dim): 1 x 512, 4, 64 8.6 -> 6.5; 1 x 512, 8, 128 8.2 -> 6.8;
-// 1 x 2048, 8, 128 9.5 -> 9.1; 4 x 2048, 8, 128 11.7 -> 10.2; 128 x 400, 8, 128 48.5 -> 34.5; but 1 x 4096, 4, 64 8.8 -> 9.7.
-int decode_cluster(long long tiles, long long items, int ctas) {
-  if (tiles <= 2 || (tiles <= 8 && items >= ctas)) return 1;
-  if (8 * items > ctas || tiles > 64 || tiles * (ctas - 8 * items) > 26ll * ctas) return 0;
-  return tiles <= 4 ? 4 : 8;
-}
 
 int check_cache(const fa_paged_cache* c, int batch, int tokens, int q_heads) {
   if (!c) return fail(FA_INVALID_ARG, "cache is null");
@@ -140,12 +117,12 @@ int launch_narrow(const fa_paged_cache* c, const fa::DecodeParams& p, cudaStream
 }
 
 template <typename T, int D>
-int launch_rows(long long rows, bool wide, const fa_paged_cache* c, const fa::DecodeParams& p, cudaStream_t st, bool early) {
+int launch_rows(const fa::DecodePlan& plan, const fa_paged_cache* c, const fa::DecodeParams& p, cudaStream_t st, bool early) {
   using Cfg = fa::WideCfg<D>;
-  if (wide) return launch_decode<T, D>(fa::decode_wide_kernel<T, D>, Cfg::kThreads, Cfg::kSmemBytes, c, 1, p, st, early);
-  return rows <= 16   ? launch_narrow<T, D, 1>(c, p, st, early)
-         : rows <= 32 ? launch_narrow<T, D, 2>(c, p, st, early)
-                      : launch_narrow<T, D, 4>(c, p, st, early);
+  if (plan.wide) return launch_decode<T, D>(fa::decode_wide_kernel<T, D>, Cfg::kThreads, Cfg::kSmemBytes, c, 1, p, st, early);
+  return plan.part_rows == 16   ? launch_narrow<T, D, 1>(c, p, st, early)
+         : plan.part_rows == 32 ? launch_narrow<T, D, 2>(c, p, st, early)
+                                : launch_narrow<T, D, 4>(c, p, st, early);
 }
 
 int decode(const fa_paged_cache* cache, const fa_rows* q, void* o, float* lse, int batch, int tokens, int q_heads,
@@ -159,7 +136,6 @@ int decode(const fa_paged_cache* cache, const fa_rows* q, void* o, float* lse, i
   if ((reinterpret_cast<uintptr_t>(lse) | reinterpret_cast<uintptr_t>(alibi_slopes)) & 3)
     return fail(FA_INVALID_ARG, "lse and alibi_slopes must be 4-byte aligned");
   if ((rc = check_scale(softmax_scale)) != FA_OK) return rc;
-  const long long rows = static_cast<long long>(q_heads / cache->kv_heads) * tokens;
   if (static_cast<double>(batch) * q_heads * tokens > 0x7fffffff - 256)  // (so are a key head's rows, filled up to row tiles)
     return fail(FA_INVALID_ARG, "too many rows");
   if (!workspace || workspace_bytes < flash_decode_workspace_bytes(tokens, q_heads, cache->kv_heads, cache->head_dim))
@@ -188,31 +164,24 @@ int decode(const fa_paged_cache* cache, const fa_rows* q, void* o, float* lse, i
   const int tile_keys = cache->head_dim == 128 ? fa::kDecodeKeys<128> : fa::kDecodeKeys<64>;
   if (p.box_rows > tile_keys) p.box_rows = tile_keys;
   p.tile_shift = cache->head_dim == 128 ? 6 : 7;
-  p.ctas = decode_ctas(rows);
-  long long longest = static_cast<long long>(cache->max_pages) * cache->page_size;  // keys that an item may have
-  if (window_left >= 0 && longest > static_cast<long long>(window_left) + tokens)
-    longest = static_cast<long long>(window_left) + tokens;
-  const long long tiles = (longest + tile_keys - 1) / tile_keys + (window_left >= 0);
-  const auto row_tiles = [&](int of) { return (rows + of - 1) / of; };
-  const long long heads = static_cast<long long>(batch) * cache->kv_heads;
-  const bool wide = decode_wide(rows, heads * row_tiles(128) * tiles / p.ctas);
-  p.part_rows = part_rows(rows, wide);
-  p.row_tiles = static_cast<int>(row_tiles(p.part_rows));
-  const long long items = heads * p.row_tiles;
-  if (static_cast<double>(items) * (tiles + 8) > 0x7fffffff - 512)
+  const fa::DecodePlan plan = fa::decode_plan(batch, tokens, p.group, cache->kv_heads,
+                                              static_cast<long long>(cache->max_pages) * cache->page_size, window_left, tile_keys);
+  if (static_cast<double>(plan.items) * (plan.tiles + 8) > 0x7fffffff - 512)
     return fail(FA_INVALID_ARG, "more tiles of keys than 31 bits count");
-  p.cluster = decode_cluster(tiles, items, p.ctas);
-  if (wide && p.cluster > 1) p.cluster = 0;
-  p.item_units = wide ? 6 : 1;
+  p.ctas = plan.ctas;
+  p.part_rows = plan.part_rows;
+  p.row_tiles = static_cast<int>(plan.row_tiles);
+  p.cluster = plan.cluster;
+  p.item_units = plan.wide ? 6 : 1;
   p.part_o = static_cast<float*>(workspace);
   p.part_ml = p.part_o + static_cast<size_t>(2) * p.ctas * p.part_rows * cache->head_dim;
   p.status = s->status;
   p.withhold = withhold;
   if (cache->dtype == FA_FP16)
-    return cache->head_dim == 64 ? launch_rows<__half, 64>(rows, wide, cache, p, st, !captured)
-                                 : launch_rows<__half, 128>(rows, wide, cache, p, st, !captured);
-  return cache->head_dim == 64 ? launch_rows<__nv_bfloat16, 64>(rows, wide, cache, p, st, !captured)
-                               : launch_rows<__nv_bfloat16, 128>(rows, wide, cache, p, st, !captured);
+    return cache->head_dim == 64 ? launch_rows<__half, 64>(plan, cache, p, st, !captured)
+                                 : launch_rows<__half, 128>(plan, cache, p, st, !captured);
+  return cache->head_dim == 64 ? launch_rows<__nv_bfloat16, 64>(plan, cache, p, st, !captured)
+                               : launch_rows<__nv_bfloat16, 128>(plan, cache, p, st, !captured);
 }
 
 }  // namespace
@@ -274,7 +243,7 @@ int flash_cache_append(const fa_paged_cache* cache, const fa_rows* k, const fa_r
 size_t flash_decode_workspace_bytes(int tokens, int q_heads, int kv_heads, int head_dim) {
   if (tokens <= 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads != 0 || head_dim <= 0) return 0;
   const long long rows = static_cast<long long>(q_heads / kv_heads) * tokens;
-  return static_cast<size_t>(2) * decode_ctas(rows) * part_rows(rows, true) * (head_dim + 2) * sizeof(float);
+  return static_cast<size_t>(2) * fa::decode_ctas(rows) * fa::decode_part_rows(rows, true) * (head_dim + 2) * sizeof(float);
 }
 
 int flash_decode(const fa_paged_cache* cache, const fa_rows* q, void* o, float* lse, int batch, int tokens, int q_heads,

@@ -251,7 +251,8 @@ def host_workspace_bytes(seqlen, head_dim, chunk_heads):
 
 
 def check(stream=None):
-    """Waits for the stream and raises if a device-side wait gave up."""
+    """Waits for the stream and raises if a device-side wait gave up or an index in device memory was out of range (one of
+    the two a call)."""
     rc = lib().flash_forward_check(stream)
     if rc != FA_OK:
         _raise(rc)

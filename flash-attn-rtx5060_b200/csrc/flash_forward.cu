@@ -623,10 +623,12 @@ int flash_forward_check(void* stream) {
   if ((e = cudaMemcpy(host, s->status, sizeof(host), cudaMemcpyDeviceToHost)) != cudaSuccess)
     return fail_cuda("cudaMemcpy(status)", e);
   if (host[0] == 0 && host[1] == 0) return FA_OK;
-  // Only the status words are cleared: the scheduler words belong to launches that may still be running on other
-  // streams, and a kernel that gave up still leaves its own pair at zero (every CTA reaches the final count).
-  cudaMemset(s->status, 0, sizeof(host));
-  if (host[0] != 0) {
+  // Only the word that is reported is cleared: the other one is the next check's, and the scheduler words belong to launches that
+  // may still be running on other streams, and a kernel that gave up still leaves its own pair at zero (every CTA reaches the
+  // final count).
+  const int which = host[0] != 0 ? 0 : 1;
+  if ((e = cudaMemset(s->status + which, 0, sizeof(int))) != cudaSuccess) return fail_cuda("cudaMemset(status)", e);
+  if (which == 0) {
     snprintf(g_err, sizeof(g_err), "a wait inside the attention kernel ran out of time (status word %d)", host[0]);
     return FA_DEVICE_TIMEOUT;
   }

@@ -173,12 +173,13 @@ int flash_forward_host(const void* q_host, const void* k_host, const void* v_hos
                        int window_right, void* workspace, size_t workspace_bytes, int chunk_heads);
 size_t flash_forward_host_workspace_bytes(int seqlen, int head_dim, int chunk_heads);
 
-/* Waits for `stream`, then reads and clears the current device's status words. Returns FA_OK,
- * FA_DEVICE_TIMEOUT, FA_BAD_INDEX (flash_cache_append, flash_decode), or FA_CUDA_ERROR. Replaces the reference's CUDA_CHECK(cudaDeviceSynchronize())
- * + exit (src/flash_forward.h:654-655). There is ONE status word per device, not per stream: a
- * time-out raised by a launch on another stream of the device is reported (and consumed) by whichever
- * check comes first. Like flash_forward() it allocates the device's scratch on first use; hosts that
- * must not allocate use flash_forward_noalloc() and flash_forward_noalloc_check(). */
+/* Waits for `stream`, then reads the current device's status words: FA_OK, FA_DEVICE_TIMEOUT (a wait ran out),
+ * FA_BAD_INDEX (flash_cache_append, flash_decode), or FA_CUDA_ERROR. What is reported is cleared, one thing a call: where a
+ * wait ran out and an index was out of range too, the next call says so. Replaces the reference's
+ * CUDA_CHECK(cudaDeviceSynchronize()) + exit (src/flash_forward.h:654-655). The words are per device, not per stream: what
+ * a launch on another stream of the device raised is reported (and consumed) by whichever check comes first. Like
+ * flash_forward() it allocates the device's scratch on first use; hosts that must not allocate use flash_forward_noalloc()
+ * and flash_forward_noalloc_check(). */
 int flash_forward_check(void* stream);
 
 /* The reference's host entry point, positional argument for positional argument

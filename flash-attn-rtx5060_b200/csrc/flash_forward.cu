@@ -580,6 +580,33 @@ double flash_forward_dropout_keep_probability(float dropout_prob) {
   return keep_thr >= 256u ? 1.0 : keep_thr / 256.0;
 }
 
+// Waits for the stream and reports the first `words` of the status words: 2 for the caller's own check; 1, waits that ran out, for
+// the entry points that wait for a forward of theirs (an index that an earlier call on the cache met is not theirs to report, nor to
+// consume).
+static int check_words(void* stream, int words) {
+  DeviceState* s = nullptr;
+  int rc = device_state(&s);
+  if (rc != FA_OK) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  cudaError_t e = cudaStreamSynchronize(st);
+  if (e != cudaSuccess) return fail_cuda("cudaStreamSynchronize", e);
+  if (!s->status) return FA_OK;
+  int host[2] = {0, 0};
+  if ((e = cudaMemcpy(host, s->status, words * sizeof(int), cudaMemcpyDeviceToHost)) != cudaSuccess)
+    return fail_cuda("cudaMemcpy(status)", e);
+  if (host[0] == 0 && host[1] == 0) return FA_OK;
+  // Only the word that is reported is cleared: the other one is the next check's, and the scheduler words belong to launches that
+  // may still be running on other streams, and a kernel that gave up still leaves its own pair at zero (every CTA reaches the
+  // final count).
+  const int which = host[0] != 0 ? 0 : 1;
+  if ((e = cudaMemset(s->status + which, 0, sizeof(int))) != cudaSuccess) return fail_cuda("cudaMemset(status)", e);
+  if (which == 0) {
+    snprintf(g_err, sizeof(g_err), "a wait inside the attention kernel ran out of time (status word %d)", host[0]);
+    return FA_DEVICE_TIMEOUT;
+  }
+  return fail(FA_BAD_INDEX, "a page of a page table, a length, a count or a position in device memory was out of range");
+}
+
 int flash_forward_multi_gpu(int num_slabs, const int* devices, const void* const* q, const void* const* k,
                             const void* const* v, void* const* o, const int* slab_heads, int seqlen, int head_dim,
                             float softmax_scale, int is_causal, int window_left, int window_right,
@@ -605,35 +632,13 @@ int flash_forward_multi_gpu(int num_slabs, const int* devices, const void* const
   for (int i = 0; wait && i < num_slabs && rc == FA_OK; ++i) {
     if (slab_heads[i] == 0) continue;
     if ((e = cudaSetDevice(devices[i])) != cudaSuccess) { rc = fail_cuda("cudaSetDevice", e); break; }
-    rc = flash_forward_check(streams ? streams[i] : nullptr);
+    rc = check_words(streams ? streams[i] : nullptr, 1);
   }
   cudaSetDevice(prev);
   return rc;
 }
 
-int flash_forward_check(void* stream) {
-  DeviceState* s = nullptr;
-  int rc = device_state(&s);
-  if (rc != FA_OK) return rc;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  cudaError_t e = cudaStreamSynchronize(st);
-  if (e != cudaSuccess) return fail_cuda("cudaStreamSynchronize", e);
-  if (!s->status) return FA_OK;
-  int host[2] = {0, 0};
-  if ((e = cudaMemcpy(host, s->status, sizeof(host), cudaMemcpyDeviceToHost)) != cudaSuccess)
-    return fail_cuda("cudaMemcpy(status)", e);
-  if (host[0] == 0 && host[1] == 0) return FA_OK;
-  // Only the word that is reported is cleared: the other one is the next check's, and the scheduler words belong to launches that
-  // may still be running on other streams, and a kernel that gave up still leaves its own pair at zero (every CTA reaches the
-  // final count).
-  const int which = host[0] != 0 ? 0 : 1;
-  if ((e = cudaMemset(s->status + which, 0, sizeof(int))) != cudaSuccess) return fail_cuda("cudaMemset(status)", e);
-  if (which == 0) {
-    snprintf(g_err, sizeof(g_err), "a wait inside the attention kernel ran out of time (status word %d)", host[0]);
-    return FA_DEVICE_TIMEOUT;
-  }
-  return fail(FA_BAD_INDEX, "a page of a page table, a length, a count or a position in device memory was out of range");
-}
+int flash_forward_check(void* stream) { return check_words(stream, 2); }
 
 int run_flash_attention_c(int B, int N, int S, int d, void* Q, void* K, void* V, void* O, void* L, void* M,
                           int Is_dropout, int Is_causal, int Is_local, int Has_alibi, int window_size,
@@ -658,7 +663,7 @@ int run_flash_attention_c(int B, int N, int S, int d, void* Q, void* K, void* V,
   int rc = forward_impl(Q, K, V, O, B, N, S, d, 0.f, Is_causal, wl, wr, Has_alibi ? alibi_slopes : nullptr, nullptr, 0,
                         0, nullptr, nullptr, drop_p, seed);
   cudaEventRecord(t1, 0);
-  if (rc == FA_OK) rc = flash_forward_check(nullptr);
+  if (rc == FA_OK) rc = check_words(nullptr, 1);
   float ms = 0.f;
   if (rc == FA_OK && cudaEventSynchronize(t1) == cudaSuccess && cudaEventElapsedTime(&ms, t0, t1) == cudaSuccess)
     printf("TIME: %f\n", ms);
@@ -750,7 +755,7 @@ int flash_forward_host(const void* q_host, const void* k_host, const void* v_hos
   char saved[sizeof(g_err)];
   memcpy(saved, g_err, sizeof(saved));  // the message of a failed flash_forward() above
   const cudaError_t e_up = cudaStreamSynchronize(hp->up);
-  const int rc_run = flash_forward_check(hp->run);
+  const int rc_run = check_words(hp->run, 1);
   const cudaError_t e_down = cudaStreamSynchronize(hp->down);
   if (rc != FA_OK) {
     memcpy(g_err, saved, sizeof(saved));

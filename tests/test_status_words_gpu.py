@@ -45,3 +45,39 @@ def test_both_reports_are_given_one_after_the_other(pkg):
         assert L.flash_forward_check(stream) == pkg.FA_BAD_INDEX
         assert b"out of range" in L.flash_forward_last_error()
         assert L.flash_forward_check(stream) == pkg.FA_OK
+
+
+def test_calls_that_wait_for_their_own_forward_leave_the_report_of_an_index(pkg):
+    """The blocking forward calls check for a wait of theirs that ran out. A decode before them that met a page out of range is
+    none of theirs: they return FA_OK, and the check that follows the decode still has its report."""
+    L = pkg.lib()
+    stream = torch.cuda.current_stream().cuda_stream
+    b = oracle.Batch(3, [40], [1], 1, 2, 64, 16, "fp16")
+    args, rows = b.cuda(), b.rows(4).cuda()
+    args[2][0, 1] = -1
+    g = torch.Generator().manual_seed(4)
+    host = [torch.randn((1, 2, 200, 64), generator=g).half().contiguous() for _ in range(3)]
+    q, k, v = (x.cuda() for x in host)
+    want = pkg.attention_forward(q, k, v)
+    out_host, out = torch.zeros_like(host[0]), torch.zeros_like(q)
+    nbytes = L.flash_forward_host_workspace_bytes(200, 64, 2)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device="cuda")
+    one = ctypes.c_void_p * 1
+    calls = [
+        lambda: L.flash_forward_host(*(x.data_ptr() for x in host), out_host.data_ptr(), 1, 2, 200, 64, 0.0, 0, -1, -1,
+                                     ws.data_ptr(), nbytes, 2),
+        lambda: L.run_flash_attention_c(1, 2, 200, 64, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), None, None, 0, 0,
+                                        0, 0, 0, None, 0.0, None),
+        lambda: L.flash_forward_multi_gpu(1, (ctypes.c_int * 1)(torch.cuda.current_device()),
+                                          *(one(x.data_ptr()) for x in (q, k, v, out)), (ctypes.c_int * 1)(2), 200, 64, 0.0, 0,
+                                          -1, -1, None, 1),
+    ]
+    for call in calls:
+        pkg.check(stream)
+        out.zero_()
+        pkg.attention_decode(rows, *args)
+        torch.cuda.synchronize()
+        assert call() == pkg.FA_OK
+        assert torch.equal(out_host.cuda() if call is calls[0] else out, want)
+        assert L.flash_forward_check(stream) == pkg.FA_BAD_INDEX
+        assert L.flash_forward_check(stream) == pkg.FA_OK

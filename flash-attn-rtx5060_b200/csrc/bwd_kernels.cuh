@@ -11,7 +11,8 @@
 //
 // The operands of the second products are fp16, and P and dS of a long row are far below 1: P is kept as 2^14 P, and dS as
 // 2^14 P * (dO.v - delta) / 2^e with 2^e above the head's bound max|dO_i| max|v_j| + max|delta_i|, so that neither overflows
-// and a value is rounded to 11 bits down to 2^-28 of that bound (to 2^-25 of it in steps, below it is 0). The sums are fp32.
+// and a value is rounded to 11 bits down to 2^-28 of that bound (to 2^-39 of it in steps of 2^-38, below it is 0). Rows whose norms are
+// infinite or NaN are left out of the bound. The sums are fp32.
 #pragma once
 #include "fwd_params.h"
 #include "ptx.cuh"
@@ -70,6 +71,10 @@ __device__ __forceinline__ float warp_max(float x) {
   return x;
 }
 
+// A norm for the maxima: one that is infinite or NaN is left out. Its own row has no finite result whatever the scaling, and the
+// others' has to be that of their own sizes (an infinite bound once left dS of the whole head unscaled: it overflowed).
+__device__ __forceinline__ float bwd_norm(float x) { return x < INFINITY ? x : 0.f; }
+
 // 128 rows of a head a CTA. Reads O, dO and V once: bound by bytes where rows are many (B1 H16 N8192 d128: 101 MB in 21 us under
 // ncu, caches flushed), else by one round of loads and two reductions.
 template <int D>
@@ -87,9 +92,9 @@ __global__ void __launch_bounds__(1024) bwd_rows_kernel(const BwdParams p) {
     float delta, gg, vv;
     bwd_row<D>(p, head, r, lane, delta, gg, vv);
     if (r < p.seqlen && lane % (D / 8) == 0) p.delta[head * p.seqlen + r] = delta;
-    top[0] = fmaxf(top[0], gg);
-    top[1] = fmaxf(top[1], vv);
-    top[2] = fmaxf(top[2], fabsf(delta));
+    top[0] = fmaxf(top[0], bwd_norm(gg));
+    top[1] = fmaxf(top[1], bwd_norm(vv));
+    top[2] = fmaxf(top[2], bwd_norm(fabsf(delta)));
   }
 #pragma unroll
   for (int k = 0; k < 3; ++k) {
@@ -174,12 +179,12 @@ __device__ __forceinline__ int bwd_index(int k) {
   return k * static_cast<int>(gridDim.x) + static_cast<int>(k & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
 }
 
-// 2^-e (see the top of this file) from a lane's norms. A bound that is zero, infinite or NaN leaves dS as it is. All lanes of a
-// warp.
+// 2^-e (see the top of this file) from a lane's norms. A bound of zero leaves dS as it is; one beyond fp32 (norms are finite, their
+// sum need not be) is the largest. All lanes of a warp.
 __device__ __forceinline__ float bwd_unit(float g, float v, float d) {
   const float bound = fmaf(warp_max(g), warp_max(v), warp_max(d));
   const int exponent = static_cast<int>(__float_as_uint(bound) >> 23 & 255u);  // biased by 127
-  if (exponent == 0 || exponent == 255) return 1.f;
+  if (exponent == 0) return 1.f;
   return __uint_as_float(static_cast<uint32_t>(min(max(127 - (exponent - 126), 27), 227)) << 23);
 }
 
@@ -552,9 +557,9 @@ __device__ __forceinline__ void bwd_own_rows(const BwdParams& p, int bh, uint8_t
     float delta, gg, vv;
     bwd_row<D>(p, bh, r, lane, delta, gg, vv);
     if (r < p.seqlen && lane % (D / 8) == 0) delta_of[r] = delta;
-    top[0] = fmaxf(top[0], gg);
-    top[1] = fmaxf(top[1], vv);
-    top[2] = fmaxf(top[2], fabsf(delta));
+    top[0] = fmaxf(top[0], bwd_norm(gg));
+    top[1] = fmaxf(top[1], bwd_norm(vv));
+    top[2] = fmaxf(top[2], bwd_norm(fabsf(delta)));
   }
 #pragma unroll
   for (int k = 0; k < 3; ++k) {

@@ -10,9 +10,12 @@
 // that every sum stays in tensor memory, in one order: no atomics, no fp32 copy of dQ in HBM, the same bits every time.
 //
 // The operands of the second products are fp16, and P and dS of a long row are far below 1: P is kept as 2^14 P, and dS as
-// 2^14 P * (dO.v - delta) / 2^e with 2^e above the head's bound max|dO_i| max|v_j| + max|delta_i|, so that neither overflows
-// and a value is rounded to 11 bits down to 2^-28 of that bound (to 2^-39 of it in steps of 2^-38, below it is 0). Rows whose norms are
-// infinite or NaN are left out of the bound. The sums are fp32.
+// 2^14 P * (dO.v - delta) / 2^e with 2^e above a bound of what follows P, so that neither overflows and a value is rounded to 11
+// bits down to 2^-28 of the bound (to 2^-39 of it in steps of 2^-38, below it is 0). For dQ the bound is a row's own, |dO_i| max|v_j| +
+// |delta_i| over the keys that its 128 rows see; for dK, whose sums run over the queries, that of 128 keys, max|dO_i| max|v_j| +
+// max|delta_i| over the queries that see them. (One bound a head cost the rows beside a large one their precision: error of dQ 1.6e-3
+// instead of 3e-4 beside a row of dO 2^18 times as large, 4096 rows.) Rows whose norms are infinite or NaN are left out of the
+// maxima. The sums are fp32.
 #pragma once
 #include "fwd_params.h"
 #include "ptx.cuh"
@@ -25,7 +28,7 @@ struct BwdParams {
   const float* d_lse;         // the same, or nullptr
   float* delta;               // [bh][seqlen]
   float* norms;               // [bh][tiles][3]: of 128 rows the largest |dO_i|, |v_i|, |delta_i|
-  __half *dq, *dk, *dv;
+  __half *dq, *dk, *dv;       // the place of 128 rows of dq holds, until they are written, their |dO_i|^2 as floats in a row
   int seqlen, bh, heads, tiles;  // tiles: ceil(seqlen / 128)
   int head_group;                // heads whose work items are interleaved
   int kinds_apart;               // in such a group all items of dK and dV come first, not those of one rank
@@ -91,7 +94,10 @@ __global__ void __launch_bounds__(1024) bwd_rows_kernel(const BwdParams p) {
     const int r = blockIdx.x * 128 + warp * 4 + i * kRows + lane / (D / 8);
     float delta, gg, vv;
     bwd_row<D>(p, head, r, lane, delta, gg, vv);
-    if (r < p.seqlen && lane % (D / 8) == 0) p.delta[head * p.seqlen + r] = delta;
+    if (r < p.seqlen && lane % (D / 8) == 0) {
+      p.delta[head * p.seqlen + r] = delta;
+      reinterpret_cast<float*>(p.dq + (head * p.seqlen + blockIdx.x * 128) * D)[r % 128] = gg;
+    }
     top[0] = fmaxf(top[0], bwd_norm(gg));
     top[1] = fmaxf(top[1], bwd_norm(vv));
     top[2] = fmaxf(top[2], bwd_norm(fabsf(delta)));
@@ -104,7 +110,7 @@ __global__ void __launch_bounds__(1024) bwd_rows_kernel(const BwdParams p) {
   __syncthreads();
   if (warp < 3) {  // warp k: the largest of norm k
     const float m = warp_max(s_max[lane][warp]);
-    if (lane == 0) p.norms[(head * p.tiles + blockIdx.x) * 3 + warp] = warp < 2 ? sqrtf(m) : m;
+    if (lane == 0) p.norms[(head * p.tiles + blockIdx.x) * 3 + warp] = warp < 2 ? sqrt_approx(m) : m;
   }
 }
 
@@ -120,14 +126,15 @@ struct BwdCfg {
   static constexpr int kOffFirst = 2 * kTileBytes;  // behind the item's own two tiles
   static constexpr int kOffSecond = kOffFirst + kFirst * kTileBytes;
   static constexpr int kOffStats = kOffSecond + kSecond * kTileBytes;  // per slot float[2][128]
-  static constexpr int kOffBars = kOffStats + kStats * 1024;
+  static constexpr int kOffUnits = kOffStats + kStats * 1024;  // per slot, for dQ, the exponents of 128 rows' units, a byte each
+  static constexpr int kOffBars = kOffUnits + kStats * 128;
   static constexpr int kNumBars = 2 * (kFirst + kSecond + kStats) + 10;
   static constexpr int kSmemBytes = kOffBars + kNumBars * 8 + 24;
-  // kOwnRows: delta of all rows, 16 warps' three norms and a barrier. At head_dim 128, where there is no other room, they lie in
+  // kOwnRows: delta and |dO_i|^2 of all rows, 16 warps' three norms and a barrier. At head_dim 128, where there is no other room, they lie in
   // the first ring's third slot, which the single tile of 128 rows does not reach.
   static constexpr int kMaxOwnRows = 16384 / D;
   static constexpr int kOffOwnRows = D == 128 ? kOffFirst + 2 * kTileBytes : (kSmemBytes + 15) / 16 * 16;
-  static constexpr int kOwnRowsBytes = kMaxOwnRows * 4 + 16 * 3 * 4 + 8;
+  static constexpr int kOwnRowsBytes = kMaxOwnRows * 8 + 16 * 3 * 4 + 8;
   static constexpr int kSmemBytesOwnRows = D == 128 ? kSmemBytes : kOffOwnRows + kOwnRowsBytes;
   static_assert(D == 64 || kFirst * 128 > kMaxOwnRows);
   static constexpr uint32_t kTmemCols = 512;
@@ -179,13 +186,11 @@ __device__ __forceinline__ int bwd_index(int k) {
   return k * static_cast<int>(gridDim.x) + static_cast<int>(k & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
 }
 
-// 2^-e (see the top of this file) from a lane's norms. A bound of zero leaves dS as it is; one beyond fp32 (norms are finite, their
-// sum need not be) is the largest. All lanes of a warp.
-__device__ __forceinline__ float bwd_unit(float g, float v, float d) {
-  const float bound = fmaf(warp_max(g), warp_max(v), warp_max(d));
+// The exponent field of 2^-e (see the top of this file) for a bound. A bound of zero leaves dS as it is; one beyond fp32 (norms are
+// finite, their sum need not be) is the largest.
+__device__ __forceinline__ uint32_t bwd_unit_exponent(float bound) {
   const int exponent = static_cast<int>(__float_as_uint(bound) >> 23 & 255u);  // biased by 127
-  if (exponent == 0) return 1.f;
-  return __uint_as_float(static_cast<uint32_t>(min(max(127 - (exponent - 126), 27), 227)) << 23);
+  return exponent == 0 ? 127u : static_cast<uint32_t>(min(max(127 - (exponent - 126), 27), 227));
 }
 
 // A role's place in a ring of slots, or on a barrier that is used again and again (one slot).
@@ -205,7 +210,7 @@ struct BwdBars {
   // has that of the tile before
   uint64_t *stats_empty, *p_ready, *ds_ready, *acc_empty;
   volatile int* abort_flag;
-  volatile float *unit, *slope;  // of the items of even and odd turn
+  volatile float *unit, *slope;  // of the items of even and odd turn (unit: of dK)
 };
 
 // dK and dV at head_dim 128 have one region for S.
@@ -255,8 +260,8 @@ __device__ __forceinline__ void bwd_store_rows(__half* to, int stride, int rows,
 // that take tiles in turn 10-30 %). A tile is a chain: wait, load S, exponentials, P, wait, load dP, dS. At head_dim 64 that chain
 // and the power cap set the pace (3650 clocks for the two tiles of a pair, of which 1540 are exponentials); at head_dim 128 the
 // products do, at the power cap.
-// kDq: the statistics (14 - log2(e) * lse and -delta / 2^e) are the row's, P is not needed further; else they are the
-// columns', and P goes to the tensor cores too. Returns false once a wait has run out.
+// kDq: the statistics (14 - log2(e) * lse, -delta / 2^e and e) are the row's, P is not needed further; else they are the
+// columns' (but for e), and P goes to the tensor cores too. Returns false once a wait has run out.
 template <int D, bool kAlibi, bool kDq>
 __device__ __forceinline__ bool bwd_softmax(const BwdParams& p, const BwdItem& it, BwdItem& next, const BwdBars& b,
                                             const uint8_t* smem, uint32_t tmem_base, int warp, int lane, int turn,
@@ -277,7 +282,7 @@ __device__ __forceinline__ bool bwd_softmax(const BwdParams& p, const BwdItem& i
     const float* stats = reinterpret_cast<const float*>(smem + Cfg::kOffStats + at.stats.slot * 1024);
     nl = stats[lane_base + lane];
     nd = stats[128 + lane_base + lane];
-    unit = b.unit[turn & 1];
+    unit = __uint_as_float(static_cast<uint32_t>(smem[Cfg::kOffUnits + at.stats.slot * 128 + lane_base + lane]) << 23);
     if (kAlibi) slope = b.slope[turn & 1];
     __syncwarp();
     mbar_arrive_lane0(b.stats_empty + at.stats.slot, lane);
@@ -543,34 +548,43 @@ __device__ __forceinline__ bool bwd_load(const CUtensorMap& map_q, const CUtenso
   return true;
 }
 
-// What bwd_rows_kernel computes, by the softmax warps of a CTA for all rows of its one item's head.
+// What bwd_rows_kernel computes, by the softmax warps of a CTA for all rows of its one item's head; the norms of the rows that bound
+// the item's dS.
 template <int D>
-__device__ __forceinline__ void bwd_own_rows(const BwdParams& p, int bh, uint8_t* smem, int warp, int lane) {
+__device__ __forceinline__ void bwd_own_rows(const BwdParams& p, const BwdItem& it, uint8_t* smem, int warp, int lane) {
   using Cfg = BwdCfg<D>;
   constexpr int kRows = 32 / (D / 8);  // of a warp at a time
   float* delta_of = reinterpret_cast<float*>(smem + Cfg::kOffOwnRows);
-  float* norms = delta_of + Cfg::kMaxOwnRows;
+  float* norm_of = delta_of + Cfg::kMaxOwnRows;  // |dO_i|^2
+  float* norms = norm_of + Cfg::kMaxOwnRows;
   float top[3] = {0.f, 0.f, 0.f};
 #pragma unroll 4
   for (int r0 = warp * kRows; r0 < p.seqlen; r0 += 16 * kRows) {
     const int r = r0 + lane / (D / 8);
     float delta, gg, vv;
-    bwd_row<D>(p, bh, r, lane, delta, gg, vv);
-    if (r < p.seqlen && lane % (D / 8) == 0) delta_of[r] = delta;
-    top[0] = fmaxf(top[0], bwd_norm(gg));
-    top[1] = fmaxf(top[1], bwd_norm(vv));
-    top[2] = fmaxf(top[2], bwd_norm(fabsf(delta)));
+    bwd_row<D>(p, it.bh, r, lane, delta, gg, vv);
+    if (r < p.seqlen && lane % (D / 8) == 0) {
+      delta_of[r] = delta;
+      norm_of[r] = gg;
+    }
+    const bool own = r / 128 == it.r0 / 128, column = r / 128 >= it.begin && r / 128 < it.begin + it.tiles;
+    if (it.is_dq ? own : column) {
+      top[0] = fmaxf(top[0], bwd_norm(gg));
+      top[2] = fmaxf(top[2], bwd_norm(fabsf(delta)));
+    }
+    if (it.is_dq ? column : own) top[1] = fmaxf(top[1], bwd_norm(vv));
   }
 #pragma unroll
   for (int k = 0; k < 3; ++k) {
     const float m = warp_max(top[k]);
-    if (lane == 0) norms[warp * 3 + k] = k < 2 ? sqrtf(m) : m;
+    if (lane == 0) norms[warp * 3 + k] = k < 2 ? sqrt_approx(m) : m;
   }
   __syncwarp();
   mbar_arrive_lane0(reinterpret_cast<uint64_t*>(norms + 48), lane);
 }
 
-// The warp that brings the statistics: for dK and dV those of every column tile, for dQ those of the item's own rows.
+// The warp that brings the statistics: for dK and dV those of every column tile, for dQ those of the item's own rows, each with its
+// unit.
 template <int D, bool kAlibi, bool kOwnRows>
 __device__ __forceinline__ void bwd_stats(const BwdParams& p, const BwdBars& b, uint8_t* smem, int lane) {
   using Cfg = BwdCfg<D>;
@@ -578,11 +592,12 @@ __device__ __forceinline__ void bwd_stats(const BwdParams& p, const BwdBars& b, 
   at.parity = 1;
   griddep_wait();
   const float* delta_here = reinterpret_cast<const float*>(smem + Cfg::kOffOwnRows);
-  const float* norms_here = delta_here + Cfg::kMaxOwnRows;
+  const float* norm_here = delta_here + Cfg::kMaxOwnRows;
+  const float* norms_here = norm_here + Cfg::kMaxOwnRows;
   for (int k = 0, index; (index = bwd_index(k)) < 2 * p.tiles * p.bh; ++k) {
     const BwdItem it = bwd_item(p, index);
     const int c0 = it.is_dq ? it.r0 : it.begin * 128;
-    float nl[4], nd[4];
+    float nl[4], nd[4], g[4];
     auto load = [&](int i) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -593,26 +608,54 @@ __device__ __forceinline__ void bwd_stats(const BwdParams& p, const BwdBars& b, 
       }
     };
     load(0);  // (on its way while the norms are read)
+    if (!kOwnRows && it.is_dq) {  // (this CTA alone writes the rows, and not before it has these statistics)
+      const float* norm_of = reinterpret_cast<const float*>(p.dq + (static_cast<size_t>(it.bh) * p.seqlen + it.r0) * D);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) g[j] = it.r0 + j * 32 + lane < p.seqlen ? norm_of[j * 32 + lane] : 0.f;
+    }
     const float slope = kAlibi ? p.alibi_slopes[it.bh % p.heads] * 1.4426950408889634f : 0.f;
     float norm[3] = {0.f, 0.f, 0.f};
     if (kOwnRows) {
       if (!mbar_wait_warp(reinterpret_cast<uint64_t*>(const_cast<float*>(norms_here + 48)), 0, b.abort_flag)) return;
       for (int j = 0; j < 3; ++j) norm[j] = lane < 16 ? norms_here[lane * 3 + j] : 0.f;
     } else {
-      for (int t = lane; t < p.tiles; t += 32)
-        for (int j = 0; j < 3; ++j) norm[j] = fmaxf(norm[j], p.norms[(static_cast<size_t>(it.bh) * p.tiles + t) * 3 + j]);
+      const float* norms = p.norms + static_cast<size_t>(it.bh) * p.tiles * 3;
+      for (int t = it.begin + lane; t < it.begin + it.tiles; t += 32) {
+        if (it.is_dq) {
+          norm[1] = fmaxf(norm[1], norms[3 * t + 1]);
+        } else {
+          norm[0] = fmaxf(norm[0], norms[3 * t]);
+          norm[2] = fmaxf(norm[2], norms[3 * t + 2]);
+        }
+      }
+      if (!it.is_dq) norm[1] = norms[it.r0 / 128 * 3 + 1];
     }
-    const float unit = bwd_unit(norm[0], norm[1], norm[2]);
+    for (int j = 0; j < 3; ++j) norm[j] = warp_max(norm[j]);
+    // of dK and dV; dQ has one a row
+    const float unit = __uint_as_float(bwd_unit_exponent(fmaf(norm[0], norm[1], norm[2])) << 23);
     for (int i = 0; i < (it.is_dq ? 1 : it.tiles); ++i) {
       if (i > 0) load(i);
+      if (kOwnRows) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int c = c0 + i * 128 + j * 32 + lane;
-        if (kOwnRows) nd[j] = c < p.seqlen ? -delta_here[c] : 0.f;
-        nd[j] *= unit;
+        for (int j = 0; j < 4; ++j) {
+          const int c = c0 + i * 128 + j * 32 + lane;
+          nd[j] = c < p.seqlen ? -delta_here[c] : 0.f;
+          g[j] = c < p.seqlen ? norm_here[c] : 0.f;
+        }
       }
       if (!mbar_wait_warp(b.stats_empty + at.slot, at.parity, b.abort_flag)) return;
       float* to = reinterpret_cast<float*>(smem + Cfg::kOffStats + at.slot * 1024);
+      if (it.is_dq) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t e = bwd_unit_exponent(fmaf(sqrt_approx(bwd_norm(g[j])), norm[1], bwd_norm(fabsf(nd[j]))));
+          nd[j] *= __uint_as_float(e << 23);
+          smem[Cfg::kOffUnits + at.slot * 128 + j * 32 + lane] = static_cast<uint8_t>(e);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) nd[j] *= unit;
+      }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         to[j * 32 + lane] = nl[j];
@@ -695,7 +738,7 @@ bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
   if (warp < Cfg::kSoftmaxWarps) {
     reg_inc<Cfg::kRegSoftmax>();
     BwdItem next = bwd_item(p, bwd_index(0));
-    if (kOwnRows) bwd_own_rows<D>(p, next.bh, smem, warp, lane);
+    if (kOwnRows) bwd_own_rows<D>(p, next, smem, warp, lane);
     SoftmaxTurns<D> at;
     bool ok = true;
     for (int k = 0; bwd_index(k) < 2 * p.tiles * p.bh && ok; ++k) {

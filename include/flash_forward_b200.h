@@ -118,9 +118,11 @@ int flash_forward_dropout(const void* q, const void* k, const void* v, void* o, 
  * those of the forward call; dropout has no backward pass here.
  *   lse, d_lse   float [batch][heads][seqlen]; d_lse is the gradient of the log-sum-exp, NULL for none (it is needed where
  *                the outputs over disjoint key ranges were merged by it)
- * P and dS are rounded to fp16 for the tensor cores, scaled by powers of two so that neither long rows nor small or large
- * gradients cost precision; all sums are fp32. dK, dV and dQ are summed in one order: two calls with the same arguments give
- * the same bits.
+ * P and dS are rounded to fp16 for the tensor cores, scaled by powers of two: for dQ every row by its own sizes, for dK and dV 128
+ * keys by those of the queries that see them, so that neither long rows nor small or large gradients cost precision. (In dK a
+ * query far larger than the others of its keys, by 2^16 and more, costs theirs.) All sums are fp32. dK, dV and dQ are summed in
+ * one order: two calls with the same arguments give the same bits. An element that is infinite or NaN may reach, beyond what the
+ * formula says, the blocks of 128 rows that see its block or are seen by it (0 times it is NaN), none further away.
  * workspace: flash_backward_workspace_bytes() bytes of device memory, 256-byte aligned, with any contents; calls that may
  * overlap on the GPU need one each. Asynchronous on `stream`, one launch or two; may be captured into a CUDA graph once a call
  * of this library has been made on the device. batch*heads up to 65535. flash_forward_check() reports a wait that ran out. */

@@ -1,4 +1,9 @@
-"""flash_backward where one row of a head is infinite: the rows that it does not touch. Tolerances of test_backward_gpu.py."""
+"""flash_backward where one row of a head is infinite, or far larger than the others: the rows that it does not touch.
+
+Tolerances: element by element those of test_backward_gpu.py; and for the whole, where errors that one large row would cause
+are random and hide below a sum of absolute values, the 2-norm: every dS_ij is off by at most half a step of fp16 (2^-11) and
+what the scores do to P (2^-13), every output by half a step, all of them independent of one another, so the squares add up;
+2^-13 of the norm for what a row's elements share."""
 import math
 
 import pytest
@@ -72,10 +77,47 @@ def test_rows_in_front_of_an_infinite_value(pkg, d):
            list(range(640)))
 
 
-def test_infinite_rows_in_a_short_head(pkg):
+def norm_within(got, q, k, v, out, lse, dout, dlse, rows_q, rows_k):
+    """Errors in the 2-norm of dq over rows_q and of dk over rows_k against what independent roundings add up to."""
+    want = oracle.Gradient(q, k, v, out, lse, dout, dlse, causal=True)
+    x = [t.double() for t in (q, k, v, out, lse, dout)]
+    scale = 1 / math.sqrt(q.shape[3])
+    p = torch.exp(oracle.scores(x[0], x[1], causal=True) - x[4][..., None])
+    delta = (x[5] * x[3]).sum(-1) - (0 if dlse is None else dlse.double())
+    ds2 = (p * (x[5] @ x[2].transpose(2, 3) - delta[..., None])) ** 2
+    h2, r = 2.0 ** -22, 2.0 ** -13
+    var = {"dq": scale ** 2 * (h2 + r * r) * (ds2 @ x[1] ** 2) + h2 * want.dq ** 2,
+           "dk": scale ** 2 * (h2 + r * r) * (ds2.transpose(2, 3) @ x[0] ** 2) + h2 * want.dk ** 2}
+    for name, rows in (("dq", rows_q), ("dk", rows_k)):
+        w = getattr(want, name)[:, :, rows]
+        err = (got[name][:, :, rows].double() - w).norm()
+        bound = var[name][:, :, rows].sum().sqrt() + r * w.norm()
+        assert err <= bound, (name, float(err / bound))
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_small_rows_beside_a_large_one(pkg, d):
+    """One row of dO is 2^18 times the others, and one d_lse is 10^6 or near the end of fp32: no cost to the precision of other
+    rows of dQ, nor of dK where the row is not seen."""
+    N, row = 4096, 50
+    q, k, v, dout = tensors(70 + d, 1, 1, N, d, grad=2.0 ** -6)
+    large = dout.clone()
+    large[0, 0, row] *= 2.0 ** 18
+    rest, unseen = [i for i in range(N) if i != row], list(range(128, N))
+    out, lse, got = run(pkg, q, k, v, large, causal=True)
+    norm_within(got, q, k, v, out, lse, large, None, rest, unseen)
+    for value in (1e6, 3e38):
+        dlse = torch.zeros((1, 1, N))
+        dlse[0, 0, row] = value
+        out, lse, got = run(pkg, q, k, v, dout, dlse, causal=True)
+        norm_within(got, q, k, v, out, lse, dout, dlse, rest, unseen)
+
+
+def test_small_rows_beside_a_large_one_in_a_short_head(pkg):
     """The same bits where the kernel finds the norms itself and where another kernel has found them."""
     for N, d in ((200, 64), (100, 128), (256, 64), (128, 128)):
         q, k, v, dout = (x.cuda() for x in tensors(80 + N, 31, 5, N, d, grad=2.0 ** -6))
+        dout[:, :, 3] *= 2.0 ** 18
         dout[1, 2, N - 2] = math.inf
         out, lse = pkg.attention_forward(q, k, v, causal=True, return_lse=True)
         many = pkg.attention_backward(q, k, v, out, lse, dout, causal=True)

@@ -381,7 +381,7 @@ def attention_backward(q, k, v, out, lse, dout, causal=False, window_left=-1, wi
     `dout` of out (and `dlse` of lse, if given): (dq, dk, dv), flash_backward of the C header.
 
     All tensors as attention_forward takes and gives them; dout is made contiguous if it is not. dq, dk, dv, if given,
-    are contiguous tensors like q that are written.
+    are contiguous tensors like q that are written; none of them may overlap another tensor of the call.
     """
     r = _answered_natively(0, q, k, v, out, lse, dout, causal, window_left, window_right, softmax_scale, alibi_slopes, dlse,
                            dq, dk, dv)

@@ -11,6 +11,15 @@ namespace {
 
 size_t align256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
 
+struct Range {
+  const void* at;  // nullptr: nothing
+  size_t bytes;
+};
+bool overlap(const Range& a, const Range& b) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a.at), y = reinterpret_cast<uintptr_t>(b.at);
+  return a.at && b.at && (x < y ? y - x < a.bytes : x - y < b.bytes);
+}
+
 template <int D, bool kAlibi, bool kOwnRows>
 int launch_main(const CUtensorMap (&maps)[4], const fa::BwdParams& p, int ctas, cudaStream_t st, bool early) {
   using Cfg = fa::BwdCfg<D>;
@@ -65,6 +74,17 @@ int backward(const void* q, const void* k, const void* v, const void* o, const v
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if ((rc = device_state_for(st, &s, &captured)) != FA_OK) return rc;
   if (!s->is_sm100) return fail(FA_UNSUPPORTED, "this library runs on compute capability 10.x (B200) only");
+  // (results are written while other items still read the inputs, and dq holds norms before)
+  const size_t rows = static_cast<size_t>(bh) * seqlen, whole = rows * head_dim * 2;
+  const Range written[4] = {{dq, whole}, {dk, whole}, {dv, whole}, {workspace, flash_backward_workspace_bytes(batch, heads, seqlen)}};
+  const Range read[8] = {{q, whole}, {k, whole}, {v, whole}, {o, whole}, {d_o, whole}, {lse, rows * 4}, {d_lse, rows * 4},
+                         {alibi_slopes, static_cast<size_t>(heads) * 4}};
+  for (int i = 0; i < 4; ++i) {
+    for (const Range& r : read)
+      if (overlap(written[i], r)) return fail(FA_INVALID_ARG, "dq, dk, dv and the workspace must not overlap the inputs");
+    for (int j = 0; j < i; ++j)
+      if (overlap(written[i], written[j])) return fail(FA_INVALID_ARG, "dq, dk, dv and the workspace must not overlap one another");
+  }
   if (softmax_scale <= 0.f) softmax_scale = 1.0f / sqrtf(static_cast<float>(head_dim));
 
   fa::BwdParams p;

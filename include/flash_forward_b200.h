@@ -114,8 +114,8 @@ int flash_forward_dropout(const void* q, const void* k, const void* v, void* o, 
  *   P_ij = exp(s_ij - lse_i) where key j is visible to query i, else 0;  dS_ij = P_ij (dO_i.V_j - dO_i.O_i + dlse_i)
  *   dQ_i = scale sum_j dS_ij K_j,  dK_j = scale sum_i dS_ij Q_i,  dV_j = sum_i P_ij dO_i
  * No counterpart in the reference, whose kernel is a forward. All tensors fp16, contiguous [batch][heads][seqlen][head_dim],
- * 16-byte aligned; the outputs must not overlap the inputs. Scale, causal flag, windows and alibi_slopes (NULL: no bias) are
- * those of the forward call; dropout has no backward pass here.
+ * 16-byte aligned; dq, dk, dv and the workspace overlap neither the inputs nor one another (FA_INVALID_ARG). Scale, causal
+ * flag, windows and alibi_slopes (NULL: no bias) are those of the forward call; dropout has no backward pass here.
  *   lse, d_lse   float [batch][heads][seqlen]; d_lse is the gradient of the log-sum-exp, NULL for none (it is needed where
  *                the outputs over disjoint key ranges were merged by it)
  * P and dS are rounded to fp16 for the tensor cores, scaled by powers of two: for dQ every row by its own sizes, for dK and dV 128

@@ -186,7 +186,7 @@ struct DecodeParams {
   int ctas;
   int cluster;     // CTAs of a cluster that share an item and join it themselves (1: a CTA an item), or 0: the line below
   float* part_o;   // [ctas][2][part_rows][head_dim]
-  float* part_ml;  // [ctas][2][part_rows][2]: running maximum (log2 units) and sum
+  float* part_ml;  // [ctas][2][part_rows][2]: what the exponentials were taken against (log2 units) and their sum
   int part_rows;   // rows of a row tile
   int item_units;  // tiles of keys that an item's beginning and end take as long as
   int* status;
@@ -395,8 +395,9 @@ __device__ __forceinline__ void compute_sync() {
 // matters: 64 sequences of up to 32768 tokens, 32 heads on 8 of 128, 4.8 GB in 704-741 us; one of 131072 in 89 us (6.0 TB/s, 5 of
 // them start and join). More than 16 rows leave the warps latency-bound (16 x 8 tokens, 64 heads on 8, up to 32768 tokens: 352 us
 // for 1.2 GB), so there decode_wide_kernel takes all but short work. Scores, maxima, sums and O are fp32; P is rounded to the
-// cache's type for the second product, as the operand has to be, half a step relative to the element, and its sum is taken
-// unrounded.
+// cache's type for the second product, as the operand has to be, and its sum is taken unrounded. In fp16 it is kept as 2^14 P, so
+// that it is half a step off down to 2^-28 of the row's maximum. (Kept as P, what lies 17 nats below the maximum was off by up to
+// all of itself: the tail of 131071 keys behind one that dominates them, 4e-3 of the weight, came out a quarter too large.)
 template <typename T, int D, int kRowWarps>
 __global__ void __launch_bounds__(DecodeCfg<D, kRowWarps>::kThreads, DecodeCfg<D, kRowWarps>::kCtasPerSm)
 decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
@@ -485,6 +486,7 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
     return (row >> box_shift) * (p.box_rows * D * 2) + (row & (p.box_rows - 1)) * 128;
   };
   const uint32_t panel = p.box_rows * 128;
+  constexpr float kRoom = std::is_same_v<T, __half> ? 14.f : 0.f;  // P is kept as 2^kRoom P
   bool ok = true;  // once a wait has run out, the warp goes on with whatever is there: the others may wait for it
 
   while (walk.next(p, kv_head, row_tile, t0, t1)) {
@@ -577,7 +579,7 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
             o[n][3] *= scale[1];
           }
         }
-        const float off[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
+        const float off[2] = {m[0] == -INFINITY ? 0.f : m[0] - kRoom, m[1] == -INFINITY ? 0.f : m[1] - kRoom};
 #pragma unroll
         for (int n = 0; n < Cfg::kChunk / 16; ++n) {
           uint32_t pf[4];
@@ -630,6 +632,7 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
     ok = __all_sync(0xffffffffu, ok);
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
+      m[r] -= kRoom;  // from here on what the sum and O were taken against
       l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
       l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
     }

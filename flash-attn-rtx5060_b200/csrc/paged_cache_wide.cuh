@@ -25,7 +25,7 @@ struct WideCfg {
   static constexpr int kSmemBytes = kOffBars + kNumBars * 8 + 16;
   // tensor memory: scores of either group of softmax warps, in which P takes their place, and its O
   static constexpr uint32_t kColO = kRegions * kKeys;
-  static constexpr float kLazy = 8.f;
+  static constexpr float kLazy = 8.f, kRoom = 7.f;  // kRoom: in fp16, where P is kept as 2^kRoom P
   static constexpr int kMaxCopies = kKeys / 32;
 };
 
@@ -37,7 +37,7 @@ struct WideCfg {
 // takes a part of a tile's keys (its P is 0 for the others), so that all warps share the exponentials; the copies are summed at
 // the end of the item (32 rows d64 x up to 8192: 62 -> 46 us). The reference that a row's exponentials are taken against moves
 // only when the maximum has grown by 2^8 over it, so that O is rarely rescaled; P is at most 2^8 and is rounded once to the
-// cache's type. Warps whose rows are all padding only hand on. Everything is summed in an order that depends on the lengths alone.
+// cache's type, in fp16 as 2^7 P: half a step off down to 2^-21 of the row's maximum, and at most 2^-32 of that below. Warps whose rows are all padding only hand on. Everything is summed in an order that depends on the lengths alone.
 // 12 warps: 0-7 softmax, 8 issues the products, 9 loads, 10 and 11 bring Q of the next item (with Q brought by the softmax warps
 // themselves an item took 5000 clocks more).
 // Bound by HBM where contexts are long: 16 x 8 tokens, 64 heads on 8 of 128, up to 32768 tokens 209 us (5.8 TB/s); by the chain
@@ -94,6 +94,7 @@ decode_wide_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
     float2* ml = reinterpret_cast<float2*>(smem + Cfg::kOffMl);         // [group][row]
     uint32_t s_at = 0, done_at = 0, o_at = 0, q_at = 0;  // parities at the start of the item; s_at: a bit a region
     int loaded = 0;  // tiles of the items before
+    constexpr float room = std::is_same_v<T, __half> ? Cfg::kRoom : 0.f;
     while (walk.next(p, kv_head, row_tile, t0, t1)) {
       const int n = t1 - t0, r = row_tile * Cfg::kRows + in_tile % copy_rows;
       const int t = r / p.group, head = kv_head * p.group + r % p.group;
@@ -186,7 +187,7 @@ decode_wide_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
               }
             }
           }
-          const float off = m == -INFINITY ? 0.f : m;
+          const float off = m == -INFINITY ? 0.f : m - room;
 #pragma unroll 1
           for (int chunk = 0; chunk < chunks; chunk += kKept) {
 #pragma unroll
@@ -226,7 +227,7 @@ decode_wide_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
       const long long out_row = (static_cast<long long>(walk.b) * p.q_heads + head) * p.cache.tokens + t;
       const long long part = (2ll * blockIdx.x + (t0 == 0 ? 1 : 0)) * p.part_rows + in_tile % copy_rows;
       // ---- the parts of both groups and of all copies joined ----
-      ml[group * Cfg::kRows + in_tile] = make_float2(m, l);
+      ml[group * Cfg::kRows + in_tile] = make_float2(m - room, l);  // what the sum and O were taken against
       if (n > 0) {
         ok &= mbar_wait(o_full, o_at, abort_flag);
         o_at ^= 1;

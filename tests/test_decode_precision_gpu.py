@@ -1,0 +1,41 @@
+"""flash_decode on rows that one key dominates.
+
+Tolerances: as in test_paged_cache_gpu.py; and where P is so small beside the row's maximum that fp16 holds it in steps,
+half a step a key: P is kept as 2^14 P for up to 16 rows and as 2^7 P or more for more, so that is at most 2^-32 of the
+maximum (2^-25 / 2^7), times |V|."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def one_sequence_many_times(keys, values, copies, page=128):
+    """A pool that holds one sequence [keys][d], and a table by which `copies` sequences share it."""
+    n, d = keys.shape
+    pages = n // page
+    pools = [x.view(pages, 1, page, d).cuda() for x in (keys, values)]
+    table = torch.arange(pages, dtype=torch.int32)[None].repeat(copies, 1).cuda()
+    return pools + [table, torch.full((copies,), n, dtype=torch.int32).cuda()]
+
+
+@pytest.mark.parametrize("head_dim", [64, 128])
+@pytest.mark.parametrize("rows", [1, 24, 40, 128])
+def test_a_long_tail_behind_a_dominating_key(pkg, rows, head_dim):
+    """An early key 17.3 nats above 131071 others, whose values the output is made of: they have 4e-3 of the weight together,
+    3e-8 each. Many sequences, so that a CTA has all of a sequence's keys."""
+    n, copies = 131072, 320
+    keys, values = torch.zeros((n, head_dim)), torch.ones((n, head_dim))
+    keys[3, 0], values[3] = 17.3125, 0.0
+    args = one_sequence_many_times(keys.half(), values.half(), copies)
+    q = torch.zeros((copies, rows, 1, head_dim))
+    q[..., 0] = 1.0
+    out, lse = pkg.attention_decode(q.half().cuda(), *args, softmax_scale=1.0, return_lse=True)
+    pkg.check(torch.cuda.current_stream().cuda_stream)
+    total = math.exp(17.3125) + n - 1
+    want = (n - 1) / total
+    bound = 2.0 ** -11 * 2 * want + 2.0 ** -13 * want + n * 2.0 ** -32
+    err = float((out.double() - want).abs().max())
+    assert err <= bound, (err, bound)
+    assert float((lse.double() - math.log(total)).abs().max()) <= 5e-4

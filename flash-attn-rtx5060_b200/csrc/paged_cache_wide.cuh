@@ -165,10 +165,9 @@ decode_wide_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
               top = fmaxf(top, fmaxf(a, b));
             }
           }
-          const bool grown = top > m + Cfg::kLazy;
-          if (__any_sync(0xffffffffu, grown)) {
-            const float alpha = grown ? ex2_approx(m - top) : 1.f;
-            if (grown) m = top;
+          if (__any_sync(0xffffffffu, top > m + Cfg::kLazy)) {
+            const float alpha = top > m ? ex2_approx(m - top) : 1.f;
+            m = fmaxf(m, top);
             l *= alpha;
             if (i >= 2) {
               if (Cfg::kRegions > 2) {  // the group's last product has to be summed (else S came behind it)

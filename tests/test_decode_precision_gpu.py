@@ -2,7 +2,7 @@
 
 Tolerances: as in test_paged_cache_gpu.py; and where P is so small beside the row's maximum that fp16 holds it in steps,
 half a step a key: P is kept as 2^14 P for up to 16 rows and as 2^7 P or more for more, so that is at most 2^-32 of the
-maximum (2^-25 / 2^7), times |V|."""
+maximum (2^-25 / 2^7), times |V|. The exact main term has no rounding of P, only that of the output."""
 import math
 
 import pytest
@@ -39,3 +39,33 @@ def test_a_long_tail_behind_a_dominating_key(pkg, rows, head_dim):
     err = float((out.double() - want).abs().max())
     assert err <= bound, (err, bound)
     assert float((lse.double() - math.log(total)).abs().max()) <= 5e-4
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("head_dim", [64, 128])
+def test_a_dominating_key_whose_neighbour_row_moves(pkg, head_dim, dtype):
+    """128 rows in products of 128: in a later tile the maximum of every second row grows by less than 2^8, that of the others
+    by far more. The rows move along together, and the key that dominates a row has P = 1, without a rounding."""
+    n, page = 1 << 16, 128
+    eps = torch.finfo(dtype).eps / 2
+    scale = math.log2(128.45) / 7.0 * math.log(2.0)  # a product of 7 is a P of 128.45: 128 in bf16
+    g = torch.Generator().manual_seed(3)
+    keys, values = torch.zeros((n, head_dim)), torch.randn((n, head_dim), generator=g).to(dtype)
+    keys[:, 0] = keys[:, 1] = -40.0
+    keys[1, 0] = keys[1, 1] = 0.0
+    first_of_third_tile = 2 * (64 if head_dim == 128 else 128)
+    keys[first_of_third_tile, 0], keys[first_of_third_tile, 1] = 7.0, 40.0
+    args = one_sequence_many_times(keys.to(dtype), values, 4, page)
+    q = torch.zeros((4, 128, 1, head_dim))
+    q[:, ::2, :, 0] = 1.0
+    q[:, 1::2, :, 1] = 1.0
+    out = pkg.attention_decode(q.to(dtype).cuda(), *args, softmax_scale=scale).cpu().double()
+    pkg.check(torch.cuda.current_stream().cuda_stream)
+    for rows, dim in ((slice(0, None, 2), 0), (slice(1, None, 2), 1)):
+        p = torch.softmax(keys[:, dim].double() * scale, 0)
+        want = p @ values.double()
+        size = p[:, None] * values.double().abs()
+        minor = size.sum(0) - size[first_of_third_tile]
+        bound = eps * (want.abs() + minor) + 2.0 ** -13 * size.sum(0)
+        err = (out[:, rows, 0] - want).abs()
+        assert (err <= bound).all(), (dim, float((err / bound).max()))

@@ -36,8 +36,10 @@ struct WideCfg {
 // no exchange for its maximum and sum. Where the rows fill half of the 128 or a quarter, M holds copies of them, of which each
 // takes a part of a tile's keys (its P is 0 for the others), so that all warps share the exponentials; the copies are summed at
 // the end of the item (32 rows d64 x up to 8192: 62 -> 46 us). The reference that a row's exponentials are taken against moves
-// only when the maximum has grown by 2^8 over it, so that O is rarely rescaled; P is at most 2^8 and is rounded once to the
-// cache's type, in fp16 as 2^7 P: half a step off down to 2^-21 of the row's maximum, and at most 2^-32 of that below. Warps whose rows are all padding only hand on. Everything is summed in an order that depends on the lengths alone.
+// only when the maximum has grown by 2^8 over it, so that O is rarely rescaled, or along with another row of the warp that has to
+// (the key that sets it has P = 1 exactly, one above it a P that is rounded); P is at most 2^8 and is rounded once to the cache's
+// type, in fp16 as 2^7 P: half a step off down to 2^-21 of the row's maximum, and at most 2^-32 of that below. Warps whose rows are
+// all padding only hand on. Everything is summed in an order that depends on the lengths alone.
 // 12 warps: 0-7 softmax, 8 issues the products, 9 loads, 10 and 11 bring Q of the next item (with Q brought by the softmax warps
 // themselves an item took 5000 clocks more).
 // Bound by HBM where contexts are long: 16 x 8 tokens, 64 heads on 8 of 128, up to 32768 tokens 209 us (5.8 TB/s); by the chain

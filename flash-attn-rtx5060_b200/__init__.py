@@ -508,8 +508,8 @@ def attention_decode(q, k_pages, v_pages, page_table, lengths, counts=None, soft
     """Attention of the newest tokens of every sequence over a paged cache (flash_decode of the C header).
 
     q: [batch, q_heads, tokens, head_dim], any strides with head_dim contiguous, q_heads a multiple of the cache's heads;
-    the cache as for cache_append, after it. Returns the output, contiguous and shaped like q (`out` if given), and with
-    return_lse also float32 [batch, q_heads, tokens].
+    the cache as for cache_append, after it. Returns the output, contiguous and shaped like q (`out` if given, which may be a
+    contiguous q itself), and with return_lse also float32 [batch, q_heads, tokens].
     """
     r = _answered_natively(2, q, k_pages, v_pages, page_table, lengths, counts, softmax_scale, window_left, alibi_slopes,
                            return_lse, out)

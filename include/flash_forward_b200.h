@@ -322,9 +322,11 @@ int flash_cache_append(const fa_paged_cache* cache, const fa_rows* k, const fa_r
  * multiple of kv_heads. Query t of sequence b, at position i = lengths[b] - counts[b] + t, sees the keys j <= i, and with
  * window_left >= 0 those with j >= i - window_left; pages that lie in front of every query's window are not read.
  * alibi_slopes (NULL, or q_heads floats on the device) as for flash_forward_alibi(); softmax_scale as for flash_forward().
- *   o    contiguous [batch][q_heads][tokens][head_dim], 16-byte aligned
+ *   o    contiguous [batch][q_heads][tokens][head_dim], 16-byte aligned; may be q's own memory if q is laid out like it
  *   lse  NULL, or float [batch][q_heads][tokens]: the log-sum-exp as in flash_forward_lse()
- * Rows of padding, and of sequences without keys, are O = 0 and lse = -infinity.
+ * Rows of padding, and of sequences without keys, are O = 0 and lse = -infinity. A value of V that is infinite or NaN reaches all
+ * new tokens of its sequence that read its key head, those in front of it and those whose window it has left too (0 times it
+ * is NaN).
  * workspace: flash_decode_workspace_bytes() bytes of device memory, 16-byte aligned, with any contents; calls that may
  * overlap on the GPU need one each. Asynchronous on `stream`, one launch or two; may be captured into a CUDA graph once a call
  * has been made on the device. Two calls with the same arguments give the same bits; how a sequence's keys are shared out
@@ -337,7 +339,8 @@ size_t flash_decode_workspace_bytes(int tokens, int q_heads, int kv_heads, int h
 
 /* Frees the per-device status words, events and streams this library created, and forgets what it
  * learned about each device (scratch addresses, kernel attributes), so that it can be used again
- * after a device reset. Optional. */
+ * after a device reset. Calls of flash_backward, flash_cache_append and flash_decode that were captured into a graph hold the
+ * address of the status words: they are not to be replayed afterwards. Optional. */
 int flash_forward_shutdown(void);
 
 #ifdef __cplusplus

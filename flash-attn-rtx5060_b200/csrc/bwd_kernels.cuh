@@ -78,7 +78,7 @@ __device__ __forceinline__ float warp_max(float x) {
 // others' has to be that of their own sizes (an infinite bound once left dS of the whole head unscaled: it overflowed).
 __device__ __forceinline__ float bwd_norm(float x) { return x < INFINITY ? x : 0.f; }
 
-// 128 rows of a head a CTA. Reads O, dO and V once: bound by bytes where rows are many (B1 H16 N8192 d128: 101 MB in 21 us under
+// 128 rows of a head a CTA. Reads O, dO and V once: bound by bytes where rows are many (B1 H16 N8192 d128: 101 MB in 24 us under
 // ncu, caches flushed), else by one round of loads and two reductions.
 template <int D>
 __global__ void __launch_bounds__(1024) bwd_rows_kernel(const BwdParams p) {
@@ -258,7 +258,7 @@ __device__ __forceinline__ void bwd_store_rows(__half* to, int stride, int rows,
 // The sixteen softmax warps: a thread has one row and 32 columns of every tile (warps 0-3 the first 32, and so on), so that four
 // warps a sub-partition hide one another's latencies (eight warps with 64 columns each: 10-20 % slower, and two groups of eight
 // that take tiles in turn 10-30 %). A tile is a chain: wait, load S, exponentials, P, wait, load dP, dS. At head_dim 64 that chain
-// and the power cap set the pace (3650 clocks for the two tiles of a pair, of which 1540 are exponentials); at head_dim 128 the
+// and the power cap set the pace (3680 clocks for the two tiles of a pair, of which 1540 are exponentials); at head_dim 128 the
 // products do, at the power cap.
 // kDq: the statistics (14 - log2(e) * lse, -delta / 2^e and e) are the row's, P is not needed further; else they are the
 // columns' (but for e), and P goes to the tensor cores too. Returns false once a wait has run out.
@@ -673,8 +673,8 @@ __device__ __forceinline__ void bwd_stats(const BwdParams& p, const BwdBars& b, 
 }
 
 // One CTA a SM walks the work items bwd_index(0), bwd_index(1), ... (a CTA an item, started by the hardware, took 7 us an item
-// for its start and end: window 1024 2576 -> 2153 us with all that came with it). Bound by the tensor pipe at head_dim 128: 4490
-// clocks a pair of tiles for 3584 of products, 80 % busy at 1.3-1.5 GHz under the power cap; B2 H32 N8192 causal 3400-3560 us,
+// for its start and end: window 1024 2576 -> 2153 us with all that came with it). Bound by the tensor pipe at head_dim 128: 4510
+// clocks a pair of tiles for 3584 of products, 79 % busy at 1.3-1.5 GHz under the power cap; B2 H32 N8192 causal 3400-3560 us,
 // 770-810 TFLOP/s of the five products that the gradient has; B2 H16 N4096 d64 causal 266-304 us. 20 warps: 0-15 softmax and
 // epilogue, 16 issues the products, 17 loads tiles, 18 brings the statistics, 19 only donates registers.
 // kOwnRows: short heads, an item a CTA, no bwd_rows_kernel: the softmax warps, idle until the first products, do its work for

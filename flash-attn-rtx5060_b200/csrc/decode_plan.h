@@ -12,11 +12,12 @@ inline int decode_part_rows(long long rows, bool wide) {
   return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 || !wide ? 64 : 128;
 }
 // Whether decode_wide_kernel takes a call: it starts and ends an item later by 5 us together, and takes half as long over a tile.
-// `work`: tiles of keys a CTA, if all sequences were as long as they may be. us, decode_kernel -> decode_wide_kernel, 16 sequences
-// on 8 key heads: 64 rows d128 x 512 26.6 -> 29.6, x 1024 (14 tiles a CTA) 36.1 -> 33.5, x 4096 93 -> 67, up to 32768 352 -> 209;
-// 32 rows d128 x 4096 (55) 58.8 -> 60.5, up to 32768 220 -> 198; 32 rows d64 x 4096 (28) 38.3 -> 36.7; and 2048 tokens of
-// 32 heads on 8 over 8192 keys 1271 -> 404, 4 x 256 tokens 395 -> 147; but 128 rows d64 x 512 (3) 21.9 -> 28.8, 400 rows x 512 (1)
-// 12.7 -> 17.8.
+// `work`: tiles of keys a CTA, if all sequences were as long as they may be. us, decode_kernel -> decode_wide_kernel, 16 sequences of
+// one length on 8 key heads (in brackets the tiles a CTA). d128: 32 rows (27) 37.0 -> 38.9, (48) 53.8 -> 53.8, (83) 82.8 -> 78.6,
+// (166) 167 -> 140; 64 rows (6) 31.1 -> 32.2, (13) 41.9 -> 37.2, (27) 60.8 -> 48.8; 128 rows (3) 22.6 -> 31.0, (6) 32.9 -> 34.0, (10)
+// 51.7 -> 36.9, (20) 81.4 -> 50.3. d64, where the borders are not the best ones: 32 rows (6) 18.0 -> 19.5, (13) 24.2 -> 24.1, (27)
+// 37.5 -> 36.2, (41) 49.7 -> 45.6, (55) 61.9 -> 55.8; 64 rows (3) 19.2 -> 23.4, (6) 27.5 -> 27.0, (13) 37.9 -> 32.6; 128 rows (3) 21.6
+// -> 28.7, (5) 28.1 -> 31.9, (6) 34.1 -> 34.1, (10) 53.2 -> 38.8. 2048 tokens of 32 heads on 8 over 8192 keys 1271 -> 404.
 inline bool decode_wide(long long rows, long long work) { return rows > 16 && work >= (rows > 64 ? 5 : rows > 32 ? 10 : 48); }
 // CTAs of a cluster that takes an item (a sequence, key head and tile of rows) of up to `tiles` tiles of keys as a whole, 1 for
 // a CTA alone, or 0 where the items are cut by the line and joined by a second launch (which takes as long as four tiles or

@@ -43,8 +43,9 @@ struct WideCfg {
 // 12 warps: 0-7 softmax, 8 issues the products, 9 loads, 10 and 11 bring Q of the next item (with Q brought by the softmax warps
 // themselves an item took 5000 clocks more).
 // Bound by HBM where contexts are long: 16 x 8 tokens, 64 heads on 8 of 128, up to 32768 tokens 209 us (5.8 TB/s); by the chain
-// where many tokens share the keys: 2048 tokens of 32 heads on 8 over 8192 keys, 241 GFLOP under the mask, in 404 us. An item's
-// start and end take as long as six tiles.
+// where many tokens share the keys: 2048 tokens of 32 heads on 8 over 8192 keys, 241 GFLOP under the mask, in 404 us, an eighth
+// of it for tiles that a row tile does not see (the line has a sequence's tiles for every row tile; of a prompt without a past it is
+// half). An item's start and end take as long as six tiles.
 template <typename T, int D>
 __global__ void __launch_bounds__(WideCfg<D>::kThreads, 1)
 decode_wide_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,

@@ -383,6 +383,12 @@ __device__ __forceinline__ float2 dsmem_ld2(const void* here, uint32_t rank) {
                : "memory");
   return v;
 }
+// What exponentials are taken against for a maximum of m, so that the largest is 2^kRoom. Rounded up: scores so large that fp32 has
+// steps of 4 and more there would else be taken against something further below, up to 2^16, which fp16 does not hold.
+template <int kRoom>
+__device__ __forceinline__ float reference_of(float m) {
+  return kRoom > 0 ? __fadd_ru(m, -static_cast<float>(kRoom)) : m;
+}
 // barrier of the warps that compute
 template <int kThreads>
 __device__ __forceinline__ void compute_sync() {
@@ -486,7 +492,7 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
     return (row >> box_shift) * (p.box_rows * D * 2) + (row & (p.box_rows - 1)) * 128;
   };
   const uint32_t panel = p.box_rows * 128;
-  constexpr float kRoom = std::is_same_v<T, __half> ? 14.f : 0.f;  // P is kept as 2^kRoom P
+  constexpr int kRoom = std::is_same_v<T, __half> ? 14 : 0;  // P is kept as 2^kRoom P
   bool ok = true;  // once a wait has run out, the warp goes on with whatever is there: the others may wait for it
 
   while (walk.next(p, kv_head, row_tile, t0, t1)) {
@@ -567,7 +573,7 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
         if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1])) {
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            scale[r] = top[r] == -INFINITY ? 1.f : ex2_approx(m[r] - top[r]);
+            scale[r] = top[r] == -INFINITY ? 1.f : ex2_approx(reference_of<kRoom>(m[r]) - reference_of<kRoom>(top[r]));
             m[r] = top[r];
             l[r] *= scale[r];
           }
@@ -579,7 +585,8 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
             o[n][3] *= scale[1];
           }
         }
-        const float off[2] = {m[0] == -INFINITY ? 0.f : m[0] - kRoom, m[1] == -INFINITY ? 0.f : m[1] - kRoom};
+        const float off[2] = {m[0] == -INFINITY ? 0.f : reference_of<kRoom>(m[0]),
+                              m[1] == -INFINITY ? 0.f : reference_of<kRoom>(m[1])};
 #pragma unroll
         for (int n = 0; n < Cfg::kChunk / 16; ++n) {
           uint32_t pf[4];
@@ -632,7 +639,7 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
     ok = __all_sync(0xffffffffu, ok);
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      m[r] -= kRoom;  // from here on what the sum and O were taken against
+      m[r] = reference_of<kRoom>(m[r]);  // from here on what the sum and O were taken against
       l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
       l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
     }

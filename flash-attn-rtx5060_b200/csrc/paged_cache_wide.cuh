@@ -25,7 +25,8 @@ struct WideCfg {
   static constexpr int kSmemBytes = kOffBars + kNumBars * 8 + 16;
   // tensor memory: scores of either group of softmax warps, in which P takes their place, and its O
   static constexpr uint32_t kColO = kRegions * kKeys;
-  static constexpr float kLazy = 8.f, kRoom = 7.f;  // kRoom: in fp16, where P is kept as 2^kRoom P
+  static constexpr float kLazy = 8.f;
+  static constexpr int kRoom = 7;  // in fp16: P is kept as 2^kRoom P
   static constexpr int kMaxCopies = kKeys / 32;
 };
 
@@ -97,7 +98,7 @@ decode_wide_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
     float2* ml = reinterpret_cast<float2*>(smem + Cfg::kOffMl);         // [group][row]
     uint32_t s_at = 0, done_at = 0, o_at = 0, q_at = 0;  // parities at the start of the item; s_at: a bit a region
     int loaded = 0;  // tiles of the items before
-    constexpr float room = std::is_same_v<T, __half> ? Cfg::kRoom : 0.f;
+    constexpr int kRoom = std::is_same_v<T, __half> ? Cfg::kRoom : 0;
     while (walk.next(p, kv_head, row_tile, t0, t1)) {
       const int n = t1 - t0, r = row_tile * Cfg::kRows + in_tile % copy_rows;
       const int t = r / p.group, head = kv_head * p.group + r % p.group;
@@ -168,8 +169,8 @@ decode_wide_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
               top = fmaxf(top, fmaxf(a, b));
             }
           }
-          if (__any_sync(0xffffffffu, top > m + Cfg::kLazy)) {
-            const float alpha = top > m ? ex2_approx(m - top) : 1.f;
+          if (__any_sync(0xffffffffu, top - m > Cfg::kLazy)) {  // (the difference is exact where a sum would be rounded)
+            const float alpha = top > m ? ex2_approx(reference_of<kRoom>(m) - reference_of<kRoom>(top)) : 1.f;
             m = fmaxf(m, top);
             l *= alpha;
             if (i >= 2) {
@@ -189,7 +190,7 @@ decode_wide_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
               }
             }
           }
-          const float off = m == -INFINITY ? 0.f : m - room;
+          const float off = m == -INFINITY ? 0.f : reference_of<kRoom>(m);
 #pragma unroll 1
           for (int chunk = 0; chunk < chunks; chunk += kKept) {
 #pragma unroll
@@ -229,7 +230,7 @@ decode_wide_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
       const long long out_row = (static_cast<long long>(walk.b) * p.q_heads + head) * p.cache.tokens + t;
       const long long part = (2ll * blockIdx.x + (t0 == 0 ? 1 : 0)) * p.part_rows + in_tile % copy_rows;
       // ---- the parts of both groups and of all copies joined ----
-      ml[group * Cfg::kRows + in_tile] = make_float2(m - room, l);  // what the sum and O were taken against
+      ml[group * Cfg::kRows + in_tile] = make_float2(reference_of<kRoom>(m), l);  // what the sum and O were taken against
       if (n > 0) {
         ok &= mbar_wait(o_full, o_at, abort_flag);
         o_at ^= 1;

@@ -69,3 +69,29 @@ def test_a_dominating_key_whose_neighbour_row_moves(pkg, head_dim, dtype):
         bound = eps * (want.abs() + minor) + 2.0 ** -13 * size.sum(0)
         err = (out[:, rows, 0] - want).abs()
         assert (err <= bound).all(), (dim, float((err / bound).max()))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("head_dim", [64, 128])
+@pytest.mark.parametrize("rows", [1, 128, 300])
+@pytest.mark.parametrize("power", [20, 24.9, 25.3, 26, 26.6, 27, 27.5, 28, 31])
+def test_scores_so_large_that_steps_of_fp32_are(pkg, rows, head_dim, dtype, power):
+    """Scores of 2^20 to 2^31 (log2 units), where fp32 has steps of up to 256: keys with the largest share the weight, evenly,
+    in one tile and across tiles, also where the maximum has grown from a key one step below."""
+    n = 1 << 14
+    keys, values = torch.zeros((n, head_dim)), torch.randn((n, head_dim), generator=torch.Generator().manual_seed(5)).to(dtype)
+    top = [5, 9, 4000, 4001, 9000, 16000]
+    keys[:, 0] = -8.0
+    keys[2, 0] = 8.0 - 2.0 ** -4 if dtype == torch.bfloat16 else 8.0 - 2.0 ** -7
+    keys[top, 0] = 8.0
+    q = torch.zeros((4, rows, 1, head_dim))
+    q[..., 0] = 8.0
+    args = one_sequence_many_times(keys.to(dtype), values, 4)
+    scale = 2.0 ** power / 64 * math.log(2.0)
+    out, lse = (x.cpu() for x in pkg.attention_decode(q.to(dtype).cuda(), *args, softmax_scale=scale, return_lse=True))
+    pkg.check(torch.cuda.current_stream().cuda_stream)
+    want = values[top].double().mean(0)
+    # P of the six is 1, 2^7 or 2^14; the output is rounded, and the join divides in fp32
+    bound = torch.finfo(dtype).eps / 2 * want.abs() + 2.0 ** -20 * values[top].double().abs().mean(0)
+    assert ((out.double() - want).abs() <= bound).all()
+    assert float((lse.double() / (2.0 ** power * math.log(2.0)) - 1).abs().max()) <= 2.0 ** -15

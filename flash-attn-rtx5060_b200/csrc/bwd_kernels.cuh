@@ -130,8 +130,8 @@ struct BwdCfg {
   static constexpr int kOffBars = kOffUnits + kStats * 128;
   static constexpr int kNumBars = 2 * (kFirst + kSecond + kStats) + 10;
   static constexpr int kSmemBytes = kOffBars + kNumBars * 8 + 24;
-  // kOwnRows: delta and |dO_i|^2 of all rows, 16 warps' three norms and a barrier. At head_dim 128, where there is no other room, they lie in
-  // the first ring's third slot, which the single tile of 128 rows does not reach.
+  // kOwnRows: delta and |dO_i|^2 of all rows, 16 warps' three norms and a barrier. At head_dim 128, where there is no other room,
+  // they lie in the first ring's third slot, which the single tile of 128 rows does not reach.
   static constexpr int kMaxOwnRows = 16384 / D;
   static constexpr int kOffOwnRows = D == 128 ? kOffFirst + 2 * kTileBytes : (kSmemBytes + 15) / 16 * 16;
   static constexpr int kOwnRowsBytes = kMaxOwnRows * 8 + 16 * 3 * 4 + 8;

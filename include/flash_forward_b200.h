@@ -117,7 +117,8 @@ int flash_forward_dropout(const void* q, const void* k, const void* v, void* o, 
  * 16-byte aligned; dq, dk, dv and the workspace overlap neither the inputs nor one another (FA_INVALID_ARG). Scale, causal
  * flag, windows and alibi_slopes (NULL: no bias) are those of the forward call; dropout has no backward pass here.
  *   lse, d_lse   float [batch][heads][seqlen]; d_lse is the gradient of the log-sum-exp, NULL for none (it is needed where
- *                the outputs over disjoint key ranges were merged by it)
+ *                the outputs over disjoint key ranges were merged by it). P is as exact as lse is as a float, a factor within
+ *                2^-20 |lse| of 1; scores beyond 2^20 have no useful gradient
  * P and dS are rounded to fp16 for the tensor cores, scaled by powers of two: for dQ every row by its own sizes, for dK and dV 128
  * keys by those of the queries that see them, so that neither long rows nor small or large gradients cost precision. (In dK a
  * query far larger than the others of its keys, by 2^16 and more, costs theirs.) All sums are fp32. dK, dV and dQ are summed in
